@@ -1,0 +1,99 @@
+// A step of several drafted tokens over the paged cache: what its append, its attention and the keeping of the accepted path share.
+// Sequence b has n nodes, the rows behind its cached tokens; parents[t] < t is the node that node t follows, -1 for the cached tokens.
+#pragma once
+#include "common.cuh"
+
+namespace grl {
+
+// Device status word, kind 6: a sequence whose numbers do not fit ([1] = what, [2] = sequence, [3] = the number).
+enum { TREE_BAD_PARENT = 1, TREE_BAD_COUNT = 2, TREE_BAD_LENGTH = 3, TREE_BAD_PAGE = 4, TREE_BAD_PATH = 5 };
+
+int check_tree_layout(const grl_kv_layout& kv);
+inline int pool_pages(const grl_kv_layout& kv) { return kv.num_pages > 0 ? kv.num_pages : kv.batch * kv.max_pages; }
+
+// ---- tree attention
+struct TreeArgs {
+    const void* k_pages;
+    const void* v_pages;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    const void* q;
+    void* out;
+    const int32_t* parents;
+    const int32_t* n_nodes;
+    float* part;            // [split][ O (rows, D) | (m, l) (rows) ], rows = (sequence, kv head, node, head of the group); m in the exp2 domain
+    int32_t* status;
+    int B, Hq, Hkv, G, T, R, D, P, max_pages, num_pages, n_splits;      // R = T * G rows of a (sequence, kv head)
+    float scale_log2;
+    long long wait_limit;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void tree_fail(int32_t* status, int what, int b, int value) {
+    if (status && atomicCAS(status, 0, GRL_ERR_INVALID) == 0) {
+        status[1] = (6 << 28) | what;
+        status[2] = b;
+        status[3] = value;
+    }
+}
+__device__ __forceinline__ int tree_count(const int32_t* n_nodes, int T, int b) { return n_nodes ? n_nodes[b] : T; }
+// Nodes of a sequence and the cached tokens ahead of them, where seq_lens counts both; -1 (and the status word) where they do not fit.
+__device__ __forceinline__ int tree_nodes(const TreeArgs& a, int b, int* prefix, bool tell) {
+    const int n = tree_count(a.n_nodes, a.T, b), len = a.seq_lens[b];
+    *prefix = len - n;
+    if (n < 0 || n > a.T) {
+        if (tell) tree_fail(a.status, TREE_BAD_COUNT, b, n);
+        return -1;
+    }
+    if (len < n || len > a.max_pages * a.P) {
+        if (tell) tree_fail(a.status, TREE_BAD_LENGTH, b, len);
+        return -1;
+    }
+    return n;
+}
+
+// Ancestors of the first n <= GRL_MAX_TREE nodes, each one's own bit among them, by doubling: after round i a node knows 2^i generations.
+struct TreeMasks {
+    uint4 seen[GRL_MAX_TREE];
+    int up[GRL_MAX_TREE];
+};
+__device__ __forceinline__ uint4 low_bits(int n) {      // bits 0 .. n-1 of 128
+    const auto word = [n](int w) { const int k = n - 32 * w; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
+    return make_uint4(word(0), word(1), word(2), word(3));
+}
+// The whole CTA (at least GRL_MAX_TREE threads) calls it; returns whether the parents are a tree.
+__device__ __forceinline__ bool tree_masks(TreeMasks& m, const int32_t* parents, int n) {
+    const int t = threadIdx.x;
+    if (!parents) {
+        if (t < n) m.seen[t] = low_bits(t + 1);
+        __syncthreads();
+        return true;
+    }
+    int p = t < n ? parents[t] : -1;
+    const bool bad = t < n && (p < -1 || p >= t);
+    if (bad) p = -1;
+    uint4 own = make_uint4(0u, 0u, 0u, 0u);
+    if (t < n) {
+        const uint32_t bit = 1u << (t & 31);
+        own = make_uint4(t >> 5 == 0 ? bit : 0u, t >> 5 == 1 ? bit : 0u, t >> 5 == 2 ? bit : 0u, t >> 5 == 3 ? bit : 0u);
+        m.seen[t] = own;
+        m.up[t] = p;
+    }
+    if (__syncthreads_or(bad)) return false;
+    while (__syncthreads_or(p >= 0)) {
+        int next = -1;
+        if (p >= 0) {
+            const uint4 s = m.seen[p];
+            own = make_uint4(own.x | s.x, own.y | s.y, own.z | s.z, own.w | s.w);
+            next = m.up[p];
+        }
+        __syncthreads();
+        if (t < n) { m.seen[t] = own; m.up[t] = next; }
+        p = next;
+    }
+    return true;
+}
+__device__ __forceinline__ int mask_depth(const uint4 m) { return __popc(m.x) + __popc(m.y) + __popc(m.z) + __popc(m.w) - 1; }
+#endif
+
+}  // namespace grl

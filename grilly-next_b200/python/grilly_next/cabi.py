@@ -13,7 +13,8 @@ F32, BF16, FP8_INT4 = 0, 1, 2
 ROPE_NONE, ROPE_INTERLEAVED, ROPE_HALF = 0, 1, 2
 MASK_NONE, MASK_KEY, MASK_BSS, MASK_BHSS = 0, 1, 2, 3
 KERNEL_AUTO, KERNEL_SIMT_F32, KERNEL_TCGEN05, KERNEL_SIMT_F32_WIDE = 0, 1, 2, 3
-ERR_TIMEOUT = -4
+ERR_INVALID, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_KERNEL = -1, -3, -4, -6
+MAX_TREE = 128
 
 # every symbol that include/grilly_cuda.h declares
 SYMBOLS = [
@@ -30,6 +31,8 @@ SYMBOLS = [
     "grl_rope_table_prepare", "grl_group_unique_id", "grl_group_init_rank", "grl_group_info", "grl_group_allgather",
     "grl_linear", "grl_gemm_f32", "grl_mla_concat", "grl_mla_split", "grl_group_allreduce_max_f64", "grl_group_allgather_merge", "grl_group_sync", "grl_group_destroy",
     "grl_attention_scores", "grl_softmax", "grl_attention_output", "grl_attention_backward",
+    "grl_qk_norm_rope", "grl_qk_norm_rope_backward_workspace_bytes", "grl_qk_norm_rope_backward", "grl_kv_append_norm",
+    "grl_tree_workspace_bytes", "grl_tree_attention", "grl_kv_commit",
 ]
 
 
@@ -82,6 +85,49 @@ class DecodeParams(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("partial_out", C.c_void_p),
                 ("force_simt", C.c_int32), ("scores_out", C.c_void_p), ("scores_ld", C.c_int32),
                 ("exchange", C.POINTER(ExchangeParams))]
+
+
+class RopeSpec(C.Structure):
+    _fields_ = [("mode", C.c_int32), ("rotary_dim", C.c_int32), ("theta", C.c_float), ("scaling", C.c_float),
+                ("gain", C.c_float), ("inv_freq", C.c_void_p)]
+
+
+class QKNormParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("in_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("batch", C.c_int32), ("seq_len", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32),
+                ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3),
+                ("q_out_strides", C.c_int64 * 3), ("k_out_strides", C.c_int64 * 3),
+                ("eps", C.c_float), ("rope", RopeSpec), ("positions", C.c_void_p), ("pos_base", C.c_int32)]
+
+
+class QKNormGradParams(C.Structure):
+    _fields_ = [("fwd", QKNormParams), ("q_out_grad", C.c_void_p), ("k_out_grad", C.c_void_p),
+                ("q_grad", C.c_void_p), ("k_grad", C.c_void_p), ("q_weight_grad", C.c_void_p), ("k_weight_grad", C.c_void_p),
+                ("q_grad_strides", C.c_int64 * 3), ("k_grad_strides", C.c_int64 * 3),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class AppendNormParams(C.Structure):
+    _fields_ = [("kv", KVLayout), ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("q_in", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_token_stride", C.c_int64), ("v_token_stride", C.c_int64), ("q_token_stride", C.c_int64),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float),
+                ("in_dtype", C.c_int32), ("q_out_dtype", C.c_int32), ("n_new", C.c_int32), ("num_q_heads", C.c_int32),
+                ("rope", RopeSpec), ("pos_base", C.c_int32), ("update_lens", C.c_int32), ("pos_offsets", C.c_void_p),
+                ("parents", C.c_void_p), ("n_nodes", C.c_void_p)]
+
+
+class TreeParams(C.Structure):
+    _fields_ = [("kv", KVLayout), ("q", C.c_void_p), ("out", C.c_void_p), ("io_dtype", C.c_int32),
+                ("num_q_heads", C.c_int32), ("n_tree", C.c_int32), ("scale", C.c_float),
+                ("parents", C.c_void_p), ("n_nodes", C.c_void_p), ("max_seq_len", C.c_int32), ("n_splits", C.c_int32),
+                ("kernel", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class CommitParams(C.Structure):
+    _fields_ = [("kv", KVLayout), ("path", C.c_void_p), ("n_path", C.c_void_p), ("n_nodes", C.c_void_p),
+                ("max_path", C.c_int32), ("n_tree", C.c_int32), ("lens_out", C.c_void_p), ("meta", C.POINTER(KVMeta))]
 
 
 class GrlError(RuntimeError):
@@ -160,6 +206,13 @@ def lib():
                                   C.c_float, C.c_int, C.c_void_p, C.c_void_p]
         _lib.grl_attention_mask.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                             C.c_float]
+        _lib.grl_qk_norm_rope.argtypes = [C.c_void_p, C.POINTER(QKNormParams)]
+        _lib.grl_qk_norm_rope_backward_workspace_bytes.argtypes = [C.c_void_p, C.POINTER(QKNormGradParams), C.POINTER(C.c_size_t)]
+        _lib.grl_qk_norm_rope_backward.argtypes = [C.c_void_p, C.POINTER(QKNormGradParams)]
+        _lib.grl_kv_append_norm.argtypes = [C.c_void_p, C.POINTER(AppendNormParams)]
+        _lib.grl_tree_workspace_bytes.argtypes = [C.c_void_p, C.POINTER(TreeParams), C.POINTER(C.c_size_t)]
+        _lib.grl_tree_attention.argtypes = [C.c_void_p, C.POINTER(TreeParams)]
+        _lib.grl_kv_commit.argtypes = [C.c_void_p, C.POINTER(CommitParams)]
         _lib.grl_device_open.argtypes = [C.c_int, C.POINTER(C.c_void_p)]
         _lib.grl_device_close.argtypes = [C.c_void_p]
         _lib.grl_device_get_info.argtypes = [C.c_void_p, C.POINTER(DeviceInfo)]

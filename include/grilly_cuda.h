@@ -268,12 +268,146 @@ int grl_attention_backward(grl_device* dev, const float* grad_out, const float* 
                            const float* attn, float* grad_q, float* grad_k, float* grad_v, float* scratch, int batch,
                            int heads, int seq_len, int head_dim, float scale);
 
+/* ---- normalised and rotated heads: for models that normalise every query and key head before the rotation.  No counterpart in
+ * the reference; these entry points stand beside grl_rope, grl_kv_append and grl_attention_backward.
+ *   y = R(pos) (w * x / sqrt(mean(x^2) + eps))     over the head_dim elements x of every (sequence, token, head)
+ * The rotation R turns the first rotary_dim elements of a head (pairs as GRL_ROPE_INTERLEAVED or GRL_ROPE_HALF over those) and
+ * leaves the others as they are.  Its frequencies are theta^(-2j/rotary_dim) / scaling, or given; cosine and sine are multiplied by gain
+ * (the attention factor of some long-context scalings).  Angles are formed in double from the int32 position.  Everything is
+ * computed in float32 and rounded once. */
+typedef struct {
+    int32_t mode;           /* GRL_ROPE_* */
+    int32_t rotary_dim;     /* even, at most head_dim; 0 is read as head_dim */
+    float theta;            /* base, e.g. 10000; not read where inv_freq is given */
+    float scaling;          /* positions are divided by it; 0 is read as 1; not read where inv_freq is given */
+    float gain;             /* 0 is read as 1 */
+    const float* inv_freq;  /* optional device float32[rotary_dim / 2] */
+} grl_rope_spec;
+
+/* q: (B,S,Hq,D), k: (B,S,Hkv,D) in index order; strides are in elements, of (sequence, token, head), D is contiguous; three
+ * zeros are read as contiguous (B,S,H,D).  So (B,H,S,D) memory, as grl_flash_fwd takes it, and the parts of one packed
+ * projection are served in place.  Results must not overlap one another; q_out may be q (k_out may be k) where strides and
+ * types are the same.  k may be NULL: queries only. */
+typedef struct {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const float* q_weight;      /* float32[head_dim], or NULL for ones */
+    const float* k_weight;
+    int32_t in_dtype;           /* GRL_F32 or GRL_BF16 */
+    int32_t out_dtype;
+    int32_t batch, seq_len, num_q_heads, num_kv_heads, head_dim;    /* head_dim even, at most 256 */
+    int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+    float eps;                  /* 0 is read as 1e-6 */
+    grl_rope_spec rope;
+    const int32_t* positions;   /* optional device int32 (B,S); NULL: token s of a sequence stands at s */
+    int32_t pos_base;           /* added to every position */
+} grl_qk_norm_params;
+int grl_qk_norm_rope(grl_device* dev, const grl_qk_norm_params* p);
+
+/* Gradients of grl_qk_norm_rope: of its inputs (in_dtype) and of its weights (float32, summed over all tokens and heads, written,
+ * not added to).  fwd holds the forward call; its q_out and k_out are not read, q_out_grad and k_out_grad (out_dtype) lie at its
+ * q_out_strides and k_out_strides.  The normalisation is formed again from the inputs.  The same inputs give the same bits.
+ * A call needs a workspace where it is asked for a weight gradient. */
+typedef struct {
+    grl_qk_norm_params fwd;
+    const void* q_out_grad;
+    const void* k_out_grad;
+    void* q_grad;
+    void* k_grad;
+    float* q_weight_grad;       /* float32[head_dim], or NULL */
+    float* k_weight_grad;
+    int64_t q_grad_strides[3], k_grad_strides[3];
+    void* workspace;
+    size_t workspace_bytes;     /* >= grl_qk_norm_rope_backward_workspace_bytes() */
+} grl_qk_norm_grad_params;
+int grl_qk_norm_rope_backward_workspace_bytes(grl_device* dev, const grl_qk_norm_grad_params* p, size_t* bytes);
+int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p);
+
+/* ---- a step of several drafted tokens.  Every sequence brings up to n_new (n_tree) nodes; sequence b has n_nodes[b] of them (NULL:
+ * all), nodes past that are padding.  parents[b][t] is the node that node t follows, below t, or -1 for one that follows the
+ * cached tokens; parents NULL is a chain (node t follows t - 1).  Trees have at most GRL_MAX_TREE nodes, chains of an append any number.
+ *   grl_kv_append_norm   normalises and rotates the nodes' keys and queries at position  cached tokens + depth  and stores keys and
+ *                        values behind the cached tokens, in node order
+ *   grl_tree_attention   a node attends to the cached tokens, its ancestors and itself
+ *   grl_kv_commit        the rows of the accepted path close up behind the cached tokens, the others are dropped
+ * A sequence whose numbers do not fit (a parent that is no earlier node, more nodes than n_new, a length past the block table, a page
+ * outside the pool, a path that does not ascend) is left as it is (attention: its rows are written as 0) and the next
+ * grl_sync returns GRL_ERR_KERNEL.  bf16 and float32 caches; GRL_FP8_INT4 is refused (GRL_ERR_UNSUPPORTED). */
+#define GRL_MAX_TREE 128
+/* k_new, v_new (B,n_new,Hkv,D), q_in, q_out (B,n_new,Hq,D); the token strides (elements, 0 is read as H*D; of a sequence n_new
+ * times that) let the parts of one packed projection be read in place; q_out is contiguous.  Rows of q_out past a sequence's nodes
+ * are written as 0.  seq_lens[b] counts the tokens ahead of the step; update_lens != 0 adds n_nodes[b] afterwards.  The node at depth d
+ * stands at position pos_base + pos_offsets[b] + seq_lens[b] + d.  q_in may be NULL: keys and values only. */
+typedef struct {
+    grl_kv_layout kv;
+    const void* k_new;
+    const void* v_new;
+    const void* q_in;
+    void* q_out;
+    int64_t k_token_stride, v_token_stride, q_token_stride;
+    const float* q_weight;      /* float32[head_dim], or NULL for ones */
+    const float* k_weight;
+    float eps;                  /* 0 is read as 1e-6 */
+    int32_t in_dtype;           /* of k_new, v_new and q_in: GRL_F32 or GRL_BF16 */
+    int32_t q_out_dtype;
+    int32_t n_new, num_q_heads;
+    grl_rope_spec rope;
+    int32_t pos_base;
+    int32_t update_lens;
+    const int32_t* pos_offsets; /* optional device int32[B], as in grl_append_params */
+    const int32_t* parents;     /* optional device int32 (B,n_new) */
+    const int32_t* n_nodes;     /* optional device int32[B] */
+} grl_append_norm_params;
+int grl_kv_append_norm(grl_device* dev, const grl_append_norm_params* p);
+
+/* q, out: (B,n_tree,Hq,D) contiguous, io_dtype, already rotated; kv.seq_lens[b] counts the cached tokens AND the step's nodes, which
+ * are its last n_nodes[b] rows.  Rows of out past a sequence's nodes are written as 0.  head_dim 32, 64, 128 or 256.  bf16 queries over a bf16
+ * cache (head_dim 64 or 128, pages of 64, 32 or 16 tokens) run on the tensor cores, where probabilities are rounded to bf16;
+ * everything else is computed in float32.
+ * What a row must not see does not touch its result: rows past a sequence's end and nodes of other branches may hold anything. */
+typedef struct {
+    grl_kv_layout kv;
+    const void* q;
+    void* out;
+    int32_t io_dtype;           /* of q and out: GRL_F32 or GRL_BF16 */
+    int32_t num_q_heads;
+    int32_t n_tree;
+    float scale;                /* 0 => 1/sqrt(D) */
+    const int32_t* parents;
+    const int32_t* n_nodes;
+    int32_t max_seq_len;        /* upper bound of seq_lens (host knowledge; sizes the split); 0: the block table's capacity */
+    int32_t n_splits;           /* 0 => chosen */
+    int32_t kernel;             /* GRL_KERNEL_AUTO, _SIMT_F32 (float32 arithmetic) or _TCGEN05 (tensor cores, refused where they do not apply) */
+    void* workspace;            /* >= grl_tree_workspace_bytes(); calls that overlap on the GPU need one each */
+    size_t workspace_bytes;
+} grl_tree_params;
+int grl_tree_workspace_bytes(grl_device* dev, const grl_tree_params* p, size_t* bytes);
+int grl_tree_attention(grl_device* dev, const grl_tree_params* p);
+
+/* path (B,max_path): the accepted nodes of every sequence, ascending, the first n_path[b] entries (at most n_nodes[b], 0 keeps none).  Row
+ * seq_lens[b] - n_nodes[b] + path[b][i] moves to seq_lens[b] - n_nodes[b] + i, keys and values, and the length becomes
+ * seq_lens[b] - n_nodes[b] + n_path[b].  It is written to lens_out, or to kv.seq_lens where that is NULL.  meta: optional, the
+ * eviction metadata of the cache: the entries of the accepted nodes move with them, those of the dropped ones are cleared. */
+struct grl_kv_meta_s;
+typedef struct {
+    grl_kv_layout kv;
+    const int32_t* path;
+    const int32_t* n_path;      /* device int32[B] */
+    const int32_t* n_nodes;     /* optional device int32[B]; NULL: n_tree each */
+    int32_t max_path, n_tree;
+    int32_t* lens_out;
+    const struct grl_kv_meta_s* meta;
+} grl_commit_params;
+int grl_kv_commit(grl_device* dev, const grl_commit_params* p);
+
 /* ---- eviction on the paged cache: replaces the host loops of kvCacheEvictH2O
  * (cpp/src/ops/kv_cache.cpp:595-634), the untrained-head branch of kvCacheEvictSpeculative (:905-929)
  * and kvCacheCompact (:941-992; signatures kv_cache.h:186-229).  The reference's TokenMeta array
  * (kv_cache.h:68-73) becomes device arrays, one entry per token slot of every sequence; all-zero is
  * the state of a fresh cache, and appended tokens need no initialisation. */
-typedef struct {
+typedef struct grl_kv_meta_s {
     float* cum_score;     /* [B][capacity] attention mass received so far (TokenMeta.cumulativeScore) */
     uint8_t* tombstone;   /* [B][capacity] 1 = evicted, awaiting compaction (nextActive == UINT32_MAX-1) */
     float* relevance;     /* [B][capacity] TokenMeta.predictedRelevance; may be NULL */
