@@ -22,11 +22,14 @@ struct TreeArgs {
     const int32_t* parents;
     const int32_t* n_nodes;
     float* part;            // [split][ O (rows, D) | (m, l) (rows) ], rows = (sequence, kv head, node, head of the group); m in the exp2 domain
+    size_t part_stride;     // floats of a split, rows * (D + 2) rounded up to 16 bytes
     int32_t* status;
     int B, Hq, Hkv, G, T, R, D, P, max_pages, num_pages, n_splits;      // R = T * G rows of a (sequence, kv head)
     float scale_log2;
     long long wait_limit;
 };
+
+inline size_t tree_part_stride(size_t rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }
 
 #ifdef __CUDACC__
 __device__ __forceinline__ void tree_fail(int32_t* status, int what, int b, int value) {

@@ -4,6 +4,8 @@
 
 namespace grl {
 
+int tree_sm100_launch(grl_device* dev, const TreeArgs& a);
+
 constexpr int kTreeKeys = 32;       // keys of a tile of the float32 kernel
 constexpr int kTreeRows = 8;        // rows of a CTA of it, a warp each
 
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(32 * kTreeRows) tree_rows_kernel(const __grid_
         return;
     }
     const size_t rows = (size_t)a.B * a.Hkv * a.R, row = ((size_t)b * a.Hkv + kvh) * a.R + r;
-    float* part = a.part + (size_t)split * rows * (D + 2);
+    float* part = a.part + split * a.part_stride;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) part[row * D + lane + 32 * i] = acc[i];
     if (lane == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * row) = make_float2(m, l);
@@ -116,14 +118,16 @@ __global__ void __launch_bounds__(32 * kTreeRows) tree_rows_kernel(const __grid_
 // A warp a row: the splits' sums at their common maximum.
 template <typename TIO>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeArgs a) {
-    const size_t rows = (size_t)a.B * a.Hkv * a.R, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5), stride = rows * (a.D + 2);
+    const size_t rows = (size_t)a.B * a.Hkv * a.R, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5), stride = a.part_stride;
     const int lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
     if (row >= rows) return;
     const float* ml = a.part + rows * a.D + 2 * row;
     float m = -INFINITY;
     for (int s = lane; s < a.n_splits; s += 32) {
         const float2 v = *reinterpret_cast<const float2*>(ml + s * stride);
-        if (v.y > 0.f) m = fmaxf(m, v.x);
+        if (v.y != 0.f) m = fmaxf(m, v.x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     for (int s = 0; s < a.n_splits; ++s) {
         const float2 v = *reinterpret_cast<const float2*>(ml + s * stride);
-        if (!(v.y > 0.f)) continue;
+        if (v.y == 0.f) continue;       // saw nothing: its O is not written
         const float w = exp2f(v.x - m);
         l = fmaf(w, v.y, l);
         const float* o = a.part + s * stride + row * a.D;
@@ -143,7 +147,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     const int r = (int)(row % a.R), kvh = (int)(row / a.R % a.Hkv);
     const size_t b = row / a.R / a.Hkv;
     TIO* out = reinterpret_cast<TIO*>(a.out) + ((b * a.T + r / a.G) * a.Hq + kvh * a.G + r % a.G) * a.D;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (lane + 32 * i < a.D) store_from_float<TIO>(out + lane + 32 * i, acc[i] * inv);
@@ -186,6 +190,13 @@ int check_tree_layout(const grl_kv_layout& kv) {
     return GRL_OK;
 }
 
+static bool tensor_cores_apply(const grl_tree_params* p) {
+    const grl_kv_layout& kv = p->kv;
+    return kv.cache_dtype == GRL_BF16 && p->io_dtype == GRL_BF16 && (kv.head_dim == 128 || kv.head_dim == 64) &&
+           (kv.page_tokens == 64 || kv.page_tokens == 32 || kv.page_tokens == 16) &&
+           (long long)pool_pages(kv) * kv.num_kv_heads * kv.page_tokens < (1LL << 31);
+}
+
 static int check_tree(const grl_tree_params* p) {
     GRL_REQUIRE(p, "params is NULL");
     const grl_kv_layout& kv = p->kv;
@@ -201,7 +212,8 @@ static int check_tree(const grl_tree_params* p) {
     GRL_REQUIRE(p->kernel == GRL_KERNEL_AUTO || p->kernel == GRL_KERNEL_SIMT_F32 || p->kernel == GRL_KERNEL_TCGEN05, "unknown kernel");
     if (kv.head_dim != 32 && kv.head_dim != 64 && kv.head_dim != 128 && kv.head_dim != 256)
         return set_error(GRL_ERR_UNSUPPORTED, "head_dim %d not supported (32, 64, 128 or 256)", kv.head_dim);
-    if (p->kernel == GRL_KERNEL_TCGEN05) return set_error(GRL_ERR_UNSUPPORTED, "tree attention runs in float32 arithmetic only");
+    if (p->kernel == GRL_KERNEL_TCGEN05 && !tensor_cores_apply(p))
+        return set_error(GRL_ERR_UNSUPPORTED, "the tensor-core kernel takes bf16 queries over a bf16 cache, head_dim 128 or 64, pages of 64, 32 or 16 tokens");
     GRL_REQUIRE((uintptr_t)kv.k_pages % 16 == 0 && (uintptr_t)kv.v_pages % 16 == 0, "page pools must be 16-byte aligned");
     GRL_REQUIRE((uintptr_t)p->q % 16 == 0 && (uintptr_t)p->out % 16 == 0, "q and out must be 16-byte aligned");
     const long long chunks = ((long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads) + kTreeRows - 1) / kTreeRows;
@@ -209,19 +221,26 @@ static int check_tree(const grl_tree_params* p) {
     return GRL_OK;
 }
 
-// Two CTAs an SM, every split at least four tiles.
-static int tree_splits(const grl_device* dev, const grl_tree_params* p) {
+struct TreePlan {
+    bool tensor;
+    int splits;
+};
+static TreePlan tree_plan(const grl_device* dev, const grl_tree_params* p) {
     const grl_kv_layout& kv = p->kv;
     const int cap = kv.max_pages * kv.page_tokens, longest = p->max_seq_len > 0 && p->max_seq_len < cap ? p->max_seq_len : cap;
-    if (p->n_splits > 0) return p->n_splits;
-    const long long R = (long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads), ctas = kv.batch * kv.num_kv_heads * ((R + kTreeRows - 1) / kTreeRows);
-    long long s = 4LL * dev->prop.multiProcessorCount / ctas, most = longest / (4 * kTreeKeys);
+    const long long R = (long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads), heads = (long long)kv.batch * kv.num_kv_heads;
+    TreePlan t;
+    t.tensor = p->kernel != GRL_KERNEL_SIMT_F32 && tensor_cores_apply(p);
+    // tensor cores: one CTA an SM, every split at least two stages; float32: some four CTAs an SM, every split at least four tiles
+    const long long ctas = heads * (t.tensor ? (R > 128 ? (R + 255) / 256 : 1) : (R + kTreeRows - 1) / kTreeRows);
+    long long s = (t.tensor ? 1LL : 4LL) * dev->prop.multiProcessorCount / ctas, most = longest / (4 * kTreeKeys);
     if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    t.splits = p->n_splits > 0 ? p->n_splits : (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    return t;
 }
 
 static size_t tree_workspace(const grl_tree_params* p, int splits) {
-    return splits == 1 ? 0 : sizeof(float) * (size_t)splits * p->kv.batch * p->n_tree * p->num_q_heads * (p->kv.head_dim + 2);
+    return splits == 1 ? 0 : sizeof(float) * splits * tree_part_stride((size_t)p->kv.batch * p->n_tree * p->num_q_heads, p->kv.head_dim);
 }
 
 }  // namespace grl
@@ -234,7 +253,7 @@ int grl_tree_workspace_bytes(grl_device* dev, const grl_tree_params* p, size_t* 
     int rc = check_tree(p);
     if (rc) return rc;
     GRL_REQUIRE(dev && bytes, "NULL argument");
-    *bytes = tree_workspace(p, tree_splits(dev, p));
+    *bytes = tree_workspace(p, tree_plan(dev, p).splits);
     return GRL_OK;
 }
 
@@ -250,20 +269,23 @@ int grl_tree_attention(grl_device* dev, const grl_tree_params* p) {
     a.D = kv.head_dim; a.P = kv.page_tokens; a.max_pages = kv.max_pages; a.num_pages = pool_pages(kv);
     a.scale_log2 = (p->scale == 0.f ? 1.f / sqrtf((float)a.D) : p->scale) * 1.4426950408889634f;
     a.wait_limit = dev->wait_limit_cycles;
-    a.n_splits = tree_splits(dev, p);
+    const TreePlan plan = tree_plan(dev, p);
+    a.n_splits = plan.splits;
     const size_t need = tree_workspace(p, a.n_splits);
     GRL_REQUIRE(!need || (p->workspace && p->workspace_bytes >= need), "tree attention workspace too small: %zu < %zu",
                 p->workspace ? p->workspace_bytes : 0, need);
     GRL_REQUIRE((uintptr_t)p->workspace % 16 == 0, "workspace must be 16-byte aligned");
     a.part = static_cast<float*>(p->workspace);
+    a.part_stride = tree_part_stride((size_t)a.B * a.Hkv * a.R, a.D);
     DeviceGuard g(dev->ordinal);
     dev->status_dirty = true;
     const bool c32 = kv.cache_dtype == GRL_F32, io32 = p->io_dtype == GRL_F32;
-    rc = io32 ? (c32 ? launch_rows_d<float, float>(dev, a) : launch_rows_d<float, __nv_bfloat16>(dev, a))
-              : (c32 ? launch_rows_d<__nv_bfloat16, float>(dev, a) : launch_rows_d<__nv_bfloat16, __nv_bfloat16>(dev, a));
+    rc = plan.tensor ? tree_sm100_launch(dev, a)
+       : io32 ? (c32 ? launch_rows_d<float, float>(dev, a) : launch_rows_d<float, __nv_bfloat16>(dev, a))
+       : (c32 ? launch_rows_d<__nv_bfloat16, float>(dev, a) : launch_rows_d<__nv_bfloat16, __nv_bfloat16>(dev, a));
     if (rc || a.n_splits == 1) return rc;
     const size_t rows = (size_t)a.B * a.Hkv * a.R;
-    (io32 ? tree_merge_kernel<float> : tree_merge_kernel<__nv_bfloat16>)<<<(unsigned)((rows + 3) / 4), 128, 0, dev->stream>>>(a);
+    GRL_CUDA(launch_pdl(io32 ? tree_merge_kernel<float> : tree_merge_kernel<__nv_bfloat16>, dim3((unsigned)((rows + 3) / 4)), 128, 0, dev->stream, a));
     GRL_LAUNCHED("tree_merge_kernel");
     return GRL_OK;
 }
