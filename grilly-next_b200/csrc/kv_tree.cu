@@ -53,6 +53,8 @@ template <typename TIn, typename TC, typename TQ>
 __global__ void __launch_bounds__(256) append_norm_rows_kernel(const __grid_constant__ AppendNormArgs a) {
     __shared__ TreeMasks masks;
     const int b = blockIdx.y, lane = threadIdx.x & 31, pairs = a.D / 2;
+    pdl_wait();
+    pdl_trigger();
     const int len0 = a.seq_lens[b], n = tree_count(a.n_nodes, a.n_new, b);
     bool ok = append_fits(a, b, len0, n);
     if (ok && a.parents && !tree_masks(masks, a.parents + (size_t)b * a.n_new, n)) {
@@ -118,6 +120,103 @@ __global__ void __launch_bounds__(256) append_norm_rows_kernel(const __grid_cons
     if (a.update_lens && ok) {
         __syncthreads();        // every thread has read the length
         if (threadIdx.x == 0) a.seq_lens[b] = len0 + n;
+    }
+}
+
+// Rows of 32, 64, 128 or 256 elements on 16-byte boundaries: the form of qk_norm_kernel (qk_norm.cu).  A run is kRun heads of the keys, the
+// values or the queries of a node.  A group's first run is on its way while the sequence's numbers are read and checked.
+constexpr int kRun = 4;
+template <typename TIn, typename TC, typename TQ, int LANES, bool HALF>
+__global__ void __launch_bounds__(256) append_norm_kernel(const __grid_constant__ AppendNormArgs a) {
+    __shared__ TreeMasks masks;
+    constexpr int D = 8 * LANES;
+    const int b = blockIdx.y, l = threadIdx.x % LANES;
+    const RowPlace at = row_place<HALF>(l, a.rope.rd);
+    double freq[4];
+    row_freq(a.rope, l, at.turned, freq);
+    const int kv_runs = (a.Hkv + kRun - 1) / kRun, runs = 2 * kv_runs + (a.Hq + kRun - 1) / kRun;
+    const long long total = (long long)a.n_new * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const long long lo = mine * total / all, hi = (mine + 1) * total / all, most = (total + all - 1) / all;
+    float x[kRun][8];
+    int t = 0, kind = 0, h0 = 0, heads = 0;
+    auto fetch = [&](long long item, bool live) {
+        t = (int)(item / runs);
+        const int run = (int)(item - (long long)t * runs);
+        kind = run < kv_runs ? 0 : run < 2 * kv_runs ? 1 : 2;
+        h0 = (run - kind * kv_runs) * kRun;
+        heads = live ? min(kRun, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
+        const TIn* in = reinterpret_cast<const TIn*>(kind == 0 ? a.k_new : kind == 1 ? a.v_new : a.q_in) +
+                        ((size_t)b * a.n_new + t) * (kind == 0 ? a.ks : kind == 1 ? a.vs : a.qs) + (size_t)h0 * D;
+#pragma unroll
+        for (int h = 0; h < kRun; ++h)
+            if (h < heads) row_load<HALF>(in + h * D, at, x[h]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
+            }
+    };
+    pdl_wait();
+    pdl_trigger();
+    fetch(lo < hi ? lo : 0, lo < hi);
+    const int len0 = a.seq_lens[b], n = tree_count(a.n_nodes, a.n_new, b), offset = a.pos_offsets ? a.pos_offsets[b] : 0;
+    bool ok = append_fits(a, b, len0, n);
+    if (ok && a.parents && !tree_masks(masks, a.parents + (size_t)b * a.n_new, n)) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
+        ok = false;
+    }
+    const int nodes = ok ? n : 0, pos0 = a.pos_base + offset + len0;
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    int angles_of = -1;
+    size_t row = 0;         // of the node in the pools, for kv head 0
+    for (long long i = 0; i < most; ++i) {
+        if (i > 0) fetch(lo + i < hi ? lo + i : 0, lo + i < hi);
+        const bool node = t < nodes;
+        if (heads > 0 && node && angles_of != t) {
+            const int slot = len0 + t;
+            row = ((size_t)a.block_table[(size_t)b * a.max_pages + slot / a.P] * a.Hkv * a.P + slot % a.P) * D;
+            row_angles(a.rope, freq, at.turned, pos0 + (a.parents ? mask_depth(masks.seen[t]) : t), c, s);
+            angles_of = t;
+        }
+        const float* weight = kind == 2 ? a.q_weight : a.k_weight;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = weight ? __ldg(weight + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
+#pragma unroll
+        for (int h = 0; h < kRun; ++h) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[h][e], x[h][e], sum);
+            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps);
+            if (h >= heads) continue;
+            if (kind != 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[h][e] = x[h][e] * r * w[e];
+                row_turn<HALF, false>(x[h], c, s, at.turned);
+            }
+            if (kind == 2) {
+                if (!node) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
+                }
+                row_store<HALF>(reinterpret_cast<TQ*>(a.q_out) + (((size_t)b * a.n_new + t) * a.Hq + h0 + h) * D, at, x[h]);
+            } else if (node) {
+                row_store<HALF>(reinterpret_cast<TC*>(kind ? a.v_pages : a.k_pages) + row + (size_t)(h0 + h) * a.P * D, at, x[h]);
+            }
+        }
+    }
+    if (a.update_lens && ok) {
+        __syncthreads();        // every thread has read the length
+        if (threadIdx.x == 0) a.seq_lens[b] = len0 + n;
+    }
+}
+
+template <typename TIn, typename TC, typename TQ>
+static void (*append_lane_instance(int D, bool half))(AppendNormArgs) {
+    switch (D) {
+        case 32: return half ? append_norm_kernel<TIn, TC, TQ, 4, true> : append_norm_kernel<TIn, TC, TQ, 4, false>;
+        case 64: return half ? append_norm_kernel<TIn, TC, TQ, 8, true> : append_norm_kernel<TIn, TC, TQ, 8, false>;
+        case 128: return half ? append_norm_kernel<TIn, TC, TQ, 16, true> : append_norm_kernel<TIn, TC, TQ, 16, false>;
+        default: return half ? append_norm_kernel<TIn, TC, TQ, 32, true> : append_norm_kernel<TIn, TC, TQ, 32, false>;
     }
 }
 
@@ -200,10 +299,14 @@ __global__ void __launch_bounds__(1024) commit_kernel(const __grid_constant__ Co
     if (tid == 0) a.lens_out[b] = prefix + m;
 }
 
+template <typename TIn, typename TC, typename TQ>
+static void (*append_instance(bool fast, int D, bool half))(AppendNormArgs) {
+    return fast ? append_lane_instance<TIn, TC, TQ>(D, half) : append_norm_rows_kernel<TIn, TC, TQ>;
+}
 template <typename TIn>
-static void (*append_norm_instance(bool cache32, bool q32))(AppendNormArgs) {
-    return cache32 ? (q32 ? append_norm_rows_kernel<TIn, float, float> : append_norm_rows_kernel<TIn, float, __nv_bfloat16>)
-                   : (q32 ? append_norm_rows_kernel<TIn, __nv_bfloat16, float> : append_norm_rows_kernel<TIn, __nv_bfloat16, __nv_bfloat16>);
+static void (*append_norm_instance(bool cache32, bool q32, bool fast, int D, bool half))(AppendNormArgs) {
+    return cache32 ? (q32 ? append_instance<TIn, float, float>(fast, D, half) : append_instance<TIn, float, __nv_bfloat16>(fast, D, half))
+                   : (q32 ? append_instance<TIn, __nv_bfloat16, float>(fast, D, half) : append_instance<TIn, __nv_bfloat16, __nv_bfloat16>(fast, D, half));
 }
 
 // seq_lens += nodes of the sequences that the append has taken: it raises no flag of its own, so the conditions are formed again.
@@ -259,15 +362,20 @@ int grl_kv_append_norm(grl_device* dev, const grl_append_norm_params* p) {
     fill_rope_freq(dev, p->rope, &a.rope);
     a.status = dev->d_status;
     dev->status_dirty = true;
-    const long long rows = (long long)a.n_new * (2 * a.Hkv + a.Hq), most = (8LL * dev->prop.multiProcessorCount + a.B - 1) / a.B;
-    int ctas = (int)((rows + 7) / 8 < most ? (rows + 7) / 8 : most);
+    const bool fast = row_lanes_fit(a.D, a.rope.rd) && row_aligned(a.k_new, p->in_dtype, &a.ks, 1) && row_aligned(a.v_new, p->in_dtype, &a.vs, 1) &&
+                      (!a.q_in || row_aligned(a.q_in, p->in_dtype, &a.qs, 1)) &&
+                      ((uintptr_t)a.q_out | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages) % 16 == 0;
+    const long long groups = fast ? 256 / (a.D / 8) : 8, per_node = fast ? 2 * ((a.Hkv + kRun - 1) / kRun) + (a.Hq + kRun - 1) / kRun : 2 * a.Hkv + a.Hq;
+    const long long need = (a.n_new * per_node + groups - 1) / groups, most = ((fast ? 4LL : 8LL) * dev->prop.multiProcessorCount + a.B - 1) / a.B;
+    int ctas = (int)(need < most ? need : most);
     const bool fused = p->update_lens && ctas <= 4;
     if (fused) ctas = 1;
     a.update_lens = fused ? 1 : 0;
-    auto kernel = p->in_dtype == GRL_F32 ? append_norm_instance<float>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32)
-                                         : append_norm_instance<__nv_bfloat16>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32);
-    kernel<<<dim3(ctas, a.B), 256, 0, dev->stream>>>(a);
-    GRL_LAUNCHED("append_norm_rows_kernel");
+    const bool half = p->rope.mode == GRL_ROPE_HALF;
+    auto kernel = p->in_dtype == GRL_F32 ? append_norm_instance<float>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, half)
+                                         : append_norm_instance<__nv_bfloat16>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, half);
+    GRL_CUDA(launch_pdl(kernel, dim3(ctas, a.B), 256, 0, dev->stream, a));
+    GRL_LAUNCHED("append_norm_kernel");
     if (p->update_lens && !fused) {
         advance_nodes_kernel<<<a.B, GRL_MAX_TREE, 0, dev->stream>>>(a);
         GRL_LAUNCHED("advance_nodes_kernel");

@@ -75,6 +75,184 @@ __global__ void __launch_bounds__(256) qk_norm_rows_kernel(const __grid_constant
     }
 }
 
+// Rows of 32, 64, 128 or 256 elements on 16-byte boundaries: LANES threads a row, eight elements each.  Bound by HBM, each element read and
+// written once.  A thread group keeps its places in the rows, walks the heads of a token in runs of kRun rows, whose loads are in
+// flight together, and forms a token's angles (double precision) once for all of them; every group has an equal, contiguous share of all runs.
+constexpr int kRun = 4;
+struct RunPlace {
+    int b, s, h0, heads;
+    bool is_k;
+};
+template <typename A>
+__device__ __forceinline__ RunPlace run_place(const A& a, long long item, int q_runs, int runs) {
+    const long long tok = item / runs;
+    const int r = (int)(item - tok * runs);
+    RunPlace p;
+    p.is_k = r >= q_runs;
+    p.h0 = (p.is_k ? r - q_runs : r) * kRun;
+    p.heads = min(kRun, (p.is_k ? a.k.H : a.q.H) - p.h0);
+    p.b = (int)(tok / a.S);
+    p.s = (int)(tok - (long long)p.b * a.S);
+    return p;
+}
+template <typename TIn, typename TOut, int LANES, bool HALF>
+__global__ void __launch_bounds__(256) qk_norm_kernel(const __grid_constant__ NormArgs a) {
+    const int l = threadIdx.x % LANES, D = 8 * LANES;
+    const RowPlace at = row_place<HALF>(l, a.rope.rd);
+    double freq[4];
+    row_freq(a.rope, l, at.turned, freq);
+    const int q_runs = (a.q.H + kRun - 1) / kRun, runs = q_runs + (a.k.H + kRun - 1) / kRun;
+    const long long total = (long long)a.B * a.S * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const long long lo = mine * total / all, hi = (mine + 1) * total / all;
+    const long long most = (total + all - 1) / all;         // of any group: the warp's groups take the same trips, for the shuffles
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    int angles_b = -1, angles_s = -1;
+    pdl_wait();
+    pdl_trigger();
+    for (long long i = 0; i < most; ++i) {
+        const bool live = lo + i < hi;
+        const RunPlace p = run_place(a, live ? lo + i : 0, q_runs, runs);
+        const NormSide& side = p.is_k ? a.k : a.q;
+        float x[kRun][8];
+        const TIn* in = reinterpret_cast<const TIn*>(side.x) + p.b * side.xs[0] + p.s * side.xs[1] + p.h0 * side.xs[2];
+#pragma unroll
+        for (int h = 0; h < kRun; ++h)
+            if (live && h < p.heads) row_load<HALF>(in + h * side.xs[2], at, x[h]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
+            }
+        if (live && (p.b != angles_b || p.s != angles_s)) {     // under the loads
+            row_angles(a.rope, freq, at.turned, position_of(a, p.b, p.s), c, s);
+            angles_b = p.b;
+            angles_s = p.s;
+        }
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = side.w ? __ldg(side.w + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
+        TOut* out = reinterpret_cast<TOut*>(side.y) + p.b * side.ys[0] + p.s * side.ys[1] + p.h0 * side.ys[2];
+#pragma unroll
+        for (int h = 0; h < kRun; ++h) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[h][e], x[h][e], sum);
+            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[h][e] = x[h][e] * r * w[e];
+            row_turn<HALF, false>(x[h], c, s, at.turned);
+            if (live && h < p.heads) row_store<HALF>(out + h * side.ys[2], at, x[h]);
+        }
+    }
+}
+
+// The backward pass in the same form; a group keeps its shares of both weight gradients in registers, the CTA adds them in order of
+// its groups.
+constexpr int kGradRun = 2;
+template <typename TIn, typename TOut, int LANES, bool HALF>
+__global__ void __launch_bounds__(256) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int D = 8 * LANES, GROUPS = 256 / LANES;
+    __shared__ __align__(16) float sm[GROUPS][D];
+    const int l = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const RowPlace at = row_place<HALF>(l, a.rope.rd);
+    double freq[4];
+    row_freq(a.rope, l, at.turned, freq);
+    const int q_runs = (a.q.H + kGradRun - 1) / kGradRun, runs = q_runs + (a.k.H + kGradRun - 1) / kGradRun;
+    const long long total = (long long)a.B * a.S * runs, all = (long long)gridDim.x * GROUPS, mine = (long long)blockIdx.x * GROUPS + group;
+    const long long lo = mine * total / all, hi = (mine + 1) * total / all, most = (total + all - 1) / all;
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, acc[2][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
+    int angles_b = -1, angles_s = -1;
+    pdl_wait();
+    for (long long i = 0; i < most; ++i) {
+        const bool live = lo + i < hi;
+        const long long item = live ? lo + i : 0, tok = item / runs;
+        const int run = (int)(item - tok * runs), b = (int)(tok / a.S), st = (int)(tok - (long long)b * a.S);
+        const bool is_k = run >= q_runs;
+        const NormSide& side = is_k ? a.k : a.q;
+        const int h0 = (is_k ? run - q_runs : run) * kGradRun, heads = live ? min(kGradRun, side.H - h0) : 0;
+        const TIn* in = reinterpret_cast<const TIn*>(side.x) + b * side.xs[0] + st * side.xs[1] + h0 * side.xs[2];
+        const TOut* dy = reinterpret_cast<const TOut*>(side.dy) + b * side.dys[0] + st * side.dys[1] + h0 * side.dys[2];
+        float x[kGradRun][8], g[kGradRun][8];
+#pragma unroll
+        for (int h = 0; h < kGradRun; ++h)
+            if (h < heads) {
+                row_load<HALF>(in + h * side.xs[2], at, x[h]);
+                row_load<HALF>(dy + h * side.dys[2], at, g[h]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[h][e] = g[h][e] = 0.f;
+            }
+        if (live && (b != angles_b || st != angles_s)) {
+            row_angles(a.rope, freq, at.turned, position_of(a, b, st), c, s);
+            angles_b = b;
+            angles_s = st;
+        }
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = side.w ? __ldg(side.w + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
+        TIn* dx = reinterpret_cast<TIn*>(side.y) + b * side.ys[0] + st * side.ys[1] + h0 * side.ys[2];
+#pragma unroll
+        for (int h = 0; h < kGradRun; ++h) {
+            row_turn<HALF, true>(g[h], c, s, at.turned);
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum = fmaf(x[h][e], x[h][e], sum);
+                dot = fmaf(g[h][e] * w[e], x[h][e], dot);
+            }
+            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps), f = row_sum<LANES>(dot) * (1.f / D) * r * r;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float gx = g[h][e] * (x[h][e] * r);
+                if (is_k) acc[1][e] += gx;
+                else acc[0][e] += gx;
+                x[h][e] = r * (g[h][e] * w[e] - x[h][e] * f);
+            }
+            if (h < heads) row_store<HALF>(dx + h * side.ys[2], at, x[h]);
+        }
+    }
+    pdl_trigger();
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        row_store<HALF>(sm[group], at, acc[i]);
+        __syncthreads();
+        if (threadIdx.x < D) {
+            float sum = 0.f;
+#pragma unroll 8
+            for (int j = 0; j < GROUPS; ++j) sum += sm[j][threadIdx.x];
+            a.part[((size_t)blockIdx.x * 2 + i) * D + threadIdx.x] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+template <typename TIn, typename TOut, bool BACK>
+static void (*lane_instance(int D, bool half))(NormArgs) {
+    if constexpr (BACK) {
+        switch (D) {
+            case 32: return half ? qk_norm_backward_kernel<TIn, TOut, 4, true> : qk_norm_backward_kernel<TIn, TOut, 4, false>;
+            case 64: return half ? qk_norm_backward_kernel<TIn, TOut, 8, true> : qk_norm_backward_kernel<TIn, TOut, 8, false>;
+            case 128: return half ? qk_norm_backward_kernel<TIn, TOut, 16, true> : qk_norm_backward_kernel<TIn, TOut, 16, false>;
+            default: return half ? qk_norm_backward_kernel<TIn, TOut, 32, true> : qk_norm_backward_kernel<TIn, TOut, 32, false>;
+        }
+    } else {
+        switch (D) {
+            case 32: return half ? qk_norm_kernel<TIn, TOut, 4, true> : qk_norm_kernel<TIn, TOut, 4, false>;
+            case 64: return half ? qk_norm_kernel<TIn, TOut, 8, true> : qk_norm_kernel<TIn, TOut, 8, false>;
+            case 128: return half ? qk_norm_kernel<TIn, TOut, 16, true> : qk_norm_kernel<TIn, TOut, 16, false>;
+            default: return half ? qk_norm_kernel<TIn, TOut, 32, true> : qk_norm_kernel<TIn, TOut, 32, false>;
+        }
+    }
+}
+template <bool BACK>
+static void (*instance(const grl_qk_norm_params& f))(NormArgs) {
+    const bool in32 = f.in_dtype == GRL_F32, out32 = f.out_dtype == GRL_F32, half = f.rope.mode == GRL_ROPE_HALF;
+    return in32 ? (out32 ? lane_instance<float, float, BACK>(f.head_dim, half) : lane_instance<float, __nv_bfloat16, BACK>(f.head_dim, half))
+                : (out32 ? lane_instance<__nv_bfloat16, float, BACK>(f.head_dim, half) : lane_instance<__nv_bfloat16, __nv_bfloat16, BACK>(f.head_dim, half));
+}
+
 // Backward, a warp a row:  g = R^T dy,  dw += g * x r,  dx = r (w g - x r^2 mean(w g x)).
 // A warp keeps its share of both weight gradients in registers; the CTA's sum goes to the workspace, and
 // qk_norm_weight_kernel adds the CTAs' in order.
@@ -173,6 +351,8 @@ __global__ void __launch_bounds__(256) qk_norm_rows_backward_kernel(const __grid
 __global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __restrict__ part, int ctas, int D, float* dq, float* dk) {
     __shared__ double sm[32][33];
     float* out = blockIdx.y ? dk : dq;
+    pdl_wait();
+    pdl_trigger();
     if (!out) return;
     const int d = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
     double sum = 0.0;
@@ -306,6 +486,16 @@ int grl_qk_norm_rope(grl_device* dev, const grl_qk_norm_params* p) {
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->rope, &a.rope);
     const long long rows = (long long)a.B * a.S * (a.q.H + a.k.H), most = 8LL * dev->prop.multiProcessorCount;
+    bool fast = row_lanes_fit(a.D, a.rope.rd);
+    for (const NormSide* s : {&a.q, &a.k})
+        if (s->H) fast = fast && row_aligned(s->x, p->in_dtype, s->xs, 3) && row_aligned(s->y, p->out_dtype, s->ys, 3);
+    if (fast) {
+        const long long runs = (long long)a.B * a.S * ((a.q.H + kRun - 1) / kRun + (a.k.H + kRun - 1) / kRun), groups = 256 / (a.D / 8);
+        const long long need = (runs + groups - 1) / groups, held = 4LL * dev->prop.multiProcessorCount;
+        GRL_CUDA(launch_pdl(instance<false>(*p), dim3((unsigned)(need < held ? need : held)), 256, 0, dev->stream, a));
+        GRL_LAUNCHED("qk_norm_kernel");
+        return GRL_OK;
+    }
     const int ctas = (int)((rows + 7) / 8 < most ? (rows + 7) / 8 : most);
     const bool in32 = p->in_dtype == GRL_F32, out32 = p->out_dtype == GRL_F32;
     auto kernel = in32 ? (out32 ? qk_norm_rows_kernel<float, float> : qk_norm_rows_kernel<float, __nv_bfloat16>)
@@ -338,13 +528,20 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
     }
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->fwd.rope, &a.rope);
+    bool fast = row_lanes_fit(a.D, a.rope.rd);
+    for (const NormSide* s : {&a.q, &a.k})
+        if (s->H)
+            fast = fast && row_aligned(s->x, p->fwd.in_dtype, s->xs, 3) && row_aligned(s->y, p->fwd.in_dtype, s->ys, 3) &&
+                   row_aligned(s->dy, p->fwd.out_dtype, s->dys, 3);
     const bool in32 = p->fwd.in_dtype == GRL_F32, out32 = p->fwd.out_dtype == GRL_F32;
-    auto kernel = in32 ? (out32 ? qk_norm_rows_backward_kernel<float, float> : qk_norm_rows_backward_kernel<float, __nv_bfloat16>)
+    auto kernel = fast ? instance<true>(p->fwd)
+                : in32 ? (out32 ? qk_norm_rows_backward_kernel<float, float> : qk_norm_rows_backward_kernel<float, __nv_bfloat16>)
                        : (out32 ? qk_norm_rows_backward_kernel<__nv_bfloat16, float> : qk_norm_rows_backward_kernel<__nv_bfloat16, __nv_bfloat16>);
-    kernel<<<ctas, 256, 0, dev->stream>>>(a);
-    GRL_LAUNCHED("qk_norm_rows_backward_kernel");
+    if (fast) GRL_CUDA(launch_pdl(kernel, dim3(ctas), 256, 0, dev->stream, a));
+    else kernel<<<ctas, 256, 0, dev->stream>>>(a);
+    GRL_LAUNCHED("qk_norm_backward_kernel");
     if (a.part) {
-        qk_norm_weight_kernel<<<dim3((a.D + 31) / 32, 2), 1024, 0, dev->stream>>>(a.part, ctas, a.D, a.q.dw, a.k.dw);
+        GRL_CUDA(launch_pdl(qk_norm_weight_kernel, dim3((a.D + 31) / 32, 2), 1024, 0, dev->stream, (const float*)a.part, ctas, a.D, a.q.dw, a.k.dw));
         GRL_LAUNCHED("qk_norm_weight_kernel");
     }
     return GRL_OK;

@@ -18,6 +18,15 @@ int check_rope_spec(const grl_rope_spec& r, int head_dim, RopeArgs* out);
 // The frequencies of a spec that names none.
 void fill_rope_freq(grl_device* dev, const grl_rope_spec& r, RopeArgs* out);
 
+// Whether rows that start at p and lie `strides` apart serve the eight-element form.
+inline bool row_aligned(const void* p, int dtype, const long long* strides, int n) {
+    const long long unit = 16 / (dtype == GRL_BF16 ? 2 : 4);        // elements of 16 bytes
+    bool ok = (uintptr_t)p % 16 == 0;
+    for (int i = 0; i < n; ++i) ok = ok && strides[i] % unit == 0;
+    return ok;
+}
+inline bool row_lanes_fit(int D, int rd) { return (D == 32 || D == 64 || D == 128 || D == 256) && rd % 8 == 0; }
+
 #ifdef __CUDACC__
 // Element places of pair j of a row: the rotated pairs first, then the elements that are left as they are, in neighbours.
 __device__ __forceinline__ void pair_place(const RopeArgs& r, int j, int* d0, int* d1) {
@@ -31,6 +40,101 @@ __device__ __forceinline__ void pair_angle(const RopeArgs& r, int j, int pos, fl
     rope_sincos(pos, r.inv_freq ? (double)r.inv_freq[j] : r.freq.inv_freq[j], c, s);
     *c *= r.gain;
     *s *= r.gain;
+}
+// ---- rows of D = 8 * LANES elements held by LANES neighbouring threads, eight elements each: x[0..3] at o0 and x[4..7] at o1.  Rotated in
+// halves, element e and e + 4 of a thread are a pair (o1 = o0 + rd / 2); else neighbours are, and o1 = o0 + 4.  The threads behind the
+// rotated part hold the elements that are left as they are.  Needs rd % 8 == 0, and rows on boundaries of four elements
+// (eight where o1 = o0 + 4).
+struct RowPlace {
+    int o0, o1;
+    bool turned;
+};
+template <bool HALF>
+__device__ __forceinline__ RowPlace row_place(int l, int rd) {
+    RowPlace p;
+    p.turned = 8 * l < rd;
+    p.o0 = HALF && p.turned ? 4 * l : 8 * l;
+    p.o1 = HALF && p.turned ? p.o0 + rd / 2 : p.o0 + 4;
+    return p;
+}
+__device__ __forceinline__ void unpack_bf16(uint32_t w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <bool HALF>
+__device__ __forceinline__ void row_load(const float* p, const RowPlace& at, float (&x)[8]) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p + at.o0)), b = __ldcs(reinterpret_cast<const float4*>(p + at.o1));
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <bool HALF>
+__device__ __forceinline__ void row_load(const __nv_bfloat16* p, const RowPlace& at, float (&x)[8]) {
+    uint32_t w[4];
+    if constexpr (HALF) {
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p + at.o0)), b = __ldcs(reinterpret_cast<const uint2*>(p + at.o1));
+        w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+    } else {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + at.o0));
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) unpack_bf16(w[e], x[2 * e], x[2 * e + 1]);
+}
+template <bool HALF>
+__device__ __forceinline__ void row_store(float* p, const RowPlace& at, const float (&y)[8]) {
+    *reinterpret_cast<float4*>(p + at.o0) = make_float4(y[0], y[1], y[2], y[3]);
+    *reinterpret_cast<float4*>(p + at.o1) = make_float4(y[4], y[5], y[6], y[7]);
+}
+template <bool HALF>
+__device__ __forceinline__ void row_store(__nv_bfloat16* p, const RowPlace& at, const float (&y)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(y[2 * e], y[2 * e + 1]);
+    if constexpr (HALF) {
+        *reinterpret_cast<uint2*>(p + at.o0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(p + at.o1) = make_uint2(w[2], w[3]);
+    } else {
+        *reinterpret_cast<uint4*>(p + at.o0) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, LANES);
+    return v;
+}
+// cosine and sine of a thread's four pairs at a position; 1 and 0 where nothing turns
+__device__ __forceinline__ void row_angles(const RopeArgs& r, const double (&freq)[4], bool turned, int pos, float (&c)[4], float (&s)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        c[e] = 1.f;
+        s[e] = 0.f;
+        if (turned) {
+            rope_sincos(pos, freq[e], &c[e], &s[e]);
+            c[e] *= r.gain;
+            s[e] *= r.gain;
+        }
+    }
+}
+__device__ __forceinline__ void row_freq(const RopeArgs& r, int l, bool turned, double (&freq)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) freq[e] = !turned ? 0.0 : r.inv_freq ? (double)r.inv_freq[4 * l + e] : r.freq.inv_freq[4 * l + e];
+}
+// The rotation of a thread's pairs; BACK: its transpose.
+template <bool HALF, bool BACK>
+__device__ __forceinline__ void row_turn(float (&x)[8], const float (&c)[4], const float (&s)[4], bool turned) {
+    if (!turned) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int i = HALF ? e : 2 * e, j = HALF ? e + 4 : 2 * e + 1;
+        const float sn = BACK ? -s[e] : s[e], a = x[i] * c[e] - x[j] * sn, b = x[i] * sn + x[j] * c[e];
+        x[i] = a;
+        x[j] = b;
+    }
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
