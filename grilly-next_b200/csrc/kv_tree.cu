@@ -123,84 +123,94 @@ __global__ void __launch_bounds__(256) append_norm_rows_kernel(const __grid_cons
     }
 }
 
-// Rows of 32, 64, 128 or 256 elements on 16-byte boundaries: the form of qk_norm_kernel (qk_norm.cu).  A run is kRun heads of the keys, the
+// Rows of whole 8-element pieces on 16-byte boundaries: the form of qk_norm_kernel (qk_norm.cu).  A run is kRun heads of the keys, the
 // values or the queries of a node.  A group's first run is on its way while the sequence's numbers are read and checked.
-constexpr int kRun = 4;
+template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;
 template <typename TIn, typename TC, typename TQ, int LANES, bool HALF>
-__global__ void __launch_bounds__(256) append_norm_kernel(const __grid_constant__ AppendNormArgs a) {
+__global__ void __launch_bounds__(256, 3) append_norm_kernel(const __grid_constant__ AppendNormArgs a) {
+    constexpr int RUN = kRunOf<TIn>;
     __shared__ TreeMasks masks;
-    constexpr int D = 8 * LANES;
-    const int b = blockIdx.y, l = threadIdx.x % LANES;
+    __shared__ __align__(16) RowTables tables;
+    const int b = blockIdx.y, l = threadIdx.x % LANES, D = a.D;
+    const bool on = 8 * l < D;
+    const float inv_d = 1.f / D;
     const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    double freq[4];
-    row_freq(a.rope, l, at.turned, freq);
-    const int kv_runs = (a.Hkv + kRun - 1) / kRun, runs = 2 * kv_runs + (a.Hq + kRun - 1) / kRun;
+    const int kv_runs = (a.Hkv + RUN - 1) / RUN, runs = 2 * kv_runs + (a.Hq + RUN - 1) / RUN;
     const long long total = (long long)a.n_new * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const long long lo = mine * total / all, hi = (mine + 1) * total / all, most = (total + all - 1) / all;
-    float x[kRun][8];
-    int t = 0, kind = 0, h0 = 0, heads = 0;
-    auto fetch = [&](long long item, bool live) {
-        t = (int)(item / runs);
-        const int run = (int)(item - (long long)t * runs);
-        kind = run < kv_runs ? 0 : run < 2 * kv_runs ? 1 : 2;
-        h0 = (run - kind * kv_runs) * kRun;
-        heads = live ? min(kRun, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
+    const long long lo = mine * total / all;
+    const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);
+    RowRaw<TIn> raw[RUN];
+    int t = items > 0 ? (int)(lo / runs) : 0, run = items > 0 ? (int)(lo - (long long)t * runs) : 0;
+    auto place = [&](int run, int* h0) {
+        const int kind = run < kv_runs ? 0 : run < 2 * kv_runs ? 1 : 2;
+        *h0 = (run - kind * kv_runs) * RUN;
+        return kind;
+    };
+    auto fetch = [&](int t, int run, bool live) {
+        int h0;
+        const int kind = place(run, &h0), heads = live && on ? min(RUN, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
         const TIn* in = reinterpret_cast<const TIn*>(kind == 0 ? a.k_new : kind == 1 ? a.v_new : a.q_in) +
                         ((size_t)b * a.n_new + t) * (kind == 0 ? a.ks : kind == 1 ? a.vs : a.qs) + (size_t)h0 * D;
 #pragma unroll
-        for (int h = 0; h < kRun; ++h)
-            if (h < heads) row_load<HALF>(in + h * D, at, x[h]);
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
-            }
+        for (int h = 0; h < RUN; ++h)
+            if (h < heads) row_fetch<HALF>(in + h * D, at, raw[h]);
+            else row_zero(raw[h]);
     };
     pdl_wait();
     pdl_trigger();
-    fetch(lo < hi ? lo : 0, lo < hi);
+    fetch(t, run, items > 0);
     const int len0 = a.seq_lens[b], n = tree_count(a.n_nodes, a.n_new, b), offset = a.pos_offsets ? a.pos_offsets[b] : 0;
+    row_tables<HALF>(tables, a.rope, D, a.q_weight, a.k_weight);
     bool ok = append_fits(a, b, len0, n);
     if (ok && a.parents && !tree_masks(masks, a.parents + (size_t)b * a.n_new, n)) {
         if (threadIdx.x == 0 && blockIdx.x == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
         ok = false;
     }
+    __syncthreads();
     const int nodes = ok ? n : 0, pos0 = a.pos_base + offset + len0;
     float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-    int angles_of = -1;
+    bool fresh = true;
     size_t row = 0;         // of the node in the pools, for kv head 0
-    for (long long i = 0; i < most; ++i) {
-        if (i > 0) fetch(lo + i < hi ? lo + i : 0, lo + i < hi);
-        const bool node = t < nodes;
-        if (heads > 0 && node && angles_of != t) {
-            const int slot = len0 + t;
+    for (int i = 0; i < most; ++i) {
+        const int now = t, now_run = run;
+        RowRaw<TIn> x_raw[RUN];
+#pragma unroll
+        for (int h = 0; h < RUN; ++h) x_raw[h] = raw[h];
+        if (++run == runs) { run = 0; ++t; }
+        if (i + 1 < most) fetch(t, run, i + 1 < items);
+        int h0;
+        const int kind = place(now_run, &h0), heads = i < items && on ? min(RUN, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
+        const bool node = now < nodes;
+        if (heads > 0 && node && fresh) {
+            const int slot = len0 + now;
             row = ((size_t)a.block_table[(size_t)b * a.max_pages + slot / a.P] * a.Hkv * a.P + slot % a.P) * D;
-            row_angles(a.rope, freq, at.turned, pos0 + (a.parents ? mask_depth(masks.seen[t]) : t), c, s);
-            angles_of = t;
+            row_angles(tables, l, a.rope.gain, at.turned, pos0 + (a.parents ? mask_depth(masks.seen[now]) : now), c, s);
         }
-        const float* weight = kind == 2 ? a.q_weight : a.k_weight;
+        fresh = run == 0;
         float w[8];
+        row_weights(tables.w[kind != 2], at, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = weight ? __ldg(weight + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
+        for (int h = 0; h < RUN; ++h) {
+            float x[8], sum = 0.f;
+            row_unpack(x_raw[h], x);
 #pragma unroll
-        for (int h = 0; h < kRun; ++h) {
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[h][e], x[h][e], sum);
-            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps);
-            if (h >= heads) continue;
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+            const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps);
             if (kind != 1) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[h][e] = x[h][e] * r * w[e];
-                row_turn<HALF, false>(x[h], c, s, at.turned);
+                for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+                row_turn<HALF, false>(x, c, s, at.turned);
             }
-            if (kind == 2) {
-                if (!node) {
+            if (h < heads) {
+                if (kind == 2) {
+                    if (!node) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
+                        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+                    }
+                    row_store<HALF>(reinterpret_cast<TQ*>(a.q_out) + (((size_t)b * a.n_new + now) * a.Hq + h0 + h) * D, at, x);
+                } else if (node) {
+                    row_store<HALF>(reinterpret_cast<TC*>(kind ? a.v_pages : a.k_pages) + row + (size_t)(h0 + h) * a.P * D, at, x);
                 }
-                row_store<HALF>(reinterpret_cast<TQ*>(a.q_out) + (((size_t)b * a.n_new + t) * a.Hq + h0 + h) * D, at, x[h]);
-            } else if (node) {
-                row_store<HALF>(reinterpret_cast<TC*>(kind ? a.v_pages : a.k_pages) + row + (size_t)(h0 + h) * a.P * D, at, x[h]);
             }
         }
     }
@@ -212,12 +222,10 @@ __global__ void __launch_bounds__(256) append_norm_kernel(const __grid_constant_
 
 template <typename TIn, typename TC, typename TQ>
 static void (*append_lane_instance(int D, bool half))(AppendNormArgs) {
-    switch (D) {
-        case 32: return half ? append_norm_kernel<TIn, TC, TQ, 4, true> : append_norm_kernel<TIn, TC, TQ, 4, false>;
-        case 64: return half ? append_norm_kernel<TIn, TC, TQ, 8, true> : append_norm_kernel<TIn, TC, TQ, 8, false>;
-        case 128: return half ? append_norm_kernel<TIn, TC, TQ, 16, true> : append_norm_kernel<TIn, TC, TQ, 16, false>;
-        default: return half ? append_norm_kernel<TIn, TC, TQ, 32, true> : append_norm_kernel<TIn, TC, TQ, 32, false>;
-    }
+    return D <= 32 ? (half ? append_norm_kernel<TIn, TC, TQ, 4, true> : append_norm_kernel<TIn, TC, TQ, 4, false>)
+         : D <= 64 ? (half ? append_norm_kernel<TIn, TC, TQ, 8, true> : append_norm_kernel<TIn, TC, TQ, 8, false>)
+         : D <= 128 ? (half ? append_norm_kernel<TIn, TC, TQ, 16, true> : append_norm_kernel<TIn, TC, TQ, 16, false>)
+                    : (half ? append_norm_kernel<TIn, TC, TQ, 32, true> : append_norm_kernel<TIn, TC, TQ, 32, false>);
 }
 
 struct CommitArgs {
@@ -362,11 +370,12 @@ int grl_kv_append_norm(grl_device* dev, const grl_append_norm_params* p) {
     fill_rope_freq(dev, p->rope, &a.rope);
     a.status = dev->d_status;
     dev->status_dirty = true;
-    const bool fast = row_lanes_fit(a.D, a.rope.rd) && row_aligned(a.k_new, p->in_dtype, &a.ks, 1) && row_aligned(a.v_new, p->in_dtype, &a.vs, 1) &&
+    const bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0 && row_aligned(a.k_new, p->in_dtype, &a.ks, 1) && row_aligned(a.v_new, p->in_dtype, &a.vs, 1) &&
                       (!a.q_in || row_aligned(a.q_in, p->in_dtype, &a.qs, 1)) &&
                       ((uintptr_t)a.q_out | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages) % 16 == 0;
-    const long long groups = fast ? 256 / (a.D / 8) : 8, per_node = fast ? 2 * ((a.Hkv + kRun - 1) / kRun) + (a.Hq + kRun - 1) / kRun : 2 * a.Hkv + a.Hq;
-    const long long need = (a.n_new * per_node + groups - 1) / groups, most = ((fast ? 4LL : 8LL) * dev->prop.multiProcessorCount + a.B - 1) / a.B;
+    const int run = p->in_dtype == GRL_BF16 ? kRunOf<__nv_bfloat16> : kRunOf<float>;
+    const long long groups = fast ? 256 / row_lanes(a.D) : 8, per_node = fast ? 2 * ((a.Hkv + run - 1) / run) + (a.Hq + run - 1) / run : 2 * a.Hkv + a.Hq;
+    const long long need = (a.n_new * per_node + groups - 1) / groups, most = ((fast ? 3LL : 8LL) * dev->prop.multiProcessorCount + a.B - 1) / a.B;
     int ctas = (int)(need < most ? need : most);
     const bool fused = p->update_lens && ctas <= 4;
     if (fused) ctas = 1;

@@ -75,154 +75,179 @@ __global__ void __launch_bounds__(256) qk_norm_rows_kernel(const __grid_constant
     }
 }
 
-// Rows of 32, 64, 128 or 256 elements on 16-byte boundaries: LANES threads a row, eight elements each.  Bound by HBM, each element read and
-// written once.  A thread group keeps its places in the rows, walks the heads of a token in runs of kRun rows, whose loads are in
-// flight together, and forms a token's angles (double precision) once for all of them; every group has an equal, contiguous share of all runs.
-constexpr int kRun = 4;
-struct RunPlace {
-    int b, s, h0, heads;
-    bool is_k;
+// Rows of whole 8-element pieces on 16-byte boundaries: LANES threads a row, eight elements each (threads past the row's end idle).  Bound by HBM, each element read and
+// written once.  A thread group keeps its places in the rows, walks the heads of a token in runs, the next run's loads on their
+// way under the present one, and forms a token's angles (double precision) once for all of them; every group has an equal,
+// contiguous share of all runs, and steps from run to run without dividing.
+template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;      // rows of a run
+struct RunWalk {
+    int b, s, run;
+    __device__ __forceinline__ void start(long long item, int S, int runs) {
+        const long long tok = item / runs;
+        run = (int)(item - tok * runs);
+        b = (int)(tok / S);
+        s = (int)(tok - (long long)b * S);
+    }
+    __device__ __forceinline__ void step(int S, int runs) {
+        if (++run < runs) return;
+        run = 0;
+        if (++s < S) return;
+        s = 0;
+        ++b;
+    }
 };
-template <typename A>
-__device__ __forceinline__ RunPlace run_place(const A& a, long long item, int q_runs, int runs) {
-    const long long tok = item / runs;
-    const int r = (int)(item - tok * runs);
-    RunPlace p;
-    p.is_k = r >= q_runs;
-    p.h0 = (p.is_k ? r - q_runs : r) * kRun;
-    p.heads = min(kRun, (p.is_k ? a.k.H : a.q.H) - p.h0);
-    p.b = (int)(tok / a.S);
-    p.s = (int)(tok - (long long)p.b * a.S);
-    return p;
-}
 template <typename TIn, typename TOut, int LANES, bool HALF>
-__global__ void __launch_bounds__(256) qk_norm_kernel(const __grid_constant__ NormArgs a) {
-    const int l = threadIdx.x % LANES, D = 8 * LANES;
+__global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int RUN = kRunOf<TIn>;
+    __shared__ __align__(16) RowTables tables;
+    const int l = threadIdx.x % LANES, D = a.D;
+    const bool on = 8 * l < D;
+    const float inv_d = 1.f / D;
     const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    double freq[4];
-    row_freq(a.rope, l, at.turned, freq);
-    const int q_runs = (a.q.H + kRun - 1) / kRun, runs = q_runs + (a.k.H + kRun - 1) / kRun;
+    const int q_runs = (a.q.H + RUN - 1) / RUN, runs = q_runs + (a.k.H + RUN - 1) / RUN;
     const long long total = (long long)a.B * a.S * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const long long lo = mine * total / all, hi = (mine + 1) * total / all;
-    const long long most = (total + all - 1) / all;         // of any group: the warp's groups take the same trips, for the shuffles
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-    int angles_b = -1, angles_s = -1;
+    const long long lo = mine * total / all;
+    const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);      // of the group; of any group: the
+                                                                        // groups of a warp take the same trips, for the shuffles
     pdl_wait();
     pdl_trigger();
-    for (long long i = 0; i < most; ++i) {
-        const bool live = lo + i < hi;
-        const RunPlace p = run_place(a, live ? lo + i : 0, q_runs, runs);
-        const NormSide& side = p.is_k ? a.k : a.q;
-        float x[kRun][8];
-        const TIn* in = reinterpret_cast<const TIn*>(side.x) + p.b * side.xs[0] + p.s * side.xs[1] + p.h0 * side.xs[2];
+    RunWalk at_run;
+    at_run.start(items > 0 ? lo : 0, a.S, runs);
+    RowRaw<TIn> raw[RUN];
+    auto fetch = [&](const RunWalk& w, bool live) {
+        const bool is_k = w.run >= q_runs;
+        const NormSide& side = is_k ? a.k : a.q;
+        const int h0 = (is_k ? w.run - q_runs : w.run) * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
+        const TIn* in = reinterpret_cast<const TIn*>(side.x) + w.b * side.xs[0] + w.s * side.xs[1] + h0 * side.xs[2];
 #pragma unroll
-        for (int h = 0; h < kRun; ++h)
-            if (live && h < p.heads) row_load<HALF>(in + h * side.xs[2], at, x[h]);
-            else {
+        for (int h = 0; h < RUN; ++h)
+            if (h < heads) row_fetch<HALF>(in + h * side.xs[2], at, raw[h]);
+            else row_zero(raw[h]);
+    };
+    fetch(at_run, items > 0);
+    row_tables<HALF>(tables, a.rope, D, a.q.w, a.k.w);
+    __syncthreads();
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    bool fresh = true;          // a token whose angles are not formed yet
+    for (int i = 0; i < most; ++i) {
+        const RunWalk now = at_run;
+        RowRaw<TIn> x_raw[RUN];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[h][e] = 0.f;
-            }
-        if (live && (p.b != angles_b || p.s != angles_s)) {     // under the loads
-            row_angles(a.rope, freq, at.turned, position_of(a, p.b, p.s), c, s);
-            angles_b = p.b;
-            angles_s = p.s;
-        }
+        for (int h = 0; h < RUN; ++h) x_raw[h] = raw[h];
+        const bool live = i < items;
+        at_run.step(a.S, runs);
+        if (i + 1 < most) fetch(at_run, i + 1 < items);
+        if (live && fresh) row_angles(tables, l, a.rope.gain, at.turned, position_of(a, now.b, now.s), c, s);
+        fresh = at_run.run == 0;
+        const bool is_k = now.run >= q_runs;
+        const NormSide& side = is_k ? a.k : a.q;
+        const int h0 = (is_k ? now.run - q_runs : now.run) * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
+        TOut* out = reinterpret_cast<TOut*>(side.y) + now.b * side.ys[0] + now.s * side.ys[1] + h0 * side.ys[2];
         float w[8];
+        row_weights(tables.w[is_k], at, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = side.w ? __ldg(side.w + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
-        TOut* out = reinterpret_cast<TOut*>(side.y) + p.b * side.ys[0] + p.s * side.ys[1] + p.h0 * side.ys[2];
+        for (int h = 0; h < RUN; ++h) {
+            float x[8], sum = 0.f;
+            row_unpack(x_raw[h], x);
 #pragma unroll
-        for (int h = 0; h < kRun; ++h) {
-            float sum = 0.f;
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+            const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[h][e], x[h][e], sum);
-            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[h][e] = x[h][e] * r * w[e];
-            row_turn<HALF, false>(x[h], c, s, at.turned);
-            if (live && h < p.heads) row_store<HALF>(out + h * side.ys[2], at, x[h]);
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+            row_turn<HALF, false>(x, c, s, at.turned);
+            if (h < heads) row_store<HALF>(out + h * side.ys[2], at, x);
         }
     }
 }
 
-// The backward pass in the same form; a group keeps its shares of both weight gradients in registers, the CTA adds them in order of
-// its groups.
-constexpr int kGradRun = 2;
+// The backward pass in the same form, the queries and then the keys; a group keeps its share of the weight's gradient in registers, the CTA adds
+// them in order of its groups.
+template <typename T> constexpr int kGradRunOf = sizeof(T) == 2 ? 2 : 1;
 template <typename TIn, typename TOut, int LANES, bool HALF>
-__global__ void __launch_bounds__(256) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
-    constexpr int D = 8 * LANES, GROUPS = 256 / LANES;
-    __shared__ __align__(16) float sm[GROUPS][D];
-    const int l = threadIdx.x % LANES, group = threadIdx.x / LANES;
+__global__ void __launch_bounds__(256, 3) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int GROUPS = 256 / LANES, RUN = kGradRunOf<TIn>;
+    __shared__ __align__(16) RowTables tables;
+    __shared__ __align__(16) float sm[GROUPS][8 * LANES];
+    const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, D = a.D;
+    const bool on = 8 * l < D;
+    const float inv_d = 1.f / D;
     const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    double freq[4];
-    row_freq(a.rope, l, at.turned, freq);
-    const int q_runs = (a.q.H + kGradRun - 1) / kGradRun, runs = q_runs + (a.k.H + kGradRun - 1) / kGradRun;
-    const long long total = (long long)a.B * a.S * runs, all = (long long)gridDim.x * GROUPS, mine = (long long)blockIdx.x * GROUPS + group;
-    const long long lo = mine * total / all, hi = (mine + 1) * total / all, most = (total + all - 1) / all;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, acc[2][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
-    int angles_b = -1, angles_s = -1;
+    const long long all = (long long)gridDim.x * GROUPS, mine = (long long)blockIdx.x * GROUPS + group;
     pdl_wait();
-    for (long long i = 0; i < most; ++i) {
-        const bool live = lo + i < hi;
-        const long long item = live ? lo + i : 0, tok = item / runs;
-        const int run = (int)(item - tok * runs), b = (int)(tok / a.S), st = (int)(tok - (long long)b * a.S);
-        const bool is_k = run >= q_runs;
-        const NormSide& side = is_k ? a.k : a.q;
-        const int h0 = (is_k ? run - q_runs : run) * kGradRun, heads = live ? min(kGradRun, side.H - h0) : 0;
-        const TIn* in = reinterpret_cast<const TIn*>(side.x) + b * side.xs[0] + st * side.xs[1] + h0 * side.xs[2];
-        const TOut* dy = reinterpret_cast<const TOut*>(side.dy) + b * side.dys[0] + st * side.dys[1] + h0 * side.dys[2];
-        float x[kGradRun][8], g[kGradRun][8];
+    row_tables<HALF>(tables, a.rope, D, a.q.w, a.k.w);
+    __syncthreads();
+#pragma unroll 1
+    for (int side_i = 0; side_i < 2; ++side_i) {
+        const NormSide& side = side_i ? a.k : a.q;
+        const int runs = (side.H + RUN - 1) / RUN;
+        const long long total = (long long)a.B * a.S * runs, lo = mine * total / all;
+        const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);
+        RunWalk at_run{0, 0, 0};
+        if (items > 0) at_run.start(lo, a.S, runs);
+        RowRaw<TIn> xr[RUN];
+        RowRaw<TOut> gr[RUN];
+        auto fetch = [&](const RunWalk& w, bool live) {
+            const int h0 = w.run * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
+            const TIn* in = reinterpret_cast<const TIn*>(side.x) + w.b * side.xs[0] + w.s * side.xs[1] + h0 * side.xs[2];
+            const TOut* dy = reinterpret_cast<const TOut*>(side.dy) + w.b * side.dys[0] + w.s * side.dys[1] + h0 * side.dys[2];
 #pragma unroll
-        for (int h = 0; h < kGradRun; ++h)
-            if (h < heads) {
-                row_load<HALF>(in + h * side.xs[2], at, x[h]);
-                row_load<HALF>(dy + h * side.dys[2], at, g[h]);
-            } else {
+            for (int h = 0; h < RUN; ++h)
+                if (h < heads) {
+                    row_fetch<HALF>(in + h * side.xs[2], at, xr[h]);
+                    row_fetch<HALF>(dy + h * side.dys[2], at, gr[h]);
+                } else {
+                    row_zero(xr[h]);
+                    row_zero(gr[h]);
+                }
+        };
+        if (most > 0) fetch(at_run, items > 0);
+        float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, acc[8], w[8];
+        row_weights(tables.w[side_i], at, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[h][e] = g[h][e] = 0.f;
+        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+        bool fresh = true;
+        for (int i = 0; i < most; ++i) {
+            const RunWalk now = at_run;
+            RowRaw<TIn> xn[RUN];
+            RowRaw<TOut> gn[RUN];
+#pragma unroll
+            for (int h = 0; h < RUN; ++h) { xn[h] = xr[h]; gn[h] = gr[h]; }
+            const bool live = i < items;
+            at_run.step(a.S, runs);
+            if (i + 1 < most) fetch(at_run, i + 1 < items);
+            if (live && fresh) row_angles(tables, l, a.rope.gain, at.turned, position_of(a, now.b, now.s), c, s);
+            fresh = at_run.run == 0;
+            const int h0 = now.run * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
+            TIn* dx = reinterpret_cast<TIn*>(side.y) + now.b * side.ys[0] + now.s * side.ys[1] + h0 * side.ys[2];
+#pragma unroll
+            for (int h = 0; h < RUN; ++h) {
+                float x[8], g[8], sum = 0.f, dot = 0.f;
+                row_unpack(xn[h], x);
+                row_unpack(gn[h], g);
+                row_turn<HALF, true>(g, c, s, at.turned);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    sum = fmaf(x[e], x[e], sum);
+                    dot = fmaf(g[e] * w[e], x[e], dot);
+                }
+                const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps), f = row_sum<LANES>(dot) * inv_d * r * r;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    acc[e] = fmaf(g[e], x[e] * r, acc[e]);
+                    x[e] = r * (g[e] * w[e] - x[e] * f);
+                }
+                if (h < heads) row_store<HALF>(dx + h * side.ys[2], at, x);
             }
-        if (live && (b != angles_b || st != angles_s)) {
-            row_angles(a.rope, freq, at.turned, position_of(a, b, st), c, s);
-            angles_b = b;
-            angles_s = st;
         }
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = side.w ? __ldg(side.w + (e < 4 ? at.o0 : at.o1 - 4) + e) : 1.f;
-        TIn* dx = reinterpret_cast<TIn*>(side.y) + b * side.ys[0] + st * side.ys[1] + h0 * side.ys[2];
-#pragma unroll
-        for (int h = 0; h < kGradRun; ++h) {
-            row_turn<HALF, true>(g[h], c, s, at.turned);
-            float sum = 0.f, dot = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sum = fmaf(x[h][e], x[h][e], sum);
-                dot = fmaf(g[h][e] * w[e], x[h][e], dot);
-            }
-            const float r = rsqrtf(row_sum<LANES>(sum) * (1.f / D) + a.eps), f = row_sum<LANES>(dot) * (1.f / D) * r * r;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float gx = g[h][e] * (x[h][e] * r);
-                if (is_k) acc[1][e] += gx;
-                else acc[0][e] += gx;
-                x[h][e] = r * (g[h][e] * w[e] - x[h][e] * f);
-            }
-            if (h < heads) row_store<HALF>(dx + h * side.ys[2], at, x[h]);
-        }
-    }
-    pdl_trigger();
-    if (!a.part) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        row_store<HALF>(sm[group], at, acc[i]);
+        if (side_i == 1) pdl_trigger();
+        if (!a.part) continue;
+        if (on) row_store<HALF>(sm[group], at, acc);
         __syncthreads();
         if (threadIdx.x < D) {
             float sum = 0.f;
 #pragma unroll 8
             for (int j = 0; j < GROUPS; ++j) sum += sm[j][threadIdx.x];
-            a.part[((size_t)blockIdx.x * 2 + i) * D + threadIdx.x] = sum;
+            a.part[((size_t)blockIdx.x * 2 + side_i) * D + threadIdx.x] = sum;
         }
         __syncthreads();
     }
@@ -231,19 +256,15 @@ __global__ void __launch_bounds__(256) qk_norm_backward_kernel(const __grid_cons
 template <typename TIn, typename TOut, bool BACK>
 static void (*lane_instance(int D, bool half))(NormArgs) {
     if constexpr (BACK) {
-        switch (D) {
-            case 32: return half ? qk_norm_backward_kernel<TIn, TOut, 4, true> : qk_norm_backward_kernel<TIn, TOut, 4, false>;
-            case 64: return half ? qk_norm_backward_kernel<TIn, TOut, 8, true> : qk_norm_backward_kernel<TIn, TOut, 8, false>;
-            case 128: return half ? qk_norm_backward_kernel<TIn, TOut, 16, true> : qk_norm_backward_kernel<TIn, TOut, 16, false>;
-            default: return half ? qk_norm_backward_kernel<TIn, TOut, 32, true> : qk_norm_backward_kernel<TIn, TOut, 32, false>;
-        }
+        return D <= 32 ? (half ? qk_norm_backward_kernel<TIn, TOut, 4, true> : qk_norm_backward_kernel<TIn, TOut, 4, false>)
+             : D <= 64 ? (half ? qk_norm_backward_kernel<TIn, TOut, 8, true> : qk_norm_backward_kernel<TIn, TOut, 8, false>)
+             : D <= 128 ? (half ? qk_norm_backward_kernel<TIn, TOut, 16, true> : qk_norm_backward_kernel<TIn, TOut, 16, false>)
+                        : (half ? qk_norm_backward_kernel<TIn, TOut, 32, true> : qk_norm_backward_kernel<TIn, TOut, 32, false>);
     } else {
-        switch (D) {
-            case 32: return half ? qk_norm_kernel<TIn, TOut, 4, true> : qk_norm_kernel<TIn, TOut, 4, false>;
-            case 64: return half ? qk_norm_kernel<TIn, TOut, 8, true> : qk_norm_kernel<TIn, TOut, 8, false>;
-            case 128: return half ? qk_norm_kernel<TIn, TOut, 16, true> : qk_norm_kernel<TIn, TOut, 16, false>;
-            default: return half ? qk_norm_kernel<TIn, TOut, 32, true> : qk_norm_kernel<TIn, TOut, 32, false>;
-        }
+        return D <= 32 ? (half ? qk_norm_kernel<TIn, TOut, 4, true> : qk_norm_kernel<TIn, TOut, 4, false>)
+             : D <= 64 ? (half ? qk_norm_kernel<TIn, TOut, 8, true> : qk_norm_kernel<TIn, TOut, 8, false>)
+             : D <= 128 ? (half ? qk_norm_kernel<TIn, TOut, 16, true> : qk_norm_kernel<TIn, TOut, 16, false>)
+                        : (half ? qk_norm_kernel<TIn, TOut, 32, true> : qk_norm_kernel<TIn, TOut, 32, false>);
     }
 }
 template <bool BACK>
@@ -369,7 +390,7 @@ __global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __res
 
 // CTAs of the backward pass: what the GPU holds at once, or a warp a row.
 static int backward_ctas(grl_device* dev, const grl_qk_norm_params& f) {
-    const long long rows = (long long)f.batch * f.seq_len * f.num_q_heads, most = 4LL * dev->prop.multiProcessorCount;
+    const long long rows = (long long)f.batch * f.seq_len * f.num_q_heads, most = 3LL * dev->prop.multiProcessorCount;
     const long long ctas = (rows + 7) / 8;
     return (int)(ctas < most ? ctas : most);
 }
@@ -486,12 +507,13 @@ int grl_qk_norm_rope(grl_device* dev, const grl_qk_norm_params* p) {
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->rope, &a.rope);
     const long long rows = (long long)a.B * a.S * (a.q.H + a.k.H), most = 8LL * dev->prop.multiProcessorCount;
-    bool fast = row_lanes_fit(a.D, a.rope.rd);
+    bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0;
     for (const NormSide* s : {&a.q, &a.k})
         if (s->H) fast = fast && row_aligned(s->x, p->in_dtype, s->xs, 3) && row_aligned(s->y, p->out_dtype, s->ys, 3);
     if (fast) {
-        const long long runs = (long long)a.B * a.S * ((a.q.H + kRun - 1) / kRun + (a.k.H + kRun - 1) / kRun), groups = 256 / (a.D / 8);
-        const long long need = (runs + groups - 1) / groups, held = 4LL * dev->prop.multiProcessorCount;
+        const int run = p->in_dtype == GRL_BF16 ? kRunOf<__nv_bfloat16> : kRunOf<float>;
+        const long long runs = (long long)a.B * a.S * ((a.q.H + run - 1) / run + (a.k.H + run - 1) / run), groups = 256 / row_lanes(a.D);
+        const long long need = (runs + groups - 1) / groups, held = 3LL * dev->prop.multiProcessorCount;
         GRL_CUDA(launch_pdl(instance<false>(*p), dim3((unsigned)(need < held ? need : held)), 256, 0, dev->stream, a));
         GRL_LAUNCHED("qk_norm_kernel");
         return GRL_OK;
@@ -528,7 +550,7 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
     }
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->fwd.rope, &a.rope);
-    bool fast = row_lanes_fit(a.D, a.rope.rd);
+    bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0;
     for (const NormSide* s : {&a.q, &a.k})
         if (s->H)
             fast = fast && row_aligned(s->x, p->fwd.in_dtype, s->xs, 3) && row_aligned(s->y, p->fwd.in_dtype, s->ys, 3) &&

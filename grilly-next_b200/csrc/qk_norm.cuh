@@ -25,7 +25,7 @@ inline bool row_aligned(const void* p, int dtype, const long long* strides, int 
     for (int i = 0; i < n; ++i) ok = ok && strides[i] % unit == 0;
     return ok;
 }
-inline bool row_lanes_fit(int D, int rd) { return (D == 32 || D == 64 || D == 128 || D == 256) && rd % 8 == 0; }
+inline int row_lanes(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }      // threads of a row
 
 #ifdef __CUDACC__
 // Element places of pair j of a row: the rotated pairs first, then the elements that are left as they are, in neighbours.
@@ -41,9 +41,9 @@ __device__ __forceinline__ void pair_angle(const RopeArgs& r, int j, int pos, fl
     *c *= r.gain;
     *s *= r.gain;
 }
-// ---- rows of D = 8 * LANES elements held by LANES neighbouring threads, eight elements each: x[0..3] at o0 and x[4..7] at o1.  Rotated in
+// ---- rows of up to 8 * LANES elements held by LANES neighbouring threads, eight elements each: x[0..3] at o0 and x[4..7] at o1.  Rotated in
 // halves, element e and e + 4 of a thread are a pair (o1 = o0 + rd / 2); else neighbours are, and o1 = o0 + 4.  The threads behind the
-// rotated part hold the elements that are left as they are.  Needs rd % 8 == 0, and rows on boundaries of four elements
+// rotated part hold the elements that are left as they are.  Needs D % 8 == 0 and rd % 8 == 0, and rows on boundaries of four elements
 // (eight where o1 = o0 + 4).
 struct RowPlace {
     int o0, o1;
@@ -65,24 +65,38 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// A thread's part of a row as it lies in memory: what is on its way for later rows takes no more registers than that.
+template <typename T> struct RowRaw {
+    uint32_t w[sizeof(T) * 2];
+};
 template <bool HALF>
-__device__ __forceinline__ void row_load(const float* p, const RowPlace& at, float (&x)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p + at.o0)), b = __ldcs(reinterpret_cast<const float4*>(p + at.o1));
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+__device__ __forceinline__ void row_fetch(const float* p, const RowPlace& at, RowRaw<float>& r) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + at.o0)), b = __ldcs(reinterpret_cast<const uint4*>(p + at.o1));
+    r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+    r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
 }
 template <bool HALF>
-__device__ __forceinline__ void row_load(const __nv_bfloat16* p, const RowPlace& at, float (&x)[8]) {
-    uint32_t w[4];
+__device__ __forceinline__ void row_fetch(const __nv_bfloat16* p, const RowPlace& at, RowRaw<__nv_bfloat16>& r) {
     if constexpr (HALF) {
         const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p + at.o0)), b = __ldcs(reinterpret_cast<const uint2*>(p + at.o1));
-        w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+        r.w[0] = a.x; r.w[1] = a.y; r.w[2] = b.x; r.w[3] = b.y;
     } else {
         const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + at.o0));
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
     }
+}
+template <typename T>
+__device__ __forceinline__ void row_zero(RowRaw<T>& r) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) unpack_bf16(w[e], x[2 * e], x[2 * e + 1]);
+    for (int i = 0; i < (int)sizeof(T) * 2; ++i) r.w[i] = 0u;
+}
+__device__ __forceinline__ void row_unpack(const RowRaw<float>& r, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(r.w[e]);
+}
+__device__ __forceinline__ void row_unpack(const RowRaw<__nv_bfloat16>& r, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) unpack_bf16(r.w[e], x[2 * e], x[2 * e + 1]);
 }
 template <bool HALF>
 __device__ __forceinline__ void row_store(float* p, const RowPlace& at, const float (&y)[8]) {
@@ -107,22 +121,36 @@ __device__ __forceinline__ float row_sum(float v) {
     for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, LANES);
     return v;
 }
+// Frequencies of the pairs and the weights of both sides, in shared memory: a thread's own are read where they are used.
+struct RowTables {
+    double freq[128];
+    float w[2][256];
+};
+template <bool HALF>
+__device__ __forceinline__ void row_tables(RowTables& t, const RopeArgs& r, int D, const float* w0, const float* w1) {
+    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+        t.w[0][i] = w0 ? __ldg(w0 + i) : 1.f;
+        t.w[1][i] = w1 ? __ldg(w1 + i) : 1.f;
+        if (2 * i < r.rd) t.freq[i] = r.inv_freq ? (double)__ldg(r.inv_freq + i) : r.freq.inv_freq[i];
+    }
+}
+__device__ __forceinline__ void row_weights(const float* w, const RowPlace& at, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(w + at.o0), b = *reinterpret_cast<const float4*>(w + at.o1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
 // cosine and sine of a thread's four pairs at a position; 1 and 0 where nothing turns
-__device__ __forceinline__ void row_angles(const RopeArgs& r, const double (&freq)[4], bool turned, int pos, float (&c)[4], float (&s)[4]) {
+__device__ __forceinline__ void row_angles(const RowTables& t, int l, float gain, bool turned, int pos, float (&c)[4], float (&s)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         c[e] = 1.f;
         s[e] = 0.f;
         if (turned) {
-            rope_sincos(pos, freq[e], &c[e], &s[e]);
-            c[e] *= r.gain;
-            s[e] *= r.gain;
+            rope_sincos(pos, t.freq[4 * l + e], &c[e], &s[e]);
+            c[e] *= gain;
+            s[e] *= gain;
         }
     }
-}
-__device__ __forceinline__ void row_freq(const RopeArgs& r, int l, bool turned, double (&freq)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) freq[e] = !turned ? 0.0 : r.inv_freq ? (double)r.inv_freq[4 * l + e] : r.freq.inv_freq[4 * l + e];
 }
 // The rotation of a thread's pairs; BACK: its transpose.
 template <bool HALF, bool BACK>
