@@ -123,109 +123,117 @@ __global__ void __launch_bounds__(256) append_norm_rows_kernel(const __grid_cons
     }
 }
 
-// Rows of whole 8-element pieces on 16-byte boundaries: the form of qk_norm_kernel (qk_norm.cu).  A run is kRun heads of the keys, the
-// values or the queries of a node.  A group's first run is on its way while the sequence's numbers are read and checked.
+// Rows of whole 8-element pieces on 16-byte boundaries: the form of qk_norm_kernel (qk_norm.cu).  A node's rows are its Hkv keys, Hkv values and
+// Hq queries; a warp's first rows are on their way while the sequence's numbers are read and checked.
 template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;
-template <typename TIn, typename TC, typename TQ, int LANES, bool HALF>
+template <typename TIn, typename TC, typename TQ, int LANES, bool HALF, bool FULL>
 __global__ void __launch_bounds__(256, 3) append_norm_kernel(const __grid_constant__ AppendNormArgs a) {
-    constexpr int RUN = kRunOf<TIn>;
+    constexpr int RUN = kRunOf<TIn>, GPW = 32 / LANES;
     __shared__ TreeMasks masks;
     __shared__ __align__(16) RowTables tables;
-    const int b = blockIdx.y, l = threadIdx.x % LANES, D = a.D;
-    const bool on = 8 * l < D;
+    const int seq = blockIdx.y, l = threadIdx.x % LANES, g = (threadIdx.x & 31) / LANES, D = FULL ? 8 * LANES : a.D;
+    const bool on = FULL || 8 * l < D;
     const float inv_d = 1.f / D;
-    const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    const int kv_runs = (a.Hkv + RUN - 1) / RUN, runs = 2 * kv_runs + (a.Hq + RUN - 1) / RUN;
-    const long long total = (long long)a.n_new * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const long long lo = mine * total / all;
-    const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);
+    const RowPlace at = row_place<HALF>(l, FULL ? D : a.rope.rd);
+    const int gap = FULL && HALF ? 4 * LANES : at.gap();
+    const int slots = 2 * a.Hkv + a.Hq;
+    const Share share((long long)a.n_new * slots);
+    int t = (int)(share.lo / slots), slot = (int)(share.lo - (long long)t * slots), left = share.items;
     RowRaw<TIn> raw[RUN];
-    int t = items > 0 ? (int)(lo / runs) : 0, run = items > 0 ? (int)(lo - (long long)t * runs) : 0;
-    auto place = [&](int run, int* h0) {
-        const int kind = run < kv_runs ? 0 : run < 2 * kv_runs ? 1 : 2;
-        *h0 = (run - kind * kv_runs) * RUN;
-        return kind;
-    };
-    auto fetch = [&](int t, int run, bool live) {
-        int h0;
-        const int kind = place(run, &h0), heads = live && on ? min(RUN, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
-        const TIn* in = reinterpret_cast<const TIn*>(kind == 0 ? a.k_new : kind == 1 ? a.v_new : a.q_in) +
-                        ((size_t)b * a.n_new + t) * (kind == 0 ? a.ks : kind == 1 ? a.vs : a.qs) + (size_t)h0 * D;
+    const TIn* in = nullptr;
+    int kind = 0, h0 = 0, n = 0;        // the segment: keys, values or queries, its first head, its rows
+    auto aim = [&] {
+        kind = slot < a.Hkv ? 0 : slot < 2 * a.Hkv ? 1 : 2;
+        h0 = slot - kind * a.Hkv;
+        n = min(left, (kind == 2 ? a.Hq : a.Hkv) - h0);
+        in = reinterpret_cast<const TIn*>(kind == 0 ? a.k_new : kind == 1 ? a.v_new : a.q_in) +
+             (((long long)seq * a.n_new + t) * (kind == 0 ? a.ks : kind == 1 ? a.vs : a.qs) + (h0 + g) * D + at.o0);
 #pragma unroll
         for (int h = 0; h < RUN; ++h)
-            if (h < heads) row_fetch<HALF>(in + h * D, at, raw[h]);
+            if (on && g + GPW * h < n) row_fetch<HALF>(in + GPW * h * D, gap, raw[h]);
             else row_zero(raw[h]);
     };
     pdl_wait();
     pdl_trigger();
-    fetch(t, run, items > 0);
-    const int len0 = a.seq_lens[b], n = tree_count(a.n_nodes, a.n_new, b), offset = a.pos_offsets ? a.pos_offsets[b] : 0;
-    row_tables<HALF>(tables, a.rope, D, a.q_weight, a.k_weight);
-    bool ok = append_fits(a, b, len0, n);
-    if (ok && a.parents && !tree_masks(masks, a.parents + (size_t)b * a.n_new, n)) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
+    if (left > 0) aim();
+    const int len0 = a.seq_lens[seq], count = tree_count(a.n_nodes, a.n_new, seq), offset = a.pos_offsets ? a.pos_offsets[seq] : 0;
+    row_tables(tables, a.rope, D, a.q_weight, a.k_weight);
+    bool ok = append_fits(a, seq, len0, count);
+    if (ok && a.parents && !tree_masks(masks, a.parents + (size_t)seq * a.n_new, count)) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) tree_fail(a.status, TREE_BAD_PARENT, seq, count);
         ok = false;
     }
     __syncthreads();
-    const int nodes = ok ? n : 0, pos0 = a.pos_base + offset + len0;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    const int nodes = ok ? count : 0, pos0 = a.pos_base + offset + len0;
+    Pairs angle;
     bool fresh = true;
     size_t row = 0;         // of the node in the pools, for kv head 0
-    for (int i = 0; i < most; ++i) {
-        const int now = t, now_run = run;
-        RowRaw<TIn> x_raw[RUN];
-#pragma unroll
-        for (int h = 0; h < RUN; ++h) x_raw[h] = raw[h];
-        if (++run == runs) { run = 0; ++t; }
-        if (i + 1 < most) fetch(t, run, i + 1 < items);
-        int h0;
-        const int kind = place(now_run, &h0), heads = i < items && on ? min(RUN, (kind == 2 ? a.Hq : a.Hkv) - h0) : 0;
-        const bool node = now < nodes;
-        if (heads > 0 && node && fresh) {
-            const int slot = len0 + now;
-            row = ((size_t)a.block_table[(size_t)b * a.max_pages + slot / a.P] * a.Hkv * a.P + slot % a.P) * D;
-            row_angles(tables, l, a.rope.gain, at.turned, pos0 + (a.parents ? mask_depth(masks.seen[now]) : now), c, s);
+    for (bool first = true; left > 0; first = false) {
+        if (!first) aim();
+        const bool node = t < nodes;
+        if (fresh && node) {
+            const int place = len0 + t;
+            row = ((size_t)a.block_table[(size_t)seq * a.max_pages + place / a.P] * a.Hkv * a.P + place % a.P) * D;
+            angle = row_angles(tables, l, a.rope.gain, at.turned, pos0 + (a.parents ? mask_depth(masks.seen[t]) : t));
+            fresh = false;
         }
-        fresh = run == 0;
-        float w[8];
-        row_weights(tables.w[kind != 2], at, w);
+        Turn turn;
+        if (kind != 1) turn = weighted_turn(row_weights<HALF>(tables.w[kind != 2], at), angle);
+        TQ* q_at = reinterpret_cast<TQ*>(a.q_out) + (((long long)seq * a.n_new + t) * a.Hq + h0 + g) * D + at.o0;
+        TC* kv_at = reinterpret_cast<TC*>(kind ? a.v_pages : a.k_pages) + row + (long long)(h0 + g) * a.P * D + at.o0;
+        const int kv_step = GPW * a.P * D;
+        for (int i = g; i < n + g; i += GPW * RUN) {
+            in += RUN * GPW * D;
 #pragma unroll
-        for (int h = 0; h < RUN; ++h) {
-            float x[8], sum = 0.f;
-            row_unpack(x_raw[h], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-            const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps);
-            if (kind != 1) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
-                row_turn<HALF, false>(x, c, s, at.turned);
-            }
-            if (h < heads) {
-                if (kind == 2) {
-                    if (!node) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+            for (int h = 0; h < RUN; ++h) {
+                Pairs x = row_pairs<HALF>(raw[h]);
+                if (on && i + GPW * (RUN + h) < n) row_fetch<HALF>(in + GPW * h * D, gap, raw[h]);
+                if (kind != 1) {
+                    const float r = rsqrtf(row_sum<LANES>(squares(x)) * inv_d + a.eps);
+                    turn_scaled(x, turn, r);
+                }
+                if (on && i + GPW * h < n) {
+                    if (kind == 2) {
+                        if (!node) x.f[0] = x.f[1] = x.g[0] = x.g[1] = make_float2(0.f, 0.f);
+                        row_store<HALF>(q_at + GPW * h * D, gap, x);
+                    } else if (node) {
+                        row_store<HALF>(kv_at + (long long)h * kv_step, gap, x);
                     }
-                    row_store<HALF>(reinterpret_cast<TQ*>(a.q_out) + (((size_t)b * a.n_new + now) * a.Hq + h0 + h) * D, at, x);
-                } else if (node) {
-                    row_store<HALF>(reinterpret_cast<TC*>(kind ? a.v_pages : a.k_pages) + row + (size_t)(h0 + h) * a.P * D, at, x);
                 }
             }
+            q_at += RUN * GPW * D;
+            kv_at += (long long)RUN * kv_step;
+        }
+        slot += n;
+        left -= n;
+        if (slot == slots) {
+            slot = 0;
+            ++t;
+            fresh = true;
         }
     }
     if (a.update_lens && ok) {
         __syncthreads();        // every thread has read the length
-        if (threadIdx.x == 0) a.seq_lens[b] = len0 + n;
+        if (threadIdx.x == 0) a.seq_lens[seq] = len0 + count;
     }
 }
 
+template <typename TIn, typename TC, typename TQ, int LANES>
+static void (*append_form_instance(bool half, bool full))(AppendNormArgs) {
+    return half ? (full ? append_norm_kernel<TIn, TC, TQ, LANES, true, true> : append_norm_kernel<TIn, TC, TQ, LANES, true, false>)
+                : (full ? append_norm_kernel<TIn, TC, TQ, LANES, false, true> : append_norm_kernel<TIn, TC, TQ, LANES, false, false>);
+}
 template <typename TIn, typename TC, typename TQ>
-static void (*append_lane_instance(int D, bool half))(AppendNormArgs) {
-    return D <= 32 ? (half ? append_norm_kernel<TIn, TC, TQ, 4, true> : append_norm_kernel<TIn, TC, TQ, 4, false>)
-         : D <= 64 ? (half ? append_norm_kernel<TIn, TC, TQ, 8, true> : append_norm_kernel<TIn, TC, TQ, 8, false>)
-         : D <= 128 ? (half ? append_norm_kernel<TIn, TC, TQ, 16, true> : append_norm_kernel<TIn, TC, TQ, 16, false>)
-                    : (half ? append_norm_kernel<TIn, TC, TQ, 32, true> : append_norm_kernel<TIn, TC, TQ, 32, false>);
+static void (*append_instance(bool fast, int D, int rd, bool half))(AppendNormArgs) {
+    const bool full = row_full(D, rd);
+    return !fast ? append_norm_rows_kernel<TIn, TC, TQ> : D <= 32 ? append_form_instance<TIn, TC, TQ, 4>(half, full)
+         : D <= 64 ? append_form_instance<TIn, TC, TQ, 8>(half, full) : D <= 128 ? append_form_instance<TIn, TC, TQ, 16>(half, full)
+                                                                                : append_form_instance<TIn, TC, TQ, 32>(half, full);
+}
+template <typename TIn>
+static void (*append_norm_instance(bool cache32, bool q32, bool fast, int D, int rd, bool half))(AppendNormArgs) {
+    return cache32 ? (q32 ? append_instance<TIn, float, float>(fast, D, rd, half) : append_instance<TIn, float, __nv_bfloat16>(fast, D, rd, half))
+                   : (q32 ? append_instance<TIn, __nv_bfloat16, float>(fast, D, rd, half) : append_instance<TIn, __nv_bfloat16, __nv_bfloat16>(fast, D, rd, half));
 }
 
 struct CommitArgs {
@@ -307,16 +315,6 @@ __global__ void __launch_bounds__(1024) commit_kernel(const __grid_constant__ Co
     if (tid == 0) a.lens_out[b] = prefix + m;
 }
 
-template <typename TIn, typename TC, typename TQ>
-static void (*append_instance(bool fast, int D, bool half))(AppendNormArgs) {
-    return fast ? append_lane_instance<TIn, TC, TQ>(D, half) : append_norm_rows_kernel<TIn, TC, TQ>;
-}
-template <typename TIn>
-static void (*append_norm_instance(bool cache32, bool q32, bool fast, int D, bool half))(AppendNormArgs) {
-    return cache32 ? (q32 ? append_instance<TIn, float, float>(fast, D, half) : append_instance<TIn, float, __nv_bfloat16>(fast, D, half))
-                   : (q32 ? append_instance<TIn, __nv_bfloat16, float>(fast, D, half) : append_instance<TIn, __nv_bfloat16, __nv_bfloat16>(fast, D, half));
-}
-
 // seq_lens += nodes of the sequences that the append has taken: it raises no flag of its own, so the conditions are formed again.
 __global__ void advance_nodes_kernel(const __grid_constant__ AppendNormArgs a) {
     __shared__ TreeMasks masks;
@@ -370,19 +368,19 @@ int grl_kv_append_norm(grl_device* dev, const grl_append_norm_params* p) {
     fill_rope_freq(dev, p->rope, &a.rope);
     a.status = dev->d_status;
     dev->status_dirty = true;
-    const bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0 && row_aligned(a.k_new, p->in_dtype, &a.ks, 1) && row_aligned(a.v_new, p->in_dtype, &a.vs, 1) &&
+    const bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0 && a.P < (1 << 16) && row_aligned(a.k_new, p->in_dtype, &a.ks, 1) && row_aligned(a.v_new, p->in_dtype, &a.vs, 1) &&
                       (!a.q_in || row_aligned(a.q_in, p->in_dtype, &a.qs, 1)) &&
                       ((uintptr_t)a.q_out | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages) % 16 == 0;
-    const int run = p->in_dtype == GRL_BF16 ? kRunOf<__nv_bfloat16> : kRunOf<float>;
-    const long long groups = fast ? 256 / row_lanes(a.D) : 8, per_node = fast ? 2 * ((a.Hkv + run - 1) / run) + (a.Hq + run - 1) / run : 2 * a.Hkv + a.Hq;
-    const long long need = (a.n_new * per_node + groups - 1) / groups, most = ((fast ? 3LL : 8LL) * dev->prop.multiProcessorCount + a.B - 1) / a.B;
+    // a CTA for two rows of each of its groups (a row of each warp in the other form), as many as the SMs hold at once
+    const long long rows = (long long)a.n_new * (2 * a.Hkv + a.Hq), per = fast ? 2 * 256 / row_lanes(a.D) : 8;
+    const long long need = (rows + per - 1) / per, most = ((fast ? 3LL : 8LL) * dev->prop.multiProcessorCount + a.B - 1) / a.B;
     int ctas = (int)(need < most ? need : most);
     const bool fused = p->update_lens && ctas <= 4;
     if (fused) ctas = 1;
     a.update_lens = fused ? 1 : 0;
     const bool half = p->rope.mode == GRL_ROPE_HALF;
-    auto kernel = p->in_dtype == GRL_F32 ? append_norm_instance<float>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, half)
-                                         : append_norm_instance<__nv_bfloat16>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, half);
+    auto kernel = p->in_dtype == GRL_F32 ? append_norm_instance<float>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, a.rope.rd, half)
+                                         : append_norm_instance<__nv_bfloat16>(p->kv.cache_dtype == GRL_F32, p->q_out_dtype == GRL_F32, fast, a.D, a.rope.rd, half);
     GRL_CUDA(launch_pdl(kernel, dim3(ctas, a.B), 256, 0, dev->stream, a));
     GRL_LAUNCHED("append_norm_kernel");
     if (p->update_lens && !fused) {

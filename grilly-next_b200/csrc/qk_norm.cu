@@ -75,87 +75,67 @@ __global__ void __launch_bounds__(256) qk_norm_rows_kernel(const __grid_constant
     }
 }
 
-// Rows of whole 8-element pieces on 16-byte boundaries: LANES threads a row, eight elements each (threads past the row's end idle).  Bound by HBM, each element read and
-// written once.  A thread group keeps its places in the rows, walks the heads of a token in runs, the next run's loads on their
-// way under the present one, and forms a token's angles (double precision) once for all of them; every group has an equal,
-// contiguous share of all runs, and steps from run to run without dividing.
-template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;      // rows of a run
-struct RunWalk {
-    int b, s, run;
-    __device__ __forceinline__ void start(long long item, int S, int runs) {
-        const long long tok = item / runs;
-        run = (int)(item - tok * runs);
-        b = (int)(tok / S);
-        s = (int)(tok - (long long)b * S);
-    }
-    __device__ __forceinline__ void step(int S, int runs) {
-        if (++run < runs) return;
-        run = 0;
-        if (++s < S) return;
-        s = 0;
-        ++b;
-    }
-};
-template <typename TIn, typename TOut, int LANES, bool HALF>
+// Rows of whole 8-element pieces on 16-byte boundaries: LANES threads a row, eight elements each (threads past the row's end idle).  Bound by
+// HBM as to bytes, and nearly as much by instructions, so those are few: two elements an operation; weight, rotation and angle as four
+// factors for all heads of a token; addresses a step from head to head.  Every warp has an equal, contiguous share of the rows (token, head)
+// and walks it in segments, heads of one token and one side: its groups take the heads in turn, RUN rows of each in flight, the next one
+// asked for as soon as its registers are free.
+template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;
+template <typename TIn, typename TOut, int LANES, bool HALF, bool FULL>
 __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__ NormArgs a) {
-    constexpr int RUN = kRunOf<TIn>;
+    constexpr int RUN = kRunOf<TIn>, GPW = 32 / LANES;
     __shared__ __align__(16) RowTables tables;
-    const int l = threadIdx.x % LANES, D = a.D;
-    const bool on = 8 * l < D;
+    const int l = threadIdx.x % LANES, g = (threadIdx.x & 31) / LANES, D = FULL ? 8 * LANES : a.D;
+    const bool on = FULL || 8 * l < D;
     const float inv_d = 1.f / D;
-    const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    const int q_runs = (a.q.H + RUN - 1) / RUN, runs = q_runs + (a.k.H + RUN - 1) / RUN;
-    const long long total = (long long)a.B * a.S * runs, all = (long long)gridDim.x * (256 / LANES), mine = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const long long lo = mine * total / all;
-    const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);      // of the group; of any group: the
-                                                                        // groups of a warp take the same trips, for the shuffles
+    const RowPlace at = row_place<HALF>(l, FULL ? D : a.rope.rd);
+    const int gap = FULL && HALF ? 4 * LANES : at.gap();
+    const int hq = a.q.H, slots = hq + a.k.H;
+    const Share share((long long)a.B * a.S * slots);
+    const long long tok = share.lo / slots;
+    int slot = (int)(share.lo - tok * slots), b = (int)(tok / a.S), s = (int)(tok - (long long)b * a.S), left = share.items;
     pdl_wait();
     pdl_trigger();
-    RunWalk at_run;
-    at_run.start(items > 0 ? lo : 0, a.S, runs);
-    RowRaw<TIn> raw[RUN];
-    auto fetch = [&](const RunWalk& w, bool live) {
-        const bool is_k = w.run >= q_runs;
-        const NormSide& side = is_k ? a.k : a.q;
-        const int h0 = (is_k ? w.run - q_runs : w.run) * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
-        const TIn* in = reinterpret_cast<const TIn*>(side.x) + w.b * side.xs[0] + w.s * side.xs[1] + h0 * side.xs[2];
+    row_tables(tables, a.rope, D, a.q.w, a.k.w);
+    __syncthreads();
+    Pairs angle;
+    bool fresh = true;              // a token whose angles are not formed yet
+    while (left > 0) {
+        const bool is_k = slot >= hq;
+        const int n = min(left, (is_k ? slots : hq) - slot), h0 = is_k ? slot - hq : slot;
+        const long long* xs = is_k ? a.k.xs : a.q.xs;
+        const long long* ys = is_k ? a.k.ys : a.q.ys;
+        const int x_step = (int)xs[2] * GPW, y_step = (int)ys[2] * GPW;
+        const TIn* in = reinterpret_cast<const TIn*>(is_k ? a.k.x : a.q.x) + (b * xs[0] + s * xs[1] + (h0 + g) * xs[2] + at.o0);
+        TOut* out = reinterpret_cast<TOut*>(is_k ? a.k.y : a.q.y) + (b * ys[0] + s * ys[1] + (h0 + g) * ys[2] + at.o0);
+        RowRaw<TIn> raw[RUN];
 #pragma unroll
         for (int h = 0; h < RUN; ++h)
-            if (h < heads) row_fetch<HALF>(in + h * side.xs[2], at, raw[h]);
+            if (on && g + GPW * h < n) row_fetch<HALF>(in + (long long)h * x_step, gap, raw[h]);
             else row_zero(raw[h]);
-    };
-    fetch(at_run, items > 0);
-    row_tables<HALF>(tables, a.rope, D, a.q.w, a.k.w);
-    __syncthreads();
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-    bool fresh = true;          // a token whose angles are not formed yet
-    for (int i = 0; i < most; ++i) {
-        const RunWalk now = at_run;
-        RowRaw<TIn> x_raw[RUN];
+        if (fresh) {
+            angle = row_angles(tables, l, a.rope.gain, at.turned, position_of(a, b, s));
+            fresh = false;
+        }
+        const Turn turn = weighted_turn(row_weights<HALF>(tables.w[is_k], at), angle);
+        for (int i = g; i < n + g; i += GPW * RUN) {
+            in += (long long)RUN * x_step;
 #pragma unroll
-        for (int h = 0; h < RUN; ++h) x_raw[h] = raw[h];
-        const bool live = i < items;
-        at_run.step(a.S, runs);
-        if (i + 1 < most) fetch(at_run, i + 1 < items);
-        if (live && fresh) row_angles(tables, l, a.rope.gain, at.turned, position_of(a, now.b, now.s), c, s);
-        fresh = at_run.run == 0;
-        const bool is_k = now.run >= q_runs;
-        const NormSide& side = is_k ? a.k : a.q;
-        const int h0 = (is_k ? now.run - q_runs : now.run) * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
-        TOut* out = reinterpret_cast<TOut*>(side.y) + now.b * side.ys[0] + now.s * side.ys[1] + h0 * side.ys[2];
-        float w[8];
-        row_weights(tables.w[is_k], at, w);
-#pragma unroll
-        for (int h = 0; h < RUN; ++h) {
-            float x[8], sum = 0.f;
-            row_unpack(x_raw[h], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-            const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
-            row_turn<HALF, false>(x, c, s, at.turned);
-            if (h < heads) row_store<HALF>(out + h * side.ys[2], at, x);
+            for (int h = 0; h < RUN; ++h) {
+                Pairs x = row_pairs<HALF>(raw[h]);
+                if (on && i + GPW * (RUN + h) < n) row_fetch<HALF>(in + (long long)h * x_step, gap, raw[h]);
+                const float r = rsqrtf(row_sum<LANES>(squares(x)) * inv_d + a.eps);
+                turn_scaled(x, turn, r);
+                if (on && i + GPW * h < n) row_store<HALF>(out + (long long)h * y_step, gap, x);
+            }
+            out += (long long)RUN * y_step;
+        }
+        slot += n;
+        left -= n;
+        if (slot == slots) {
+            slot = 0;
+            fresh = true;
+            if (++s == a.S) { s = 0; ++b; }
         }
     }
 }
@@ -163,85 +143,88 @@ __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__
 // The backward pass in the same form, the queries and then the keys; a group keeps its share of the weight's gradient in registers, the CTA adds
 // them in order of its groups.
 template <typename T> constexpr int kGradRunOf = sizeof(T) == 2 ? 2 : 1;
-template <typename TIn, typename TOut, int LANES, bool HALF>
+template <typename TIn, typename TOut, int LANES, bool HALF, bool FULL>
 __global__ void __launch_bounds__(256, 3) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
-    constexpr int GROUPS = 256 / LANES, RUN = kGradRunOf<TIn>;
+    constexpr int GROUPS = 256 / LANES, RUN = kGradRunOf<TIn>, GPW = 32 / LANES;
     __shared__ __align__(16) RowTables tables;
     __shared__ __align__(16) float sm[GROUPS][8 * LANES];
-    const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, D = a.D;
-    const bool on = 8 * l < D;
+    const int l = threadIdx.x % LANES, g = (threadIdx.x & 31) / LANES, D = FULL ? 8 * LANES : a.D;
+    const bool on = FULL || 8 * l < D;
     const float inv_d = 1.f / D;
-    const RowPlace at = row_place<HALF>(l, a.rope.rd);
-    const long long all = (long long)gridDim.x * GROUPS, mine = (long long)blockIdx.x * GROUPS + group;
+    const RowPlace at = row_place<HALF>(l, FULL ? D : a.rope.rd);
+    const int gap = FULL && HALF ? 4 * LANES : at.gap();
     pdl_wait();
-    row_tables<HALF>(tables, a.rope, D, a.q.w, a.k.w);
+    row_tables(tables, a.rope, D, a.q.w, a.k.w);
     __syncthreads();
 #pragma unroll 1
     for (int side_i = 0; side_i < 2; ++side_i) {
         const NormSide& side = side_i ? a.k : a.q;
-        const int runs = (side.H + RUN - 1) / RUN;
-        const long long total = (long long)a.B * a.S * runs, lo = mine * total / all;
-        const int items = (int)((mine + 1) * total / all - lo), most = (int)((total + all - 1) / all);
-        RunWalk at_run{0, 0, 0};
-        if (items > 0) at_run.start(lo, a.S, runs);
-        RowRaw<TIn> xr[RUN];
-        RowRaw<TOut> gr[RUN];
-        auto fetch = [&](const RunWalk& w, bool live) {
-            const int h0 = w.run * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
-            const TIn* in = reinterpret_cast<const TIn*>(side.x) + w.b * side.xs[0] + w.s * side.xs[1] + h0 * side.xs[2];
-            const TOut* dy = reinterpret_cast<const TOut*>(side.dy) + w.b * side.dys[0] + w.s * side.dys[1] + h0 * side.dys[2];
-#pragma unroll
-            for (int h = 0; h < RUN; ++h)
-                if (h < heads) {
-                    row_fetch<HALF>(in + h * side.xs[2], at, xr[h]);
-                    row_fetch<HALF>(dy + h * side.dys[2], at, gr[h]);
+        const int H = side.H;
+        if (!H) continue;
+        const int x_step = (int)side.xs[2] * GPW, dy_step = (int)side.dys[2] * GPW, dx_step = (int)side.ys[2] * GPW;
+        const Share share((long long)a.B * a.S * H);
+        const long long tok = share.lo / H;
+        int h0 = (int)(share.lo - tok * H), b = (int)(tok / a.S), s = (int)(tok - (long long)b * a.S), left = share.items;
+        const Pairs w = row_weights<HALF>(tables.w[side_i], at);
+        Pairs acc;
+        acc.f[0] = acc.f[1] = acc.g[0] = acc.g[1] = make_float2(0.f, 0.f);
+        while (left > 0) {
+            const int n = min(left, H - h0);
+            const TIn* x_at = reinterpret_cast<const TIn*>(side.x) + (b * side.xs[0] + s * side.xs[1] + (h0 + g) * side.xs[2] + at.o0);
+            const TOut* dy_at = reinterpret_cast<const TOut*>(side.dy) + (b * side.dys[0] + s * side.dys[1] + (h0 + g) * side.dys[2] + at.o0);
+            TIn* dx_at = reinterpret_cast<TIn*>(side.y) + (b * side.ys[0] + s * side.ys[1] + (h0 + g) * side.ys[2] + at.o0);
+            RowRaw<TIn> x_raw[RUN];
+            RowRaw<TOut> dy_raw[RUN];
+            auto ask = [&](int i, int h) {
+                if (on && i + GPW * h < n) {
+                    row_fetch<HALF>(x_at + (long long)h * x_step, gap, x_raw[h]);
+                    row_fetch<HALF>(dy_at + (long long)h * dy_step, gap, dy_raw[h]);
                 } else {
-                    row_zero(xr[h]);
-                    row_zero(gr[h]);
+                    row_zero(x_raw[h]);
+                    row_zero(dy_raw[h]);
                 }
-        };
-        if (most > 0) fetch(at_run, items > 0);
-        float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, acc[8], w[8];
-        row_weights(tables.w[side_i], at, w);
+            };
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-        bool fresh = true;
-        for (int i = 0; i < most; ++i) {
-            const RunWalk now = at_run;
-            RowRaw<TIn> xn[RUN];
-            RowRaw<TOut> gn[RUN];
+            for (int h = 0; h < RUN; ++h) ask(g, h);
+            const Pairs angle = row_angles(tables, l, a.rope.gain, at.turned, position_of(a, b, s));
+            for (int i = g; i < n + g; i += GPW * RUN) {
+                x_at += (long long)RUN * x_step;
+                dy_at += (long long)RUN * dy_step;
 #pragma unroll
-            for (int h = 0; h < RUN; ++h) { xn[h] = xr[h]; gn[h] = gr[h]; }
-            const bool live = i < items;
-            at_run.step(a.S, runs);
-            if (i + 1 < most) fetch(at_run, i + 1 < items);
-            if (live && fresh) row_angles(tables, l, a.rope.gain, at.turned, position_of(a, now.b, now.s), c, s);
-            fresh = at_run.run == 0;
-            const int h0 = now.run * RUN, heads = live && on ? min(RUN, side.H - h0) : 0;
-            TIn* dx = reinterpret_cast<TIn*>(side.y) + now.b * side.ys[0] + now.s * side.ys[1] + h0 * side.ys[2];
+                for (int h = 0; h < RUN; ++h) {
+                    Pairs x = row_pairs<HALF>(x_raw[h]);
+                    const Pairs y = row_pairs<HALF>(dy_raw[h]);
+                    ask(i + GPW * RUN, h);
+                    Pairs gr, wg;
+                    float2 dot = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int h = 0; h < RUN; ++h) {
-                float x[8], g[8], sum = 0.f, dot = 0.f;
-                row_unpack(xn[h], x);
-                row_unpack(gn[h], g);
-                row_turn<HALF, true>(g, c, s, at.turned);
+                    for (int e = 0; e < 2; ++e) {
+                        gr.f[e] = __ffma2_rn(y.g[e], angle.g[e], __fmul2_rn(y.f[e], angle.f[e]));
+                        gr.g[e] = __ffma2_rn(neg2(y.f[e]), angle.g[e], __fmul2_rn(y.g[e], angle.f[e]));
+                        wg.f[e] = __fmul2_rn(gr.f[e], w.f[e]);
+                        wg.g[e] = __fmul2_rn(gr.g[e], w.g[e]);
+                        dot = __ffma2_rn(wg.f[e], x.f[e], dot);
+                        dot = __ffma2_rn(wg.g[e], x.g[e], dot);
+                    }
+                    const float r = rsqrtf(row_sum<LANES>(squares(x)) * inv_d + a.eps);
+                    const float2 rr = twice(r), back = twice(-row_sum<LANES>(dot.x + dot.y) * inv_d * r * r);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum = fmaf(x[e], x[e], sum);
-                    dot = fmaf(g[e] * w[e], x[e], dot);
+                    for (int e = 0; e < 2; ++e) {
+                        acc.f[e] = __ffma2_rn(gr.f[e], __fmul2_rn(x.f[e], rr), acc.f[e]);
+                        acc.g[e] = __ffma2_rn(gr.g[e], __fmul2_rn(x.g[e], rr), acc.g[e]);
+                        x.f[e] = __fmul2_rn(__ffma2_rn(x.f[e], back, wg.f[e]), rr);
+                        x.g[e] = __fmul2_rn(__ffma2_rn(x.g[e], back, wg.g[e]), rr);
+                    }
+                    if (on && i + GPW * h < n) row_store<HALF>(dx_at + (long long)h * dx_step, gap, x);
                 }
-                const float r = rsqrtf(row_sum<LANES>(sum) * inv_d + a.eps), f = row_sum<LANES>(dot) * inv_d * r * r;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    acc[e] = fmaf(g[e], x[e] * r, acc[e]);
-                    x[e] = r * (g[e] * w[e] - x[e] * f);
-                }
-                if (h < heads) row_store<HALF>(dx + h * side.ys[2], at, x);
+                dx_at += (long long)RUN * dx_step;
             }
+            left -= n;
+            h0 = 0;
+            if (++s == a.S) { s = 0; ++b; }
         }
-        if (side_i == 1) pdl_trigger();
         if (!a.part) continue;
-        if (on) row_store<HALF>(sm[group], at, acc);
+        if (on) row_store<HALF>(sm[threadIdx.x / LANES] + at.o0, gap, acc);
         __syncthreads();
         if (threadIdx.x < D) {
             float sum = 0.f;
@@ -251,27 +234,29 @@ __global__ void __launch_bounds__(256, 3) qk_norm_backward_kernel(const __grid_c
         }
         __syncthreads();
     }
+    pdl_trigger();
 }
 
+template <typename TIn, typename TOut, bool BACK, int LANES>
+static void (*form_instance(bool half, bool full))(NormArgs) {
+    if constexpr (BACK)
+        return half ? (full ? qk_norm_backward_kernel<TIn, TOut, LANES, true, true> : qk_norm_backward_kernel<TIn, TOut, LANES, true, false>)
+                    : (full ? qk_norm_backward_kernel<TIn, TOut, LANES, false, true> : qk_norm_backward_kernel<TIn, TOut, LANES, false, false>);
+    else
+        return half ? (full ? qk_norm_kernel<TIn, TOut, LANES, true, true> : qk_norm_kernel<TIn, TOut, LANES, true, false>)
+                    : (full ? qk_norm_kernel<TIn, TOut, LANES, false, true> : qk_norm_kernel<TIn, TOut, LANES, false, false>);
+}
 template <typename TIn, typename TOut, bool BACK>
-static void (*lane_instance(int D, bool half))(NormArgs) {
-    if constexpr (BACK) {
-        return D <= 32 ? (half ? qk_norm_backward_kernel<TIn, TOut, 4, true> : qk_norm_backward_kernel<TIn, TOut, 4, false>)
-             : D <= 64 ? (half ? qk_norm_backward_kernel<TIn, TOut, 8, true> : qk_norm_backward_kernel<TIn, TOut, 8, false>)
-             : D <= 128 ? (half ? qk_norm_backward_kernel<TIn, TOut, 16, true> : qk_norm_backward_kernel<TIn, TOut, 16, false>)
-                        : (half ? qk_norm_backward_kernel<TIn, TOut, 32, true> : qk_norm_backward_kernel<TIn, TOut, 32, false>);
-    } else {
-        return D <= 32 ? (half ? qk_norm_kernel<TIn, TOut, 4, true> : qk_norm_kernel<TIn, TOut, 4, false>)
-             : D <= 64 ? (half ? qk_norm_kernel<TIn, TOut, 8, true> : qk_norm_kernel<TIn, TOut, 8, false>)
-             : D <= 128 ? (half ? qk_norm_kernel<TIn, TOut, 16, true> : qk_norm_kernel<TIn, TOut, 16, false>)
-                        : (half ? qk_norm_kernel<TIn, TOut, 32, true> : qk_norm_kernel<TIn, TOut, 32, false>);
-    }
+static void (*lane_instance(int D, int rd, bool half))(NormArgs) {
+    const bool full = row_full(D, rd);
+    return D <= 32 ? form_instance<TIn, TOut, BACK, 4>(half, full) : D <= 64 ? form_instance<TIn, TOut, BACK, 8>(half, full)
+         : D <= 128 ? form_instance<TIn, TOut, BACK, 16>(half, full) : form_instance<TIn, TOut, BACK, 32>(half, full);
 }
 template <bool BACK>
-static void (*instance(const grl_qk_norm_params& f))(NormArgs) {
+static void (*instance(const grl_qk_norm_params& f, int rd))(NormArgs) {
     const bool in32 = f.in_dtype == GRL_F32, out32 = f.out_dtype == GRL_F32, half = f.rope.mode == GRL_ROPE_HALF;
-    return in32 ? (out32 ? lane_instance<float, float, BACK>(f.head_dim, half) : lane_instance<float, __nv_bfloat16, BACK>(f.head_dim, half))
-                : (out32 ? lane_instance<__nv_bfloat16, float, BACK>(f.head_dim, half) : lane_instance<__nv_bfloat16, __nv_bfloat16, BACK>(f.head_dim, half));
+    return in32 ? (out32 ? lane_instance<float, float, BACK>(f.head_dim, rd, half) : lane_instance<float, __nv_bfloat16, BACK>(f.head_dim, rd, half))
+                : (out32 ? lane_instance<__nv_bfloat16, float, BACK>(f.head_dim, rd, half) : lane_instance<__nv_bfloat16, __nv_bfloat16, BACK>(f.head_dim, rd, half));
 }
 
 // Backward, a warp a row:  g = R^T dy,  dw += g * x r,  dx = r (w g - x r^2 mean(w g x)).
@@ -378,7 +363,13 @@ __global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __res
     const int d = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
     double sum = 0.0;
     if (d < D)
-        for (int c = g; c < ctas; c += 32) sum += (double)part[((size_t)c * 2 + blockIdx.y) * D + d];
+        for (int c0 = g; c0 < ctas; c0 += 32 * 8) {         // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c0 + 32 * j < ctas ? __ldcg(part + ((size_t)(c0 + 32 * j) * 2 + blockIdx.y) * D + d) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += (double)v[j];
+        }
     sm[g][threadIdx.x & 31] = sum;
     __syncthreads();
     if (g == 0 && d < D) {
@@ -444,6 +435,12 @@ static int side_args(const grl_qk_norm_params& f, bool key, NormSide* s) {
     for (long long v : s->xs) GRL_REQUIRE(v >= 0, "strides must not be negative");
     return GRL_OK;
 }
+// Whether a side's rows serve the eight-element form.
+static bool side_fits(const NormSide& s, int in_dtype, int x_dtype, int out_dtype, bool back) {
+    const auto near = [](const long long* st) { return st[2] < (1LL << 27); };      // steps of eight heads fit 32 bits
+    return !s.H || (row_aligned(s.x, in_dtype, s.xs, 3) && near(s.xs) && row_aligned(s.y, x_dtype, s.ys, 3) && near(s.ys) &&
+                    (!back || (row_aligned(s.dy, out_dtype, s.dys, 3) && near(s.dys))));
+}
 
 static int check_norm(const grl_qk_norm_params& f, NormArgs* a) {
     GRL_REQUIRE(f.q, "q is NULL");
@@ -507,14 +504,12 @@ int grl_qk_norm_rope(grl_device* dev, const grl_qk_norm_params* p) {
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->rope, &a.rope);
     const long long rows = (long long)a.B * a.S * (a.q.H + a.k.H), most = 8LL * dev->prop.multiProcessorCount;
-    bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0;
-    for (const NormSide* s : {&a.q, &a.k})
-        if (s->H) fast = fast && row_aligned(s->x, p->in_dtype, s->xs, 3) && row_aligned(s->y, p->out_dtype, s->ys, 3);
+    const bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0 && side_fits(a.q, p->in_dtype, p->out_dtype, 0, false) &&
+                      side_fits(a.k, p->in_dtype, p->out_dtype, 0, false);
     if (fast) {
-        const int run = p->in_dtype == GRL_BF16 ? kRunOf<__nv_bfloat16> : kRunOf<float>;
-        const long long runs = (long long)a.B * a.S * ((a.q.H + run - 1) / run + (a.k.H + run - 1) / run), groups = 256 / row_lanes(a.D);
-        const long long need = (runs + groups - 1) / groups, held = 3LL * dev->prop.multiProcessorCount;
-        GRL_CUDA(launch_pdl(instance<false>(*p), dim3((unsigned)(need < held ? need : held)), 256, 0, dev->stream, a));
+        // a CTA for two rows of each of its groups, as many as the SMs hold at once
+        const long long two = 2 * 256 / row_lanes(a.D), need = (rows + two - 1) / two, held = 3LL * dev->prop.multiProcessorCount;
+        GRL_CUDA(launch_pdl(instance<false>(*p, a.rope.rd), dim3((unsigned)(need < held ? need : held)), 256, 0, dev->stream, a));
         GRL_LAUNCHED("qk_norm_kernel");
         return GRL_OK;
     }
@@ -550,13 +545,10 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
     }
     DeviceGuard g(dev->ordinal);
     fill_rope_freq(dev, p->fwd.rope, &a.rope);
-    bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0;
-    for (const NormSide* s : {&a.q, &a.k})
-        if (s->H)
-            fast = fast && row_aligned(s->x, p->fwd.in_dtype, s->xs, 3) && row_aligned(s->y, p->fwd.in_dtype, s->ys, 3) &&
-                   row_aligned(s->dy, p->fwd.out_dtype, s->dys, 3);
+    const bool fast = a.D % 8 == 0 && a.rope.rd % 8 == 0 && side_fits(a.q, p->fwd.in_dtype, p->fwd.in_dtype, p->fwd.out_dtype, true) &&
+                      side_fits(a.k, p->fwd.in_dtype, p->fwd.in_dtype, p->fwd.out_dtype, true);
     const bool in32 = p->fwd.in_dtype == GRL_F32, out32 = p->fwd.out_dtype == GRL_F32;
-    auto kernel = fast ? instance<true>(p->fwd)
+    auto kernel = fast ? instance<true>(p->fwd, a.rope.rd)
                 : in32 ? (out32 ? qk_norm_rows_backward_kernel<float, float> : qk_norm_rows_backward_kernel<float, __nv_bfloat16>)
                        : (out32 ? qk_norm_rows_backward_kernel<__nv_bfloat16, float> : qk_norm_rows_backward_kernel<__nv_bfloat16, __nv_bfloat16>);
     if (fast) GRL_CUDA(launch_pdl(kernel, dim3(ctas), 256, 0, dev->stream, a));

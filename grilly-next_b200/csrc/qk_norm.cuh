@@ -25,6 +25,8 @@ inline bool row_aligned(const void* p, int dtype, const long long* strides, int 
     for (int i = 0; i < n; ++i) ok = ok && strides[i] % unit == 0;
     return ok;
 }
+// FULL: every thread of a row has elements and all of them are turned, so that the gap is known to the compiler.
+inline bool row_full(int D, int rd) { return rd == D && (D == 32 || D == 64 || D == 128 || D == 256); }
 inline int row_lanes(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }      // threads of a row
 
 #ifdef __CUDACC__
@@ -48,6 +50,7 @@ __device__ __forceinline__ void pair_angle(const RopeArgs& r, int j, int pos, fl
 struct RowPlace {
     int o0, o1;
     bool turned;
+    __device__ __forceinline__ int gap() const { return o1 - o0; }
 };
 template <bool HALF>
 __device__ __forceinline__ RowPlace row_place(int l, int rd) {
@@ -57,31 +60,24 @@ __device__ __forceinline__ RowPlace row_place(int l, int rd) {
     p.o1 = HALF && p.turned ? p.o0 + rd / 2 : p.o0 + 4;
     return p;
 }
-__device__ __forceinline__ void unpack_bf16(uint32_t w, float& a, float& b) {
-    a = __uint_as_float(w << 16);
-    b = __uint_as_float(w & 0xffff0000u);
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 // A thread's part of a row as it lies in memory: what is on its way for later rows takes no more registers than that.
 template <typename T> struct RowRaw {
     uint32_t w[sizeof(T) * 2];
 };
+// p: the thread's o0 in the row, gap: o1 - o0
 template <bool HALF>
-__device__ __forceinline__ void row_fetch(const float* p, const RowPlace& at, RowRaw<float>& r) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + at.o0)), b = __ldcs(reinterpret_cast<const uint4*>(p + at.o1));
+__device__ __forceinline__ void row_fetch(const float* p, int gap, RowRaw<float>& r) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p)), b = __ldcs(reinterpret_cast<const uint4*>(p + (HALF ? gap : 4)));
     r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
     r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
 }
 template <bool HALF>
-__device__ __forceinline__ void row_fetch(const __nv_bfloat16* p, const RowPlace& at, RowRaw<__nv_bfloat16>& r) {
+__device__ __forceinline__ void row_fetch(const __nv_bfloat16* p, int gap, RowRaw<__nv_bfloat16>& r) {
     if constexpr (HALF) {
-        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p + at.o0)), b = __ldcs(reinterpret_cast<const uint2*>(p + at.o1));
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p)), b = __ldcs(reinterpret_cast<const uint2*>(p + gap));
         r.w[0] = a.x; r.w[1] = a.y; r.w[2] = b.x; r.w[3] = b.y;
     } else {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + at.o0));
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
         r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
     }
 }
@@ -90,29 +86,63 @@ __device__ __forceinline__ void row_zero(RowRaw<T>& r) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) * 2; ++i) r.w[i] = 0u;
 }
-__device__ __forceinline__ void row_unpack(const RowRaw<float>& r, float (&x)[8]) {
+// The pairs of a thread's eight elements, two to a packed operation: f the first ones, g the second ones (f and g lie side by side
+// where neighbours are turned, in the two halves where halves are).
+struct Pairs {
+    float2 f[2], g[2];
+};
+__device__ __forceinline__ float2 both(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 lows(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a << 16), __uint_as_float(b << 16)); }
+__device__ __forceinline__ float2 highs(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)); }
+template <bool HALF>
+__device__ __forceinline__ Pairs row_pairs(const RowRaw<__nv_bfloat16>& r) {
+    Pairs p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        p.f[i] = HALF ? both(r.w[i]) : lows(r.w[2 * i], r.w[2 * i + 1]);
+        p.g[i] = HALF ? both(r.w[2 + i]) : highs(r.w[2 * i], r.w[2 * i + 1]);
+    }
+    return p;
+}
+template <bool HALF>
+__device__ __forceinline__ Pairs pairs_of(const float (&x)[8]) {
+    Pairs p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        p.f[i] = HALF ? make_float2(x[2 * i], x[2 * i + 1]) : make_float2(x[4 * i], x[4 * i + 2]);
+        p.g[i] = HALF ? make_float2(x[4 + 2 * i], x[5 + 2 * i]) : make_float2(x[4 * i + 1], x[4 * i + 3]);
+    }
+    return p;
+}
+template <bool HALF>
+__device__ __forceinline__ Pairs row_pairs(const RowRaw<float>& r) {
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(r.w[e]);
+    return pairs_of<HALF>(x);
 }
-__device__ __forceinline__ void row_unpack(const RowRaw<__nv_bfloat16>& r, float (&x)[8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) unpack_bf16(r.w[e], x[2 * e], x[2 * e + 1]);
-}
-template <bool HALF>
-__device__ __forceinline__ void row_store(float* p, const RowPlace& at, const float (&y)[8]) {
-    *reinterpret_cast<float4*>(p + at.o0) = make_float4(y[0], y[1], y[2], y[3]);
-    *reinterpret_cast<float4*>(p + at.o1) = make_float4(y[4], y[5], y[6], y[7]);
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <bool HALF>
-__device__ __forceinline__ void row_store(__nv_bfloat16* p, const RowPlace& at, const float (&y)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(y[2 * e], y[2 * e + 1]);
+__device__ __forceinline__ void row_store(float* p, int gap, const Pairs& y) {
     if constexpr (HALF) {
-        *reinterpret_cast<uint2*>(p + at.o0) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(p + at.o1) = make_uint2(w[2], w[3]);
+        *reinterpret_cast<float4*>(p) = make_float4(y.f[0].x, y.f[0].y, y.f[1].x, y.f[1].y);
+        *reinterpret_cast<float4*>(p + gap) = make_float4(y.g[0].x, y.g[0].y, y.g[1].x, y.g[1].y);
     } else {
-        *reinterpret_cast<uint4*>(p + at.o0) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<float4*>(p) = make_float4(y.f[0].x, y.g[0].x, y.f[0].y, y.g[0].y);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(y.f[1].x, y.g[1].x, y.f[1].y, y.g[1].y);
+    }
+}
+template <bool HALF>
+__device__ __forceinline__ void row_store(__nv_bfloat16* p, int gap, const Pairs& y) {
+    if constexpr (HALF) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(y.f[0].x, y.f[0].y), pack_bf16x2(y.f[1].x, y.f[1].y));
+        *reinterpret_cast<uint2*>(p + gap) = make_uint2(pack_bf16x2(y.g[0].x, y.g[0].y), pack_bf16x2(y.g[1].x, y.g[1].y));
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(y.f[0].x, y.g[0].x), pack_bf16x2(y.f[0].y, y.g[0].y),
+                                                  pack_bf16x2(y.f[1].x, y.g[1].x), pack_bf16x2(y.f[1].y, y.g[1].y));
     }
 }
 template <int LANES>
@@ -121,47 +151,86 @@ __device__ __forceinline__ float row_sum(float v) {
     for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, LANES);
     return v;
 }
-// Frequencies of the pairs and the weights of both sides, in shared memory: a thread's own are read where they are used.
+// Turns per position (frequency / pi) of the pairs and the weights of both sides, in shared memory: read once for a token's heads.
 struct RowTables {
-    double freq[128];
+    double turns[128];
     float w[2][256];
 };
-template <bool HALF>
 __device__ __forceinline__ void row_tables(RowTables& t, const RopeArgs& r, int D, const float* w0, const float* w1) {
     for (int i = threadIdx.x; i < D; i += blockDim.x) {
         t.w[0][i] = w0 ? __ldg(w0 + i) : 1.f;
         t.w[1][i] = w1 ? __ldg(w1 + i) : 1.f;
-        if (2 * i < r.rd) t.freq[i] = r.inv_freq ? (double)__ldg(r.inv_freq + i) : r.freq.inv_freq[i];
+        if (2 * i < r.rd) t.turns[i] = (r.inv_freq ? (double)__ldg(r.inv_freq + i) : r.freq.inv_freq[i]) * 0.31830988618379067;     // 1 / pi
     }
 }
-__device__ __forceinline__ void row_weights(const float* w, const RowPlace& at, float (&x)[8]) {
+template <bool HALF>
+__device__ __forceinline__ Pairs row_weights(const float* w, const RowPlace& at) {
     const float4 a = *reinterpret_cast<const float4*>(w + at.o0), b = *reinterpret_cast<const float4*>(w + at.o1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return pairs_of<HALF>(x);
 }
-// cosine and sine of a thread's four pairs at a position; 1 and 0 where nothing turns
-__device__ __forceinline__ void row_angles(const RowTables& t, int l, float gain, bool turned, int pos, float (&c)[4], float (&s)[4]) {
+// Cosine (f) and sine (g) of a thread's four pairs at a position, times the gain; 1 and 0 where nothing turns.  The angle in units of pi is
+// formed and reduced to [-1, 1] in double, so that positions up to 2^24 keep some 1e-7 of a turn.
+__device__ __forceinline__ Pairs row_angles(const RowTables& t, int l, float gain, bool turned, int pos) {
+    Pairs a;
+    a.f[0] = a.f[1] = make_float2(1.f, 1.f);
+    a.g[0] = a.g[1] = make_float2(0.f, 0.f);
+    if (turned) {
+        float c[4], s[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        c[e] = 1.f;
-        s[e] = 0.f;
-        if (turned) {
-            rope_sincos(pos, t.freq[4 * l + e], &c[e], &s[e]);
-            c[e] *= gain;
-            s[e] *= gain;
+        for (int e = 0; e < 4; ++e) {
+            const double x = (double)pos * t.turns[4 * l + e];
+            sincospif((float)fma(-2.0, rint(0.5 * x), x), &s[e], &c[e]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            a.f[i] = make_float2(c[2 * i] * gain, c[2 * i + 1] * gain);
+            a.g[i] = make_float2(s[2 * i] * gain, s[2 * i + 1] * gain);
         }
     }
+    return a;
 }
-// The rotation of a thread's pairs; BACK: its transpose.
-template <bool HALF, bool BACK>
-__device__ __forceinline__ void row_turn(float (&x)[8], const float (&c)[4], const float (&s)[4], bool turned) {
-    if (!turned) return;
+// A warp's equal, contiguous share of `total` rows.
+struct Share {
+    long long lo;
+    int items;
+    __device__ __forceinline__ Share(long long total) {
+        const long long warps = (long long)gridDim.x * (blockDim.x >> 5), mine = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+        lo = mine * total / warps;
+        items = (int)((mine + 1) * total / warps - lo);
+    }
+};
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float squares(const Pairs& x) {
+    float2 s = __fmul2_rn(x.f[0], x.f[0]);
+    s = __ffma2_rn(x.f[1], x.f[1], s);
+    s = __ffma2_rn(x.g[0], x.g[0], s);
+    s = __ffma2_rn(x.g[1], x.g[1], s);
+    return s.x + s.y;
+}
+// Weight and rotation of a token's heads together: y_f = f ff + g fg, y_g = f gf + g gg.
+struct Turn {
+    float2 ff[2], fg[2], gf[2], gg[2];
+};
+__device__ __forceinline__ Turn weighted_turn(const Pairs& w, const Pairs& a) {
+    Turn t;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int i = HALF ? e : 2 * e, j = HALF ? e + 4 : 2 * e + 1;
-        const float sn = BACK ? -s[e] : s[e], a = x[i] * c[e] - x[j] * sn, b = x[i] * sn + x[j] * c[e];
-        x[i] = a;
-        x[j] = b;
+    for (int i = 0; i < 2; ++i) {
+        t.ff[i] = __fmul2_rn(w.f[i], a.f[i]);
+        t.fg[i] = neg2(__fmul2_rn(w.g[i], a.g[i]));
+        t.gf[i] = __fmul2_rn(w.f[i], a.g[i]);
+        t.gg[i] = __fmul2_rn(w.g[i], a.f[i]);
+    }
+    return t;
+}
+__device__ __forceinline__ void turn_scaled(Pairs& x, const Turn& t, float r) {
+    const float2 rr = twice(r);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 f = __fmul2_rn(__ffma2_rn(x.g[i], t.fg[i], __fmul2_rn(x.f[i], t.ff[i])), rr);
+        x.g[i] = __fmul2_rn(__ffma2_rn(x.g[i], t.gg[i], __fmul2_rn(x.f[i], t.gf[i])), rr);
+        x.f[i] = f;
     }
 }
 __device__ __forceinline__ float warp_sum(float v) {
