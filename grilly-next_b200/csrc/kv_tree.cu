@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256, 3) append_norm_kernel(const __grid_consta
     const RowPlace at = row_place<HALF>(l, FULL ? D : a.rope.rd);
     const int gap = FULL && HALF ? 4 * LANES : at.gap();
     const int slots = 2 * a.Hkv + a.Hq;
-    const Share share((long long)a.n_new * slots);
+    const Share share((long long)a.n_new * slots, blockIdx.x, gridDim.x);
     int t = (int)(share.lo / slots), slot = (int)(share.lo - (long long)t * slots), left = share.items;
     RowRaw<TIn> raw[RUN];
     const TIn* in = nullptr;

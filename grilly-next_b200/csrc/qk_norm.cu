@@ -18,7 +18,8 @@ struct NormArgs {
     float eps;
     const int32_t* positions;
     int pos_base;
-    float* part;        // backward: weight gradients of every CTA, [CTA][q, k][D]
+    float* part;        // backward: weight gradients of every CTA, [CTA][D]
+    int q_ctas;         // backward: the first CTAs take the queries, the others the keys
     RopeArgs rope;
 };
 
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__
     const RowPlace at = row_place<HALF>(l, FULL ? D : a.rope.rd);
     const int gap = FULL && HALF ? 4 * LANES : at.gap();
     const int hq = a.q.H, slots = hq + a.k.H;
-    const Share share((long long)a.B * a.S * slots);
+    const Share share((long long)a.B * a.S * slots, blockIdx.x, gridDim.x);
     const long long tok = share.lo / slots;
     int slot = (int)(share.lo - tok * slots), b = (int)(tok / a.S), s = (int)(tok - (long long)b * a.S), left = share.items;
     pdl_wait();
@@ -140,11 +141,11 @@ __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__
     }
 }
 
-// The backward pass in the same form, the queries and then the keys; a group keeps its share of the weight's gradient in registers, the CTA adds
-// them in order of its groups.
-template <typename T> constexpr int kGradRunOf = sizeof(T) == 2 ? 2 : 1;
+// The backward pass in the same form.  A CTA takes the queries or the keys, as many CTAs each as they have rows; a group keeps its share of the
+// weight's gradient in registers, the CTA adds them in order of its groups.
+template <typename T> constexpr int kGradRunOf = sizeof(T) == 2 ? 4 : 2;
 template <typename TIn, typename TOut, int LANES, bool HALF, bool FULL>
-__global__ void __launch_bounds__(256, 3) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(256, 2) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {
     constexpr int GROUPS = 256 / LANES, RUN = kGradRunOf<TIn>, GPW = 32 / LANES;
     __shared__ __align__(16) RowTables tables;
     __shared__ __align__(16) float sm[GROUPS][8 * LANES];
@@ -156,85 +157,81 @@ __global__ void __launch_bounds__(256, 3) qk_norm_backward_kernel(const __grid_c
     pdl_wait();
     row_tables(tables, a.rope, D, a.q.w, a.k.w);
     __syncthreads();
-#pragma unroll 1
-    for (int side_i = 0; side_i < 2; ++side_i) {
-        const NormSide& side = side_i ? a.k : a.q;
-        const int H = side.H;
-        if (!H) continue;
-        const int x_step = (int)side.xs[2] * GPW, dy_step = (int)side.dys[2] * GPW, dx_step = (int)side.ys[2] * GPW;
-        const Share share((long long)a.B * a.S * H);
-        const long long tok = share.lo / H;
-        int h0 = (int)(share.lo - tok * H), b = (int)(tok / a.S), s = (int)(tok - (long long)b * a.S), left = share.items;
-        const Pairs w = row_weights<HALF>(tables.w[side_i], at);
-        Pairs acc;
-        acc.f[0] = acc.f[1] = acc.g[0] = acc.g[1] = make_float2(0.f, 0.f);
-        while (left > 0) {
-            const int n = min(left, H - h0);
-            const TIn* x_at = reinterpret_cast<const TIn*>(side.x) + (b * side.xs[0] + s * side.xs[1] + (h0 + g) * side.xs[2] + at.o0);
-            const TOut* dy_at = reinterpret_cast<const TOut*>(side.dy) + (b * side.dys[0] + s * side.dys[1] + (h0 + g) * side.dys[2] + at.o0);
-            TIn* dx_at = reinterpret_cast<TIn*>(side.y) + (b * side.ys[0] + s * side.ys[1] + (h0 + g) * side.ys[2] + at.o0);
-            RowRaw<TIn> x_raw[RUN];
-            RowRaw<TOut> dy_raw[RUN];
-            auto ask = [&](int i, int h) {
-                if (on && i + GPW * h < n) {
-                    row_fetch<HALF>(x_at + (long long)h * x_step, gap, x_raw[h]);
-                    row_fetch<HALF>(dy_at + (long long)h * dy_step, gap, dy_raw[h]);
-                } else {
-                    row_zero(x_raw[h]);
-                    row_zero(dy_raw[h]);
-                }
-            };
-#pragma unroll
-            for (int h = 0; h < RUN; ++h) ask(g, h);
-            const Pairs angle = row_angles(tables, l, a.rope.gain, at.turned, position_of(a, b, s));
-            for (int i = g; i < n + g; i += GPW * RUN) {
-                x_at += (long long)RUN * x_step;
-                dy_at += (long long)RUN * dy_step;
-#pragma unroll
-                for (int h = 0; h < RUN; ++h) {
-                    Pairs x = row_pairs<HALF>(x_raw[h]);
-                    const Pairs y = row_pairs<HALF>(dy_raw[h]);
-                    ask(i + GPW * RUN, h);
-                    Pairs gr, wg;
-                    float2 dot = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        gr.f[e] = __ffma2_rn(y.g[e], angle.g[e], __fmul2_rn(y.f[e], angle.f[e]));
-                        gr.g[e] = __ffma2_rn(neg2(y.f[e]), angle.g[e], __fmul2_rn(y.g[e], angle.f[e]));
-                        wg.f[e] = __fmul2_rn(gr.f[e], w.f[e]);
-                        wg.g[e] = __fmul2_rn(gr.g[e], w.g[e]);
-                        dot = __ffma2_rn(wg.f[e], x.f[e], dot);
-                        dot = __ffma2_rn(wg.g[e], x.g[e], dot);
-                    }
-                    const float r = rsqrtf(row_sum<LANES>(squares(x)) * inv_d + a.eps);
-                    const float2 rr = twice(r), back = twice(-row_sum<LANES>(dot.x + dot.y) * inv_d * r * r);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        acc.f[e] = __ffma2_rn(gr.f[e], __fmul2_rn(x.f[e], rr), acc.f[e]);
-                        acc.g[e] = __ffma2_rn(gr.g[e], __fmul2_rn(x.g[e], rr), acc.g[e]);
-                        x.f[e] = __fmul2_rn(__ffma2_rn(x.f[e], back, wg.f[e]), rr);
-                        x.g[e] = __fmul2_rn(__ffma2_rn(x.g[e], back, wg.g[e]), rr);
-                    }
-                    if (on && i + GPW * h < n) row_store<HALF>(dx_at + (long long)h * dx_step, gap, x);
-                }
-                dx_at += (long long)RUN * dx_step;
+    const bool is_k = (int)blockIdx.x >= a.q_ctas;
+    const NormSide& side = is_k ? a.k : a.q;
+    const int H = side.H;
+    const int x_step = (int)side.xs[2] * GPW, dy_step = (int)side.dys[2] * GPW, dx_step = (int)side.ys[2] * GPW;
+    const Share share((long long)a.B * a.S * H, is_k ? blockIdx.x - a.q_ctas : blockIdx.x, is_k ? gridDim.x - a.q_ctas : a.q_ctas);
+    const long long tok = share.lo / H;
+    int h0 = (int)(share.lo - tok * H), b = (int)(tok / a.S), s = (int)(tok - (long long)b * a.S), left = share.items;
+    const Pairs w = row_weights<HALF>(tables.w[is_k], at);
+    Pairs acc;
+    acc.f[0] = acc.f[1] = acc.g[0] = acc.g[1] = make_float2(0.f, 0.f);
+    while (left > 0) {
+        const int n = min(left, H - h0);
+        const TIn* x_at = reinterpret_cast<const TIn*>(side.x) + (b * side.xs[0] + s * side.xs[1] + (h0 + g) * side.xs[2] + at.o0);
+        const TOut* dy_at = reinterpret_cast<const TOut*>(side.dy) + (b * side.dys[0] + s * side.dys[1] + (h0 + g) * side.dys[2] + at.o0);
+        TIn* dx_at = reinterpret_cast<TIn*>(side.y) + (b * side.ys[0] + s * side.ys[1] + (h0 + g) * side.ys[2] + at.o0);
+        RowRaw<TIn> x_raw[RUN];
+        RowRaw<TOut> dy_raw[RUN];
+        auto ask = [&](int i, int h) {
+            if (on && i + GPW * h < n) {
+                row_fetch<HALF>(x_at + (long long)h * x_step, gap, x_raw[h]);
+                row_fetch<HALF>(dy_at + (long long)h * dy_step, gap, dy_raw[h]);
+            } else {
+                row_zero(x_raw[h]);
+                row_zero(dy_raw[h]);
             }
-            left -= n;
-            h0 = 0;
-            if (++s == a.S) { s = 0; ++b; }
+        };
+#pragma unroll
+        for (int h = 0; h < RUN; ++h) ask(g, h);
+        const Pairs angle = row_angles(tables, l, a.rope.gain, at.turned, position_of(a, b, s));
+        for (int i = g; i < n + g; i += GPW * RUN) {
+            x_at += (long long)RUN * x_step;
+            dy_at += (long long)RUN * dy_step;
+#pragma unroll
+            for (int h = 0; h < RUN; ++h) {
+                Pairs x = row_pairs<HALF>(x_raw[h]);
+                const Pairs y = row_pairs<HALF>(dy_raw[h]);
+                ask(i + GPW * RUN, h);
+                Pairs gr, wg;
+                float2 dot = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    gr.f[e] = __ffma2_rn(y.g[e], angle.g[e], __fmul2_rn(y.f[e], angle.f[e]));
+                    gr.g[e] = __ffma2_rn(neg2(y.f[e]), angle.g[e], __fmul2_rn(y.g[e], angle.f[e]));
+                    wg.f[e] = __fmul2_rn(gr.f[e], w.f[e]);
+                    wg.g[e] = __fmul2_rn(gr.g[e], w.g[e]);
+                    dot = __ffma2_rn(wg.f[e], x.f[e], dot);
+                    dot = __ffma2_rn(wg.g[e], x.g[e], dot);
+                }
+                const float r = rsqrtf(row_sum<LANES>(squares(x)) * inv_d + a.eps);
+                const float2 rr = twice(r), back = twice(-row_sum<LANES>(dot.x + dot.y) * inv_d * r * r);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    acc.f[e] = __ffma2_rn(gr.f[e], __fmul2_rn(x.f[e], rr), acc.f[e]);
+                    acc.g[e] = __ffma2_rn(gr.g[e], __fmul2_rn(x.g[e], rr), acc.g[e]);
+                    x.f[e] = __fmul2_rn(__ffma2_rn(x.f[e], back, wg.f[e]), rr);
+                    x.g[e] = __fmul2_rn(__ffma2_rn(x.g[e], back, wg.g[e]), rr);
+                }
+                if (on && i + GPW * h < n) row_store<HALF>(dx_at + (long long)h * dx_step, gap, x);
+            }
+            dx_at += (long long)RUN * dx_step;
         }
-        if (!a.part) continue;
-        if (on) row_store<HALF>(sm[threadIdx.x / LANES] + at.o0, gap, acc);
-        __syncthreads();
-        if (threadIdx.x < D) {
-            float sum = 0.f;
-#pragma unroll 8
-            for (int j = 0; j < GROUPS; ++j) sum += sm[j][threadIdx.x];
-            a.part[((size_t)blockIdx.x * 2 + side_i) * D + threadIdx.x] = sum;
-        }
-        __syncthreads();
+        left -= n;
+        h0 = 0;
+        if (++s == a.S) { s = 0; ++b; }
     }
     pdl_trigger();
+    if (!a.part) return;
+    if (on) row_store<HALF>(sm[threadIdx.x / LANES] + at.o0, gap, acc);
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float sum = 0.f;
+#pragma unroll 8
+        for (int j = 0; j < GROUPS; ++j) sum += sm[j][threadIdx.x];
+        a.part[(size_t)blockIdx.x * D + threadIdx.x] = sum;
+    }
 }
 
 template <typename TIn, typename TOut, bool BACK, int LANES>
@@ -266,17 +263,15 @@ template <typename TIn, typename TOut>
 __global__ void __launch_bounds__(256) qk_norm_rows_backward_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float sm[256];
     const int lane = threadIdx.x & 31, pairs = a.D / 2;
-    const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
-    float acc[2][kPairs][2];
+    const bool is_k = (int)blockIdx.x >= a.q_ctas;
+    const NormSide& side = is_k ? a.k : a.q;
+    const int cta = is_k ? blockIdx.x - a.q_ctas : blockIdx.x, ctas = is_k ? gridDim.x - a.q_ctas : a.q_ctas;
+    float acc[kPairs][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < kPairs; ++e) acc[i][e][0] = acc[i][e][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const NormSide& side = i ? a.k : a.q;
+    for (int e = 0; e < kPairs; ++e) acc[e][0] = acc[e][1] = 0.f;
+    {
         const long long rows = (long long)a.B * a.S * side.H;
-        for (long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += warps) {
+        for (long long row = (long long)cta * 8 + (threadIdx.x >> 5); row < rows; row += 8LL * ctas) {
             const int h = (int)(row % side.H);
             const long long tok = row / side.H;
             const int s = (int)(tok % a.S), b = (int)(tok / a.S);
@@ -306,8 +301,8 @@ __global__ void __launch_bounds__(256) qk_norm_rows_backward_kernel(const __grid
 #pragma unroll
             for (int e = 0; e < kPairs; ++e) {
                 const int j = lane + 32 * e;
-                acc[i][e][0] = fmaf(g0[e], x0[e] * r, acc[i][e][0]);
-                acc[i][e][1] = fmaf(g1[e], x1[e] * r, acc[i][e][1]);
+                acc[e][0] = fmaf(g0[e], x0[e] * r, acc[e][0]);
+                acc[e][1] = fmaf(g1[e], x1[e] * r, acc[e][1]);
                 if (j < pairs && side.w) {
                     int d0, d1;
                     pair_place(a.rope, j, &d0, &d1);
@@ -331,42 +326,38 @@ __global__ void __launch_bounds__(256) qk_norm_rows_backward_kernel(const __grid
     }
     if (!a.part) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int w = 0; w < 8; ++w) {       // the warps of the CTA add in order
+        if ((int)(threadIdx.x >> 5) == w) {
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {       // the warps of the CTA add in order
-            if ((int)(threadIdx.x >> 5) == w) {
-#pragma unroll
-                for (int e = 0; e < kPairs; ++e) {
-                    const int j = lane + 32 * e;
-                    if (j < pairs) {
-                        int d0, d1;
-                        pair_place(a.rope, j, &d0, &d1);
-                        sm[d0] = (w ? sm[d0] : 0.f) + acc[i][e][0];
-                        sm[d1] = (w ? sm[d1] : 0.f) + acc[i][e][1];
-                    }
+            for (int e = 0; e < kPairs; ++e) {
+                const int j = lane + 32 * e;
+                if (j < pairs) {
+                    int d0, d1;
+                    pair_place(a.rope, j, &d0, &d1);
+                    sm[d0] = (w ? sm[d0] : 0.f) + acc[e][0];
+                    sm[d1] = (w ? sm[d1] : 0.f) + acc[e][1];
                 }
             }
-            __syncthreads();
         }
-        if ((int)threadIdx.x < a.D) a.part[((size_t)blockIdx.x * 2 + i) * a.D + threadIdx.x] = sm[threadIdx.x];
         __syncthreads();
     }
+    if ((int)threadIdx.x < a.D) a.part[(size_t)blockIdx.x * a.D + threadIdx.x] = sm[threadIdx.x];
 }
 
-// dw[d] = sum over the CTAs of part[CTA][side][d], in order of the CTAs for every thread group; in double, which costs nothing here.
-__global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __restrict__ part, int ctas, int D, float* dq, float* dk) {
+// dw[d] = sum of part[CTA][d] over the CTAs of a side, in the same order every time; in double, which costs nothing here.
+__global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __restrict__ part, int q_ctas, int ctas, int D, float* dq, float* dk) {
     __shared__ double sm[32][33];
     float* out = blockIdx.y ? dk : dq;
     pdl_wait();
     pdl_trigger();
     if (!out) return;
-    const int d = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+    const int d = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5, first = blockIdx.y ? q_ctas : 0, end = blockIdx.y ? ctas : q_ctas;
     double sum = 0.0;
     if (d < D)
-        for (int c0 = g; c0 < ctas; c0 += 32 * 8) {         // eight loads in flight
+        for (int c0 = first + g; c0 < end; c0 += 32 * 8) {         // eight loads in flight
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c0 + 32 * j < ctas ? __ldcg(part + ((size_t)(c0 + 32 * j) * 2 + blockIdx.y) * D + d) : 0.f;
+            for (int j = 0; j < 8; ++j) v[j] = c0 + 32 * j < end ? __ldcg(part + (size_t)(c0 + 32 * j) * D + d) : 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum += (double)v[j];
         }
@@ -374,16 +365,20 @@ __global__ void __launch_bounds__(1024) qk_norm_weight_kernel(const float* __res
     __syncthreads();
     if (g == 0 && d < D) {
         double t = 0.0;
+#pragma unroll
         for (int i = 0; i < 32; ++i) t += sm[i][threadIdx.x];
         out[d] = (float)t;
     }
 }
 
-// CTAs of the backward pass: what the GPU holds at once, or a warp a row.
-static int backward_ctas(grl_device* dev, const grl_qk_norm_params& f) {
-    const long long rows = (long long)f.batch * f.seq_len * f.num_q_heads, most = 3LL * dev->prop.multiProcessorCount;
-    const long long ctas = (rows + 7) / 8;
-    return (int)(ctas < most ? ctas : most);
+// CTAs of the backward pass: for two rows of each warp, as many as the SMs hold at once; the sides share them by their rows.
+static int backward_ctas(grl_device* dev, const grl_qk_norm_params& f, int* q_ctas) {
+    const long long tokens = (long long)f.batch * f.seq_len, heads = f.num_q_heads + (f.k ? f.num_kv_heads : 0);
+    const long long need = (tokens * heads + 15) / 16, most = 2LL * dev->prop.multiProcessorCount;
+    const int ctas = (int)(need < 2 ? 2 : need < most ? need : most);
+    const int q = (int)((ctas * (long long)f.num_q_heads + heads / 2) / heads);
+    *q_ctas = !f.k ? ctas : q < 1 ? 1 : q > ctas - 1 ? ctas - 1 : q;
+    return ctas;
 }
 
 int check_rope_spec(const grl_rope_spec& r, int head_dim, RopeArgs* out) {
@@ -527,7 +522,8 @@ int grl_qk_norm_rope_backward_workspace_bytes(grl_device* dev, const grl_qk_norm
     int rc = check_grad(p, &a);
     if (rc) return rc;
     GRL_REQUIRE(dev && bytes, "NULL argument");
-    *bytes = a.q.dw || a.k.dw ? (size_t)backward_ctas(dev, p->fwd) * 2 * a.D * sizeof(float) : 0;
+    int q_ctas;
+    *bytes = a.q.dw || a.k.dw ? (size_t)backward_ctas(dev, p->fwd, &q_ctas) * a.D * sizeof(float) : 0;
     return GRL_OK;
 }
 
@@ -536,9 +532,9 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
     int rc = check_grad(p, &a);
     if (rc) return rc;
     GRL_REQUIRE(dev, "dev is NULL");
-    const int ctas = backward_ctas(dev, p->fwd);
+    const int ctas = backward_ctas(dev, p->fwd, &a.q_ctas);
     if (a.q.dw || a.k.dw) {
-        const size_t need = (size_t)ctas * 2 * a.D * sizeof(float);
+        const size_t need = (size_t)ctas * a.D * sizeof(float);
         GRL_REQUIRE(p->workspace && p->workspace_bytes >= need, "workspace too small: %zu < %zu", p->workspace ? p->workspace_bytes : 0, need);
         GRL_REQUIRE((uintptr_t)p->workspace % 16 == 0, "workspace must be 16-byte aligned");
         a.part = static_cast<float*>(p->workspace);
@@ -555,7 +551,7 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
     else kernel<<<ctas, 256, 0, dev->stream>>>(a);
     GRL_LAUNCHED("qk_norm_backward_kernel");
     if (a.part) {
-        GRL_CUDA(launch_pdl(qk_norm_weight_kernel, dim3((a.D + 31) / 32, 2), 1024, 0, dev->stream, (const float*)a.part, ctas, a.D, a.q.dw, a.k.dw));
+        GRL_CUDA(launch_pdl(qk_norm_weight_kernel, dim3((a.D + 31) / 32, 2), 1024, 0, dev->stream, (const float*)a.part, a.q_ctas, ctas, a.D, a.q.dw, a.k.dw));
         GRL_LAUNCHED("qk_norm_weight_kernel");
     }
     return GRL_OK;

@@ -190,12 +190,12 @@ __device__ __forceinline__ Pairs row_angles(const RowTables& t, int l, float gai
     }
     return a;
 }
-// A warp's equal, contiguous share of `total` rows.
+// A warp's equal, contiguous share of the `total` rows that `ctas` CTAs have.
 struct Share {
     long long lo;
     int items;
-    __device__ __forceinline__ Share(long long total) {
-        const long long warps = (long long)gridDim.x * (blockDim.x >> 5), mine = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    __device__ __forceinline__ Share(long long total, int cta, int ctas) {
+        const long long warps = (long long)ctas * (blockDim.x >> 5), mine = (long long)cta * (blockDim.x >> 5) + (threadIdx.x >> 5);
         lo = mine * total / warps;
         items = (int)((mine + 1) * total / warps - lo);
     }

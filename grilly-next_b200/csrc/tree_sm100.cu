@@ -8,8 +8,9 @@
 //                scaled only where a maximum grew by more than 2^8
 // The two chains of products and softmax (t = 0, 1) are
 //   PAIR    two row tiles over the same stages, where there are more than 128 rows: a stage crosses shared memory once for 256 rows
-//   SPLIT   the even and the odd stages of one row tile, joined in the epilogue: one chain alone takes some 2000 cycles a stage,
-//           both 1150, and HBM brings a stage to every SM in 1400
+//   SPLIT   the even and the odd stages of one row tile, joined in the epilogue
+//   FOLD    up to 64 rows, twice in the tile: the first half of a chain's threads takes one stage of a pair, the second half the other.  P has zeros
+//           where a half's rows meet the other's keys, so that one product sums both; four streams are joined in the epilogue
 // The predicate is applied to the last stages only, those with nodes in them: a row has one bit for each of 128 nodes.  There, rows
 // of V past the sequence's end, which may hold anything, are cleared in shared memory ahead of the product, and so are elements
 // that are no finite number; rows that see such an element add it again in the epilogue, so that it reaches nobody else.
@@ -30,15 +31,19 @@ constexpr int BM = 128;             // rows of a tile (TMEM lanes)
 constexpr int BN = 64;              // tokens of a stage
 constexpr int kThreads = 384;
 constexpr int WARP_MMA0 = 0, WARP_TMA = 1, WARP_MMA1 = 2, WARP_SOFTMAX = 4;
+// Registers: the softmax warpgroups take what the first one gives up.  setmaxnreg.inc is served from what the CTA was launched with only.
+constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 208, REGS_MISC = 80;
+static_assert(2 * REGS_SOFTMAX + REGS_MISC <= 3 * REGS_LAUNCH && REGS_LAUNCH * kThreads <= 65536, "register budgets");
 constexpr int Q_BOX = BM * 128, KV_BOX = BN * 128;      // bytes of a 64-column box
 constexpr uint32_t TMEM_COLS = 512, TMEM_CHAIN = 256, TMEM_O = 128;     // a chain: two buffers of S (P overlays them), then O
 
-template <int HD, bool PAIR> struct Form {
+enum Mode { SPLIT, PAIR, FOLD };
+template <int HD, Mode MODE> struct Form {
     static constexpr int BOXES = HD / 64;
     static constexpr int SLAB = BOXES * KV_BOX;             // K (or V) of a stage
     static constexpr int STAGE = 2 * SLAB;
     static constexpr int Q_TILE = BOXES * Q_BOX;
-    static constexpr int Q_BYTES = (PAIR ? 2 : 1) * Q_TILE;
+    static constexpr int Q_BYTES = (MODE == PAIR ? 2 : 1) * Q_TILE;
     static constexpr int NST = (226 * 1024 - Q_BYTES - 1280) / STAGE < 8 ? (226 * 1024 - Q_BYTES - 1280) / STAGE : 8;
     static constexpr int SMEM_RING = Q_BYTES, SMEM_BAR = SMEM_RING + NST * STAGE;
     static constexpr int TOTAL = SMEM_BAR + 256 + 1024;     // + barriers and flags, + slack for 1024-byte alignment
@@ -141,11 +146,28 @@ __device__ __forceinline__ void clean_values(uint32_t slab, int k0, int prefix, 
     }
 }
 
+// Columns 32 ch .. of the nodes in hit that are no finite number, for a row that sees them: rare.
+template <int HD>
+__device__ __noinline__ void add_bad(const TreeArgs& a, const int32_t* table, int kvh, int prefix, int n, const uint4 hit, int ch, uint32_t (&o)[32]) {
+    for (int u = 0; u < n; ++u) {
+        const uint32_t w = u < 64 ? (u < 32 ? hit.x : hit.y) : (u < 96 ? hit.z : hit.w);
+        if (!(w >> (u & 31) & 1u)) continue;
+        const int at = prefix + u, page = table[at / a.P];
+        if ((unsigned)page >= (unsigned)a.num_pages) continue;
+        const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v_pages) + (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * HD + ch * 32;
+        for (int e = 0; e < 32; ++e) {
+            const float x = __bfloat162float(v[e]);
+            if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+        }
+    }
+}
+
 // grid (splits, Hkv * CTAs of row tiles, B)
-template <int HD, bool PAIR>
+template <int HD, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeArgs a) {
-    using F = Form<HD, PAIR>;
+    using F = Form<HD, MODE>;
+    constexpr bool PAIR = MODE == tree::PAIR, FOLD = MODE == tree::FOLD;
     constexpr int NST = F::NST;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
@@ -200,7 +222,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const int stages = (len + BN - 1) / BN, per = (stages + a.n_splits - 1) / a.n_splits;
     const int st0 = min(stages, split * per), ns = min(stages, (split + 1) * per) - st0;       // this CTA's stages
     const int chain = warp >= WARP_SOFTMAX ? (warp - WARP_SOFTMAX) >> 2 : warp == WARP_MMA1 ? 1 : 0;
-    const int row = tid & 127, r = r0 + (PAIR ? chain * BM : 0) + row;                         // softmax threads: their row
+    const int row = tid & 127, sub = FOLD ? row >> 6 : 0, r = r0 + (PAIR ? chain * BM : 0) + (FOLD ? row & 63 : row);                         // softmax threads: their row
     const int node = r / a.G;
     const bool live = r < a.R && node < n;
     const uint4 seen = live ? masks.seen[node] : make_uint4(0u, 0u, 0u, 0u);
@@ -208,7 +230,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     {   // query rows as the K-major operand, rows past the last one zero
         constexpr int CH = HD / 8, ROWS = PAIR ? 2 * BM : BM;
         for (int idx = tid; idx < ROWS * CH; idx += kThreads) {
-            const int qr = idx / CH, c = idx % CH, g = r0 + qr, t = g / a.G;
+            const int qr = idx / CH, c = idx % CH, g = r0 + (FOLD ? qr & 63 : qr), t = g / a.G;
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
             if (g < a.R && t < n)
                 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) +
@@ -222,11 +244,13 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
     // steps of a chain: all stages, or every second one; a tile without rows takes none
-    auto steps_of = [&](int t) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : (ns - t + 1) / 2; };
+    auto steps_of = [&](int t) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : FOLD ? ((ns + 1) / 2 - t + 1) / 2 : (ns - t + 1) / 2; };
     const int nh = steps_of(chain);
-    auto stage_of = [&](int i) { return PAIR ? i : 2 * i + chain; };
+    auto stage_of = [&](int i) { return PAIR ? i : FOLD ? 4 * i + 2 * chain : 2 * i + chain; };     // FOLD: the first of two
 
-    if (warp == WARP_TMA) {
+    if (warp < WARP_SOFTMAX) {
+      reg_dec<REGS_MISC>();
+      if (warp == WARP_TMA) {
         // ------------------------------------------------------------------ TMA
         const int ppt = BN / a.P;
         int first = st0 * ppt, issued = 0;
@@ -261,31 +285,51 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int i = max(0, issued - NST); i < issued; ++i)
                 while (!mbar_try_wait(bar(F::FULL + i % NST), (i / NST) & 1) && clock64() - t0 < ctx.limit) {}
         }
-    } else if (warp == WARP_MMA0 || warp == WARP_MMA1) {
+      } else if (warp == WARP_MMA0 || warp == WARP_MMA1) {
         // ------------------------------------------------------------------ products of chain t
         const int steps = uniform(nh), t = uniform(chain);
         if (steps > 0) {
             const uint32_t qa = desc_lo(base + (PAIR ? t * F::Q_TILE : 0), 16);
             const uint32_t k_lo = desc_lo(base + F::SMEM_RING, 16), v_lo = desc_lo(base + F::SMEM_RING + F::SLAB, KV_BOX);
             const uint32_t s_tmem = (uint32_t)uniform((int)tmem_base) + (uint32_t)t * TMEM_CHAIN, o_tmem = s_tmem + TMEM_O;
+            // S of a step: 64 columns of buffer i & 1; FOLD: both buffers, a stage each
             auto issue_qk = [&](int i) -> bool {
-                const int st = stage_of(i), s = st % NST;
-                if (!wait_bar_warp(ctx, F::FULL + s, (st / NST) & 1)) return false;
-                tc_fence_after();
-                const uint32_t kb = k_lo + (uint32_t)s * (F::STAGE >> 4), d = s_tmem + (uint32_t)(i & 1) * BN;
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_ss2(d, qa + (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4), kb + (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4),
-                            IDESC_QK, ks != 0);
-                mma_commit(bar(F::S_FULL + 2 * t + (i & 1)));
+                for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
+                    const int st = stage_of(i) + half, s = st % NST;
+                    if (FOLD && st >= ns) break;
+                    if (!wait_bar_warp(ctx, F::FULL + s, (st / NST) & 1)) return false;
+                    tc_fence_after();
+                    const uint32_t kb = k_lo + (uint32_t)s * (F::STAGE >> 4), d = s_tmem + (uint32_t)(FOLD ? half : i & 1) * BN;
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        mma_ss2(d, qa + (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4), kb + (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4),
+                                IDESC_QK, ks != 0);
+                }
+                mma_commit(bar(F::S_FULL + 2 * t + (FOLD ? 0 : i & 1)));
                 return true;
             };
             bool ok = true;
-            for (int i = 0; i < 2 && i < steps && ok; ++i) ok = issue_qk(i);
+            for (int i = 0; i < (FOLD ? 1 : 2) && i < steps && ok; ++i) ok = issue_qk(i);
             for (int i = 0; i < steps && ok; ++i) {
-                ok = wait_bar_warp(ctx, F::P_READY + 2 * t + (i & 1), (i >> 1) & 1);
+                ok = wait_bar_warp(ctx, F::P_READY + 2 * t + (FOLD ? 0 : i & 1), (FOLD ? i : i >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
+                if constexpr (FOLD) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int st = stage_of(i) + half, s = st % NST;
+                        if (st >= ns) break;
+                        const uint32_t p_tmem = s_tmem + (uint32_t)half * (BN / 2), vb = v_lo + (uint32_t)s * (F::STAGE >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < BN / 16; ++ks)
+                            mma_ts2(o_tmem, p_tmem + ks * 8, vb + (uint32_t)ks * (2048 >> 4), IdescPV<HD>::value, i > 0 || half > 0 || ks > 0);
+                        mma_commit(bar(F::EMPTY + s));
+                    }
+                    if (i + 1 == steps) mma_commit(bar(F::O_DONE + t));
+                    else ok = issue_qk(i + 1);      // S takes the place of P: in order behind its product
+                    continue;
+                }
                 const int s = stage_of(i) % NST;
                 const uint32_t p_tmem = s_tmem + (uint32_t)(i & 1) * BN, vb = v_lo + (uint32_t)s * (F::STAGE >> 4);
                 mma_ts2(o_tmem, p_tmem, vb, IdescPV<HD>::value, i > 0);
@@ -298,31 +342,39 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (i + 2 < steps) ok = issue_qk(i + 2);       // overwrites the buffer of P(i): in order behind its product
             }
         }
-    } else if (warp >= WARP_SOFTMAX) {
+      }
+    } else {
         // ------------------------------------------------------------------ softmax and epilogue
+        reg_inc<REGS_SOFTMAX>();
         const int t = chain;
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_addr + (uint32_t)t * TMEM_CHAIN, o_addr = s_addr + TMEM_O;
         float m_ref = -INFINITY, l = 0.f;
         bool ok = true;
         for (int i = 0; i < nh && ok; ++i) {
-            const int bf = i & 1, st = stage_of(i), k0 = (st0 + st) * BN;
-            const bool nodes = k0 + BN > prefix;
-            if (nodes) {        // S of the stage is there, so its values are
-                ok = wait_bar_warp(ctx, F::FULL + st % NST, (st / NST) & 1);
-                if (!ok) break;
-                clean_values<HD>(base + F::SMEM_RING + (st % NST) * F::STAGE + F::SLAB, k0, prefix, len, bad, row);
-                fence_async_smem();
+            const int bf = FOLD ? 0 : i & 1, st = stage_of(i) + sub, k0 = (st0 + st) * BN;
+            const bool none = FOLD && st >= ns, nodes = none || k0 + BN > prefix;       // none: the pair's second stage is another CTA's, or past the end
+            // stages with nodes in them: their values are there when their scores are
+#pragma unroll
+            for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
+                const int vs = stage_of(i) + half, v0 = (st0 + vs) * BN;
+                if (vs < ns && v0 + BN > prefix) {
+                    ok = ok && wait_bar_warp(ctx, F::FULL + vs % NST, (vs / NST) & 1);
+                    if (!ok) break;
+                    clean_values<HD>(base + F::SMEM_RING + (vs % NST) * F::STAGE + F::SLAB, v0, prefix, len, bad, row);
+                    fence_async_smem();
+                }
             }
-            ok = wait_bar_warp(ctx, F::S_FULL + 2 * t + bf, (i >> 1) & 1);
+            if (!ok) break;
+            ok = wait_bar_warp(ctx, F::S_FULL + 2 * t + bf, (FOLD ? i : i >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
             uint32_t sr[BN];
-            tmem_ld_x64_sync(s_addr + bf * BN, sr);
+            tmem_ld_x64_sync(s_addr + (FOLD ? sub : bf) * BN, sr);
             if (nodes) {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const uint32_t vis = window32(seen, k0 + 32 * w - prefix);
+                    const uint32_t vis = none ? 0u : window32(seen, k0 + 32 * w - prefix);
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
                         if (!(vis >> c & 1u)) sr[32 * w + c] = 0xff800000u;
@@ -340,8 +392,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             } else {
                 const bool need = m_new > m_ref + 8.f;
                 if (__any_sync(0xffffffffu, need)) {
-                    // P V of the step before must be in O: it is once S of the next step is there, issued behind it
-                    ok = i + 1 < nh ? wait_bar_warp(ctx, F::S_FULL + 2 * t + (bf ^ 1), ((i + 1) >> 1) & 1) : wait_bar_warp(ctx, F::O_PREV + t, 0);
+                    // P V of the step before must be in O: it is once S of the next step is there (FOLD: of this one), issued behind it
+                    if constexpr (!FOLD) ok = i + 1 < nh ? wait_bar_warp(ctx, F::S_FULL + 2 * t + (bf ^ 1), ((i + 1) >> 1) & 1) : wait_bar_warp(ctx, F::O_PREV + t, 0);
                     if (!ok) break;
                     tc_fence_after();
                     const float f = need ? ex2(m_ref - m_new) : 1.f;
@@ -373,7 +425,13 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     const __nv_bfloat162 pp = __floats2bfloat162_rn(pe.x, pe.y);
                     pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&pp);
                 }
-                tmem_st_x16(s_addr + bf * BN + ch * 16, pk);
+                tmem_st_x16(s_addr + (FOLD ? sub * (BN / 2) : bf * BN) + ch * 16, pk);
+            }
+            if constexpr (FOLD) {
+                uint32_t zero[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) zero[e] = 0u;
+                tmem_st_x32(s_addr + (sub ^ 1) * (BN / 2), zero);
             }
             l += ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
             tmem_st_wait();
@@ -381,8 +439,73 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             mbar_arrive(bar(F::P_READY + 2 * t + bf));
         }
         if (ok && nh > 0) ok = wait_bar_warp(ctx, F::O_DONE + t, 0);
+        if constexpr (FOLD) {
+            // The four streams of a row (chain, half): maxima and sums, then the accumulators at the common maximum, meet in the ring, whose
+            // stages are all read once both chains are done.
+            constexpr int CH = HD / 4;          // 16-byte pieces of an accumulator's row
+            float2* ml = reinterpret_cast<float2*>(smem + F::SMEM_RING);
+            const uint32_t rows_at = base + F::SMEM_RING + 2048;
+            static_assert(2048 + 4 * 64 * HD * 4 <= NST * F::STAGE, "the streams' rows fit the ring");
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            ml[t * BM + row] = make_float2(m_ref, l);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            ok = ok && !*ctx.abort;
+            float m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) m = fmaxf(m, ml[x * 64 + (row & 63)].x);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float2 v = ml[x * 64 + (row & 63)];
+                if (v.x != -INFINITY) sum = fmaf(ex2(v.x - m), v.y, sum);
+            }
+            const bool direct = a.n_splits == 1;
+            const float w = (m_ref == -INFINITY ? 0.f : ex2(m_ref - m)) * (direct ? 1.f / sum : 1.f);
+            const uint4 hit = make_uint4(bad[0] & seen.x, bad[1] & seen.y, bad[2] & seen.z, bad[3] & seen.w);
+            const bool mends = t == 0 && sub == 0 && (hit.x | hit.y | hit.z | hit.w) != 0u;
+            if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int ch = 0; ch < HD / 32; ++ch) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    if (nh > 0) tmem_ld_x32_sync(o_addr + ch * 32, o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = nh > 0 && m_ref != -INFINITY ? __float_as_uint(__uint_as_float(o[e]) * w) : 0u;
+                    if (mends) add_bad<HD>(a, table, kvh, prefix, n, hit, ch, o);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        sts128(rows_at + ((t * BM + row) * CH + ((ch * 8 + c) ^ (row & 15))) * 16, make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (ok) {
+                const size_t rows = (size_t)a.B * a.Hkv * a.R, base_row = ((size_t)b * a.Hkv + kvh) * a.R;
+                float* part = a.part + split * a.part_stride;
+                for (int idx = tid - WARP_SOFTMAX * 32; idx < a.R * CH; idx += 256) {
+                    const int rr = idx / CH, c = idx % CH, node_r = rr / a.G;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (ns > 0 && node_r < n) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint4 u = lds128(rows_at + ((x * 64 + rr) * CH + (c ^ (rr & 15))) * 16);
+                            v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
+                        }
+                    }
+                    if (direct) {
+                        __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
+                        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node_r) * a.Hq + kvh * a.G + rr % a.G) * HD;
+                        reinterpret_cast<uint2*>(out)[c] = make_uint2(*reinterpret_cast<uint32_t*>(&p0), *reinterpret_cast<uint32_t*>(&p1));
+                    } else if (ns > 0 && node_r < n) {
+                        reinterpret_cast<float4*>(part + (base_row + rr) * HD)[c] = v;
+                    }
+                }
+                if (!direct && r < a.R && t == 0 && sub == 0)
+                    *reinterpret_cast<float2*>(part + rows * HD + 2 * (base_row + r)) = live && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+            }
+        } else {
         float mine = 1.f, theirs = 0.f, m = m_ref;
-        if constexpr (!PAIR) {
+        if constexpr (MODE == SPLIT) {
             // the other chain's maximum and sum, through the ring: both accumulators are final, so its stages are read
             float2* ml = reinterpret_cast<float2*>(smem + F::SMEM_RING);
             tc_fence_before();
@@ -428,20 +551,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         }
                     }
                 }
-                if ((hit.x | hit.y | hit.z | hit.w) != 0u) {        // rare: what is no finite number, for the rows that see it
-                    for (int u = 0; u < n; ++u) {
-                        const uint32_t w = u < 64 ? (u < 32 ? hit.x : hit.y) : (u < 96 ? hit.z : hit.w);
-                        if (!(w >> (u & 31) & 1u)) continue;
-                        const int at = prefix + u, page = table[at / a.P];
-                        if ((unsigned)page >= (unsigned)a.num_pages) continue;
-                        const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v_pages) + (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * HD + ch * 32;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float x = __bfloat162float(v[e]);
-                            if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
-                        }
-                    }
-                }
+                if ((hit.x | hit.y | hit.z | hit.w) != 0u) add_bad<HD>(a, table, kvh, prefix, n, hit, ch, o);
                 if (direct && r < a.R) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = live ? o[e] : 0u;
@@ -452,6 +562,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
             if (!direct && r < a.R && (PAIR || t == 0))
                 *reinterpret_cast<float2*>(part + rows * HD + 2 * prow) = live && ns > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        }
         }
     }
     pdl_trigger();
@@ -471,17 +582,17 @@ static int make_pool_map(grl_device* dev, CUtensorMap* tm, const void* pool, con
     return get_tensor_map(dev, k, tm);
 }
 
-template <int HD, bool PAIR>
+template <int HD, Mode MODE>
 static int launch(grl_device* dev, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a) {
-    using F = Form<HD, PAIR>;
+    using F = Form<HD, MODE>;
     static bool attr_set[64] = {};
     if (!attr_set[dev->ordinal & 63]) {      // a function attribute belongs to the device that was current
-        GRL_CUDA(cudaFuncSetAttribute(tree_sm100_kernel<HD, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::TOTAL));
+        GRL_CUDA(cudaFuncSetAttribute(tree_sm100_kernel<HD, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::TOTAL));
         attr_set[dev->ordinal & 63] = true;
     }
-    const int rows = PAIR ? 2 * BM : BM;
+    const int rows = MODE == PAIR ? 2 * BM : BM;
     dim3 grid(a.n_splits, a.Hkv * ((a.R + rows - 1) / rows), a.B);
-    GRL_CUDA(launch_pdl(tree_sm100_kernel<HD, PAIR>, grid, kThreads, F::TOTAL, dev->stream, tk, tv, a));
+    GRL_CUDA(launch_pdl(tree_sm100_kernel<HD, MODE>, grid, kThreads, F::TOTAL, dev->stream, tk, tv, a));
     GRL_LAUNCHED("tree_sm100_kernel");
     return GRL_OK;
 }
@@ -494,9 +605,9 @@ int tree_sm100_launch(grl_device* dev, const TreeArgs& a) {
     int rc = make_pool_map(dev, &tk, a.k_pages, a);
     if (!rc) rc = make_pool_map(dev, &tv, a.v_pages, a);
     if (rc) return rc;
-    const bool pair = a.R > BM;
-    return a.D == 128 ? (pair ? launch<128, true>(dev, tk, tv, a) : launch<128, false>(dev, tk, tv, a))
-                      : (pair ? launch<64, true>(dev, tk, tv, a) : launch<64, false>(dev, tk, tv, a));
+    const Mode mode = a.R > BM ? PAIR : a.R > 64 ? SPLIT : FOLD;
+    if (a.D == 128) return mode == PAIR ? launch<128, PAIR>(dev, tk, tv, a) : mode == SPLIT ? launch<128, SPLIT>(dev, tk, tv, a) : launch<128, FOLD>(dev, tk, tv, a);
+    return mode == PAIR ? launch<64, PAIR>(dev, tk, tv, a) : mode == SPLIT ? launch<64, SPLIT>(dev, tk, tv, a) : launch<64, FOLD>(dev, tk, tv, a);
 }
 
 }  // namespace grl
