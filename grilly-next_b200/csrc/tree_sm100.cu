@@ -2,7 +2,7 @@
 //
 // The T * G rows (node, head of the group) of a (sequence, kv head) are the rows of the products, 128 to a tile; a CTA streams its
 // share of the cached keys and values once, 64 tokens a stage, through a shared-memory ring filled by TMA:
-//   warp 1       TMA: the stage's pages (boxes of 64 columns, 128-byte swizzle) of K and V
+//   warps 1, 3   TMA, every second stage each: the stage's pages (boxes of 64 columns, 128-byte swizzle) of K and V
 //   warps 0, 2   one elected lane each issues tcgen05.mma:  S = Q K^T (64 keys) into TMEM,  O += P V  with P from TMEM
 //   warps 4-7 / 8-11   softmax: a thread a row; S from TMEM, running maximum and sum in the exp2 domain, P back as bf16; the accumulator is
 //                scaled only where a maximum grew by more than 2^8
@@ -30,7 +30,7 @@ using namespace sm100;
 constexpr int BM = 128;             // rows of a tile (TMEM lanes)
 constexpr int BN = 64;              // tokens of a stage
 constexpr int kThreads = 384;
-constexpr int WARP_MMA0 = 0, WARP_TMA = 1, WARP_MMA1 = 2, WARP_SOFTMAX = 4;
+constexpr int WARP_MMA0 = 0, WARP_TMA0 = 1, WARP_MMA1 = 2, WARP_TMA1 = 3, WARP_SOFTMAX = 4;
 // Registers: the softmax warpgroups take what the first one gives up.  setmaxnreg.inc is served from what the CTA was launched with only.
 constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 208, REGS_MISC = 80;
 static_assert(2 * REGS_SOFTMAX + REGS_MISC <= 3 * REGS_LAUNCH && REGS_LAUNCH * kThreads <= 65536, "register budgets");
@@ -179,7 +179,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     uint32_t* bad = reinterpret_cast<uint32_t*>(smem + F::SMEM_BAR + 240);          // 128 bits
     const Ctx ctx{base + F::SMEM_BAR, abort_flag, a.status, a.wait_limit};
     auto bar = [&](int i) { return ctx.bars + (uint32_t)i * 8u; };
-    if (warp == WARP_TMA && lane == 0) {
+    if (warp == WARP_TMA0 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
         for (int s = 0; s < NST; ++s) {
@@ -250,40 +250,39 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 
     if (warp < WARP_SOFTMAX) {
       reg_dec<REGS_MISC>();
-      if (warp == WARP_TMA) {
-        // ------------------------------------------------------------------ TMA
-        const int ppt = BN / a.P;
+      if (warp == WARP_TMA0 || warp == WARP_TMA1) {
+        // ------------------------------------------------------------------ TMA: a warp the even stages, a warp the odd ones
+        // A lane a copy: one lane's chain of waits and copies took some 1700 cycles a stage, longer than HBM takes to bring it.
+        const int ppt = BN / a.P, odd = uniform(warp == WARP_TMA1);
         int first = st0 * ppt, issued = 0;
         int entry = table[min(first + lane, a.max_pages - 1)], next = table[min(first + 32 + lane, a.max_pages - 1)];
-        for (int i = 0; i < ns; ++i) {
+        for (int i = odd; i < ns; i += 2) {
             const int p = st0 + i, s = i % NST, it = i / NST;
             if (p * ppt - first >= 32) {
                 first += 32;
                 entry = next;
                 next = table[min(first + 32 + lane, a.max_pages - 1)];
             }
-            if (!__all_sync(0xffffffffu, lane != 0 || it == 0 || wait_bar(ctx, F::EMPTY + s, (it - 1) & 1))) break;
+            if (it > 0 && !wait_bar_warp(ctx, F::EMPTY + s, (it - 1) & 1)) break;
             const int np = min(ppt, (len - p * BN + a.P - 1) / a.P);       // pages of the stage that hold tokens
             if (lane == 0) mbar_expect_tx(bar(F::FULL + s), (uint32_t)(np * a.P * HD * 4));
             __syncwarp();
-            const int j = lane - (p * ppt - first);
-            if (j >= 0 && j < np) {
-                int page = entry;
+            // lane: page j, then K or V, then the box
+            constexpr int COPIES = 2 * F::BOXES;
+            const int j = lane / COPIES, v = lane / F::BOXES & 1, x = lane % F::BOXES;
+            int page = __shfl_sync(0xffffffffu, entry, (p * ppt - first + j) & 31);
+            if (j < np) {
                 if ((unsigned)page >= (unsigned)a.num_pages) { tree_fail(a.status, TREE_BAD_PAGE, b, page); page = 0; }
-                const int at = (page * a.Hkv + kvh) * a.P;
-                const uint32_t dst = base + F::SMEM_RING + s * F::STAGE + j * a.P * 128;
-#pragma unroll
-                for (int x = 0; x < F::BOXES; ++x) tma_load_2d(dst + x * KV_BOX, &tmK, x * 64, at, bar(F::FULL + s));
-#pragma unroll
-                for (int x = 0; x < F::BOXES; ++x) tma_load_2d(dst + F::SLAB + x * KV_BOX, &tmV, x * 64, at, bar(F::FULL + s));
+                tma_load_2d(base + F::SMEM_RING + s * F::STAGE + v * F::SLAB + x * KV_BOX + j * a.P * 128, v ? &tmV : &tmK, x * 64,
+                            (page * a.Hkv + kvh) * a.P, bar(F::FULL + s));
             }
             __syncwarp();
             issued = i + 1;
         }
         if (*ctx.abort && lane == 0) {      // copies in flight land before the shared memory is given back
             const long long t0 = clock64();
-            for (int i = max(0, issued - NST); i < issued; ++i)
-                while (!mbar_try_wait(bar(F::FULL + i % NST), (i / NST) & 1) && clock64() - t0 < ctx.limit) {}
+            for (int i = odd; i < issued; i += 2)
+                if (i >= issued - NST) while (!mbar_try_wait(bar(F::FULL + i % NST), (i / NST) & 1) && clock64() - t0 < ctx.limit) {}
         }
       } else if (warp == WARP_MMA0 || warp == WARP_MMA1) {
         // ------------------------------------------------------------------ products of chain t
