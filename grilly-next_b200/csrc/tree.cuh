@@ -29,6 +29,16 @@ struct TreeArgs {
     long long wait_limit;
 };
 
+// How the tensor-core kernel lays a call out (tree_sm100.cu).
+struct TreeTensorPlan {
+    int splits;         // CTAs of a (sequence, kv head, group of rows), where ctas is 0
+    int ctas;           // > 0: CTAs that take equal shares of the batch
+    int groups;         // of rows of a (sequence, kv head)
+    size_t workspace;
+};
+TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int capacity, int asked);
+int tree_sm100_launch(grl_device* dev, const TreeArgs& a, const TreeTensorPlan& plan);
+
 inline size_t tree_part_stride(size_t rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }
 
 #ifdef __CUDACC__

@@ -4,8 +4,6 @@
 
 namespace grl {
 
-int tree_sm100_launch(grl_device* dev, const TreeArgs& a);
-
 constexpr int kTreeKeys = 32;       // keys of a tile of the float32 kernel
 constexpr int kTreeRows = 8;        // rows of a CTA of it, a warp each
 
@@ -208,6 +206,7 @@ static int check_tree(const grl_tree_params* p) {
                 p->num_q_heads, kv.num_kv_heads);
     GRL_REQUIRE(p->n_tree > 0 && p->n_tree <= GRL_MAX_TREE, "n_tree must be 1 to %d, got %d", GRL_MAX_TREE, p->n_tree);
     GRL_REQUIRE(p->max_seq_len >= 0 && p->n_splits >= 0, "max_seq_len and n_splits must not be negative");
+    GRL_REQUIRE(p->n_splits <= 4096, "at most 4096 splits");
     GRL_REQUIRE(p->scale >= 0.f, "scale must be positive, or 0 for 1/sqrt(head_dim)");
     GRL_REQUIRE(p->kernel == GRL_KERNEL_AUTO || p->kernel == GRL_KERNEL_SIMT_F32 || p->kernel == GRL_KERNEL_TCGEN05, "unknown kernel");
     if (kv.head_dim != 32 && kv.head_dim != 64 && kv.head_dim != 128 && kv.head_dim != 256)
@@ -224,23 +223,28 @@ static int check_tree(const grl_tree_params* p) {
 struct TreePlan {
     bool tensor;
     int splits;
+    size_t workspace;
+    TreeTensorPlan t;
 };
 static TreePlan tree_plan(const grl_device* dev, const grl_tree_params* p) {
     const grl_kv_layout& kv = p->kv;
     const int cap = kv.max_pages * kv.page_tokens, longest = p->max_seq_len > 0 && p->max_seq_len < cap ? p->max_seq_len : cap;
-    const long long R = (long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads), heads = (long long)kv.batch * kv.num_kv_heads;
-    TreePlan t;
+    const int R = p->n_tree * (p->num_q_heads / kv.num_kv_heads);
+    TreePlan t{};
     t.tensor = p->kernel != GRL_KERNEL_SIMT_F32 && tensor_cores_apply(p);
-    // tensor cores: one CTA an SM, every split at least two stages; float32: some four CTAs an SM, every split at least four tiles
-    const long long ctas = heads * (t.tensor ? (R > 128 ? (R + 255) / 256 : 1) : (R + kTreeRows - 1) / kTreeRows);
-    long long s = (t.tensor ? 1LL : 4LL) * dev->prop.multiProcessorCount / ctas, most = longest / (4 * kTreeKeys);
+    if (t.tensor) {
+        t.t = tree_sm100_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, cap, p->n_splits);
+        t.splits = t.t.splits;
+        t.workspace = t.t.workspace;
+        return t;
+    }
+    // some four CTAs an SM, every split at least four tiles
+    const long long ctas = (long long)kv.batch * kv.num_kv_heads * ((R + kTreeRows - 1) / kTreeRows);
+    long long s = 4LL * dev->prop.multiProcessorCount / ctas, most = longest / (4 * kTreeKeys);
     if (s > most) s = most;
     t.splits = p->n_splits > 0 ? p->n_splits : (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    t.workspace = t.splits == 1 ? 0 : sizeof(float) * t.splits * tree_part_stride((size_t)kv.batch * p->n_tree * p->num_q_heads, kv.head_dim);
     return t;
-}
-
-static size_t tree_workspace(const grl_tree_params* p, int splits) {
-    return splits == 1 ? 0 : sizeof(float) * splits * tree_part_stride((size_t)p->kv.batch * p->n_tree * p->num_q_heads, p->kv.head_dim);
 }
 
 }  // namespace grl
@@ -253,7 +257,7 @@ int grl_tree_workspace_bytes(grl_device* dev, const grl_tree_params* p, size_t* 
     int rc = check_tree(p);
     if (rc) return rc;
     GRL_REQUIRE(dev && bytes, "NULL argument");
-    *bytes = tree_workspace(p, tree_plan(dev, p).splits);
+    *bytes = tree_plan(dev, p).workspace;
     return GRL_OK;
 }
 
@@ -271,7 +275,7 @@ int grl_tree_attention(grl_device* dev, const grl_tree_params* p) {
     a.wait_limit = dev->wait_limit_cycles;
     const TreePlan plan = tree_plan(dev, p);
     a.n_splits = plan.splits;
-    const size_t need = tree_workspace(p, a.n_splits);
+    const size_t need = plan.workspace;
     GRL_REQUIRE(!need || (p->workspace && p->workspace_bytes >= need), "tree attention workspace too small: %zu < %zu",
                 p->workspace ? p->workspace_bytes : 0, need);
     GRL_REQUIRE((uintptr_t)p->workspace % 16 == 0, "workspace must be 16-byte aligned");
@@ -280,8 +284,8 @@ int grl_tree_attention(grl_device* dev, const grl_tree_params* p) {
     DeviceGuard g(dev->ordinal);
     dev->status_dirty = true;
     const bool c32 = kv.cache_dtype == GRL_F32, io32 = p->io_dtype == GRL_F32;
-    rc = plan.tensor ? tree_sm100_launch(dev, a)
-       : io32 ? (c32 ? launch_rows_d<float, float>(dev, a) : launch_rows_d<float, __nv_bfloat16>(dev, a))
+    if (plan.tensor) return tree_sm100_launch(dev, a, plan.t);
+    rc = io32 ? (c32 ? launch_rows_d<float, float>(dev, a) : launch_rows_d<float, __nv_bfloat16>(dev, a))
        : (c32 ? launch_rows_d<__nv_bfloat16, float>(dev, a) : launch_rows_d<__nv_bfloat16, __nv_bfloat16>(dev, a));
     if (rc || a.n_splits == 1) return rc;
     const size_t rows = (size_t)a.B * a.Hkv * a.R;

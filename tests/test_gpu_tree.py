@@ -186,6 +186,11 @@ TREES = {
     "long_few_rows": tree_case(2, 8, 2, 128, 64, [9000, 8000], kind="chain"),
     "batch": tree_case(16, 8, 4, 128, 64, [300 + 17 * i for i in range(40)]),
     "batch_few_rows": tree_case(3, 8, 4, 64, 64, [300 + 17 * i for i in range(40)]),
+    "many_sequences": tree_case(3, 4, 2, 64, 64, [1 + 5 * i % 300 for i in range(3, 140)], [(i % 4) if 1 + 5 * i % 300 >= (i % 4) else 0 for i in range(3, 140)]),
+    "shares_whole_and_cut": tree_case(9, 8, 4, 128, 64, [64 * (1 + 7 * i % 13) + i for i in range(9, 60)]),
+    "shares_of_wide": tree_case(70, 8, 2, 128, 32, [70 + 64 * (5 * i % 11) for i in range(30)], [70 - i for i in range(30)]),
+    "shares_of_three_groups": tree_case(128, 16, 2, 64, 64, [900, 128, 300]),
+    "shares_of_one_tile": tree_case(30, 8, 2, 128, 64, [30 + 100 * (5 * i % 11) for i in range(30)]),
     "hint_too_short": tree_case(8, 8, 2, 128, 64, [700, 64], kw_max_seq_len=100),
     "f32": tree_case(11, 6, 2, 64, 24, [300, 97, 11], cache="f32"),
     "f32_dim_32": tree_case(11, 6, 2, 32, 7, [100, 50], cache="f32"),
@@ -249,6 +254,33 @@ def test_what_a_row_does_not_see_may_be_anything(dev, T, kind, cache_type):
             if which == 1:
                 assert np.all(np.isnan(got[b, sees]) if np.isnan(value) else got[b, sees] == value)
         cache.free()
+
+
+@pytest.mark.parametrize("T", [4, 30, 64])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(T):
+    """A budget of one cycle for the waits of long streams (a wait that the hardware suspends may still succeed, so the call is made until one runs
+    out): the kernel returns, the failure is reported, and the call after it gives what the call before gave."""
+    from grilly_next import cabi
+    dev = cabi.Device(0)
+    cache = Cache(dev, [20000, 9000 + T], 2, 128, 64, "bf16", seed=6)
+    r = np.random.default_rng(6)
+    q = round_bf16(r.standard_normal((2, T, 8, 128)).astype(np.float32))
+    parents = [draw_parents(r, T, "tree") for _ in range(2)]
+    want = attend(dev, cache, q, parents, None, io="bf16")
+    cabi.check(dev.L.grl_device_set_wait_limits(dev.h, 1, 0))
+    for _ in range(100):
+        try:
+            assert np.array_equal(attend(dev, cache, q, parents, None, io="bf16"), want)
+        except cabi.GrlError as e:
+            assert e.code == cabi.ERR_TIMEOUT and "tree attention" in str(e)
+            break
+    else:
+        raise AssertionError("no wait ran out")
+    cabi.check(dev.L.grl_device_set_wait_limits(dev.h, 0, 0))
+    for _ in range(3):
+        assert np.array_equal(attend(dev, cache, q, parents, None, io="bf16"), want)
+    cache.free()
+    dev.close()
 
 
 def test_refusals_of_the_tensor_core_kernel(dev):
