@@ -192,7 +192,8 @@ static bool tensor_cores_apply(const grl_tree_params* p) {
     const grl_kv_layout& kv = p->kv;
     return kv.cache_dtype == GRL_BF16 && p->io_dtype == GRL_BF16 && (kv.head_dim == 128 || kv.head_dim == 64) &&
            (kv.page_tokens == 64 || kv.page_tokens == 32 || kv.page_tokens == 16) &&
-           (long long)pool_pages(kv) * kv.num_kv_heads * kv.page_tokens < (1LL << 31);
+           (long long)pool_pages(kv) * kv.num_kv_heads * kv.page_tokens < (1LL << 31) &&
+           (long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads) < (1LL << 15);
 }
 
 static int check_tree(const grl_tree_params* p) {

@@ -2,7 +2,7 @@
 //
 // The T * G rows (node, head of the group) of a (sequence, kv head) are the rows of the products, 128 to a tile; a CTA streams its
 // share of the cached keys and values once, 64 tokens a stage, through a shared-memory ring filled by TMA:
-//   warps 1, 3   TMA, every second stage each: the stage's pages (boxes of 64 columns, 128-byte swizzle) of K and V
+//   warps 1, 3   TMA, the stages of one chain each (PAIR: every second one): the stage's pages (boxes of 64 columns, 128-byte swizzle) of K and V
 //   warps 0, 2   one elected lane each issues tcgen05.mma:  S = Q K^T (64 keys) into TMEM,  O += P V  with P from TMEM
 //   warps 4-7 / 8-11   softmax: a thread a row; S from TMEM, running maximum and sum in the exp2 domain, P back as bf16; the accumulator is
 //                scaled only where a maximum grew by more than 2^8
@@ -13,7 +13,7 @@
 //           where a half's rows meet the other's keys, so that one product sums both; four streams are joined in the epilogue
 // The work is a list of pieces, runs of stages of one (sequence, kv head, group of rows): one for every CTA of the grid where the caller names the
 // number of splits or there are many sequences, else an equal share of all stages of the batch for every CTA, which may end one head, hold some
-// whole and begin another.  Whole heads are written by their CTA, the parts of others meet in tree_join_kernel.  The loads of the next
+// whole and begin another.  Whole heads are written by their CTA, the parts of others meet in tree_join_kernel (a CTA's own two merges would have to wait for its neighbours).  The loads of the next
 // piece run under the epilogue of the one before.
 // The predicate is applied to the last stages only, those with nodes in them: a row has one bit for each of 128 nodes.  There, rows
 // of V past the sequence's end, which may hold anything, are cleared in shared memory ahead of the product, and so are elements
@@ -65,7 +65,10 @@ template <int HD, Mode MODE> struct Form {
     static constexpr int Q_BYTES = MODE == PAIR ? 2 * Q_TILE : Q_TILE;
     static constexpr int OUT_BYTES = 256 * 32 * 4;          // 32 columns of 256 accumulator rows, where the queries were
     static constexpr int RING = Q_BYTES > OUT_BYTES ? Q_BYTES : OUT_BYTES;
-    static constexpr int NST = (225 * 1024 - RING) / STAGE < 8 ? (225 * 1024 - RING) / STAGE : 8;
+    // PAIR: one ring that both chains read.  Else a ring for each chain: a phase of a slot's barrier is told by its parity, so whoever waits on it
+    // has to have seen the phase before, which one of two chains that share out the stages of a ring may not have when copies come in late.
+    static constexpr int FIT = (225 * 1024 - RING) / STAGE < 8 ? (225 * 1024 - RING) / STAGE : 8;
+    static constexpr int NST = MODE == PAIR ? FIT : FIT / 2 * 2, SLOTS = MODE == PAIR ? NST : NST / 2;
     static constexpr int BLOCK = RING + NST * STAGE;
     static constexpr int TOTAL = BLOCK + (int)sizeof(Block) + 1024;     // + slack for 1024-byte alignment
     static_assert(TOTAL <= 227 * 1024, "shared memory");
@@ -76,6 +79,7 @@ template <int HD, Mode MODE> struct Form {
     static_assert(NUM <= 32, "barrier block");
 };
 struct Share {
+    uint32_t per_group;     // 2^32 / G rounded up: row / G is its product's upper half (rows and G below 2^15; 0: G is 1)
     int ctas;               // > 0: equal shares of all stages; 0: one piece a CTA, grid (splits, Hkv * groups, B)
     int groups;             // of rows of a (sequence, kv head)
 };
@@ -169,6 +173,7 @@ __device__ __forceinline__ void clean_values(uint32_t slab, int k0, int prefix, 
 }
 
 
+__device__ __forceinline__ int node_of(const Share& sh, int r) { return sh.per_group ? (int)__umulhi((uint32_t)r, sh.per_group) : r; }
 struct Piece {
     int b, hg, st0, ns;     // sequence, kv head * groups + group, first stage and stages
     bool whole;
@@ -223,8 +228,7 @@ __device__ __forceinline__ int sequence_at(const Block& k, int hgs, int stage) {
     }
     return lo;
 }
-// Walks the pieces of a CTA; every role does so for itself.  32-bit arithmetic: a division of 64 bits is a call, and a called function may use more
-// registers than the warps that have given theirs up still hold.
+// Walks the pieces of a CTA; every role does so for itself.
 struct Pieces {
     int at, end;
     __device__ __forceinline__ void start(const Block& k, const TreeArgs& a, const Share& sh) {
@@ -324,25 +328,29 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         *n = only_n;
         return true;
     };
-    // steps of chain t over ns stages: all, or every second one, or every second pair; a tile without rows takes none
+    // stages of chain t of ns, and its k-th one: all, or every second one, or every second pair
+    auto count_of = [&](int t, int ns) { return PAIR ? ns : FOLD ? ns / 4 * 2 + max(0, min(2, ns % 4 - 2 * t)) : (ns - t + 1) / 2; };
+    auto stage_of = [&](int t, int k) { return PAIR ? k : FOLD ? 4 * (k >> 1) + 2 * t + (k & 1) : 2 * k + t; };
+    auto slot_of = [&](int t, int x) { return (PAIR ? 0 : t * F::SLOTS) + x % F::SLOTS; };        // of the x-th stage of a chain since the start
+    // steps of chain t over ns stages: one for each, or for two; a tile without rows takes none
     auto steps_of = [&](int t, int ns, int r0) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : FOLD ? ((ns + 1) / 2 - t + 1) / 2 : (ns - t + 1) / 2; };
 
     if (warp < WARP_SOFTMAX) {
       reg_dec<REGS_MISC>();
       if (warp == WARP_TMA0 || warp == WARP_TMA1) {
-        // ------------------------------------------------------------------ TMA: a warp the even stages, a warp the odd ones
+        // ------------------------------------------------------------------ TMA: a warp the stages of a chain (PAIR: the even or the odd ones)
         // A lane a copy: one lane's chain of waits and copies took some 1700 cycles a stage, longer than HBM takes to bring it.
-        const int ppt = BN / a.P, odd = uniform(warp == WARP_TMA1);
+        const int ppt = BN / a.P, t = uniform(warp == WARP_TMA1);
         int done = 0, last = -1, len, n;        // stages of earlier pieces; the last one this warp has asked for
         Piece pc;
         bool ok = true;
         while (ok && take(&pc, &len, &n)) {
             const int32_t* table = a.block_table + (size_t)pc.b * a.max_pages;
-            const int kvh = pc.hg / sh.groups;
+            const int kvh = pc.hg / sh.groups, count = count_of(t, pc.ns);
             int first = pc.st0 * ppt;
             int entry = table[min(first + lane, a.max_pages - 1)], next = table[min(first + 32 + lane, a.max_pages - 1)];
-            for (int i = (done ^ odd) & 1; i < pc.ns; i += 2) {
-                const int p = pc.st0 + i, s = (done + i) % NST, it = (done + i) / NST;
+            for (int k = PAIR ? (done ^ t) & 1 : 0; k < count; k += PAIR ? 2 : 1) {
+                const int p = pc.st0 + stage_of(t, k), s = slot_of(t, done + k), it = (done + k) / F::SLOTS;
                 if (p * ppt - first >= 32) {
                     first += 32;
                     entry = next;
@@ -362,14 +370,14 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                                 (page * a.Hkv + kvh) * a.P, bar(F::FULL + s));
                 }
                 __syncwarp();
-                last = done + i;
+                last = done + k;
             }
-            if (ok) done += pc.ns;
+            if (ok) done += count;
         }
         if (*ctx.abort) {       // copies in flight land before the shared memory is given back
             const long long t0 = clock64();
-            for (int x = last; x >= 0 && x > last - NST; x -= 2)
-                while (!mbar_try_wait(bar(F::FULL + x % NST), (x / NST) & 1) && clock64() - t0 < kDrainCycles) {}
+            for (int x = last; x >= 0 && x > last - F::SLOTS; x -= PAIR ? 2 : 1)
+                while (!mbar_try_wait(bar(F::FULL + slot_of(t, x)), (x / F::SLOTS) & 1) && clock64() - t0 < kDrainCycles) {}
         }
       } else {
         // ------------------------------------------------------------------ products of chain t
@@ -377,21 +385,21 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const uint32_t qa = desc_lo(base + (PAIR ? t * F::Q_TILE : 0), 16);
         const uint32_t k_lo = desc_lo(base + F::RING, 16), v_lo = desc_lo(base + F::RING + F::SLAB, KV_BOX);
         const uint32_t s_tmem = (uint32_t)uniform((int)tmem_base) + (uint32_t)t * TMEM_CHAIN, o_tmem = s_tmem + TMEM_O;
-        int done = 0, steps_done = 0, count = 0, len, n;        // stages, this chain's steps and pieces so far
+        int done = 0, steps_done = 0, count = 0, len, n;        // this chain's stages and steps, and pieces so far
         Piece pc;
         bool ok = true;
         while (ok && take(&pc, &len, &n)) {
             const int ns = uniform(pc.ns), r0 = pc.hg % sh.groups * (PAIR ? 2 * BM : BM);
             const int steps = uniform(steps_of(t, ns, r0)), others = PAIR ? uniform(steps_of(t ^ 1, ns, r0)) : 1;
-            auto stage_of = [&](int i) { return PAIR ? i : FOLD ? 4 * i + 2 * t : 2 * i + t; };
+            const int mine = uniform(count_of(t, ns));
             // S of a step: 64 columns of the buffers in turn; FOLD: both buffers, a stage each
             auto issue_qk = [&](int i) -> bool {
                 const int ci = steps_done + i;
 #pragma unroll
                 for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int st = stage_of(i) + half, s = (done + st) % NST;
-                    if (FOLD && st >= ns) break;
-                    if (!wait_bar_warp(ctx, F::FULL + s, ((done + st) / NST) & 1)) return false;
+                    const int k = FOLD ? 2 * i + half : i, s = slot_of(t, done + k);
+                    if (FOLD && k >= mine) break;
+                    if (!wait_bar_warp(ctx, F::FULL + s, ((done + k) / F::SLOTS) & 1)) return false;
                     tc_fence_after();
                     const uint32_t kb = k_lo + (uint32_t)s * (F::STAGE >> 4), d = s_tmem + (uint32_t)(FOLD ? half : ci & 1) * BN;
 #pragma unroll
@@ -412,8 +420,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 tc_fence_after();
 #pragma unroll
                 for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int st = stage_of(i) + half, s = (done + st) % NST;
-                    if (FOLD && st >= ns) break;
+                    const int k = FOLD ? 2 * i + half : i, s = slot_of(t, done + k);
+                    if (FOLD && k >= mine) break;
                     const uint32_t p_tmem = s_tmem + (FOLD ? (uint32_t)half * (BN / 2) : (uint32_t)(ci & 1) * BN), vb = v_lo + (uint32_t)s * (F::STAGE >> 4);
 #pragma unroll
                     for (int ks = 0; ks < BN / 16; ++ks)
@@ -428,7 +436,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
             // for a chain without steps too, so that nobody falls two pieces behind
             if (ok) mma_commit(bar(F::O_DONE + t));
-            done += ns;
+            done += mine;
             steps_done += steps;
             ++count;
         }
@@ -446,7 +454,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int row = tid & 127, sub = FOLD ? row >> 6 : 0;
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_addr + (uint32_t)t * TMEM_CHAIN, o_addr = s_addr + TMEM_O;
-        constexpr int CH = HD / 8, Q_ROWS = PAIR ? 2 * BM : BM, PER = Q_ROWS * CH / 256;    // 16-byte pieces of the query rows, of a thread
+        constexpr int CH = HD / 8, PER = F::ROWS * CH / 256;     // 16-byte pieces of a query row, of a thread
         int done = 0, steps_done = 0, count = 0, prevs = 0, len = 0, n = 0;
         Piece pc{};
         auto meet = [] {        // both warpgroups; the barrier is for converged warps
@@ -458,22 +466,24 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                       prefix = len - n;
             const bool whole = pc.whole;
             const int part_at = pc.part;
-            const int r = r0 + (PAIR ? t * BM : 0) + (FOLD ? row & 63 : row), node = r / a.G;
+            const int r = r0 + (PAIR ? t * BM : 0) + (FOLD ? row & 63 : row), node = node_of(sh, r);
             {   // query rows as the K-major operand, rows past the last one zero; parents
                 const int up = a.parents && st_id < now_n ? a.parents[(size_t)b * a.T + st_id] : -1;
+                const int c = st_id % CH, first = st_id / CH;
+                const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD) + c;
                 uint4 v[PER];
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const int idx = st_id + e * 256, qr = idx / CH, c = idx % CH, g = r0 + (FOLD ? qr & 63 : qr);
+                    const int g = r0 + first + e * (256 / CH), at = node_of(sh, g);
                     v[e] = make_uint4(0u, 0u, 0u, 0u);
-                    if (g < a.R)
-                        v[e] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) +
-                                                                    (((size_t)b * a.T + g / a.G) * a.Hq + kvh * a.G + g % a.G) * HD) + c);
+                    if (g < a.R) v[e] = __ldg(q + (at * a.Hq + g - at * a.G) * CH);
                 }
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const int idx = st_id + e * 256, qr = idx / CH, c = idx % CH;
-                    sts128(base + (qr >> 7) * F::Q_TILE + (c >> 3) * Q_BOX + (qr & 127) * 128 + (((c & 7) ^ (qr & 7)) << 4), v[e]);
+                    const int qr = first + e * (256 / CH);
+                    const uint32_t to = base + (qr >> 7) * F::Q_TILE + (c >> 3) * Q_BOX + (qr & 127) * 128 + (((c & 7) ^ (qr & 7)) << 4);
+                    sts128(to, v[e]);
+                    if (FOLD) sts128(to + 64 * 128, v[e]);
                 }
                 if (a.parents && st_id < now_n) {
                     if (up < -1 || up >= st_id) blk.bad_tree = 1;
@@ -499,21 +509,20 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     }
             }
             __syncwarp();
-            const int nh = steps_of(t, ns, r0);
-            auto stage_of = [&](int i) { return PAIR ? i : FOLD ? 4 * i + 2 * t : 2 * i + t; };
+            const int nh = steps_of(t, ns, r0), mine = count_of(t, ns);
             float m_ref = -INFINITY, l = 0.f;
             bool ok = true;
             for (int i = 0; i < nh && ok; ++i) {
-                const int ci = steps_done + i, bf = FOLD ? 0 : ci & 1, st = stage_of(i) + sub, k0 = (st0 + st) * BN;
-                const bool none = FOLD && st >= ns, nodes = none || k0 + BN > prefix;       // none: the pair's second stage is another CTA's, or past the end
+                const int ci = steps_done + i, bf = FOLD ? 0 : ci & 1, own = FOLD ? 2 * i + sub : i, k0 = (st0 + stage_of(t, own)) * BN;
+                const bool none = FOLD && own >= mine, nodes = none || k0 + BN > prefix;       // none: the pair's second stage is another CTA's, or past the end
                 // stages with nodes in them: their values are there when their scores are
 #pragma unroll
                 for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int vs = stage_of(i) + half, v0 = (st0 + vs) * BN;
-                    if (vs < ns && v0 + BN > prefix) {
-                        ok = ok && wait_bar_warp(ctx, F::FULL + (done + vs) % NST, ((done + vs) / NST) & 1);
+                    const int k = FOLD ? 2 * i + half : i, v0 = (st0 + stage_of(t, k)) * BN, s = slot_of(t, done + k);
+                    if (k < mine && v0 + BN > prefix) {
+                        ok = ok && wait_bar_warp(ctx, F::FULL + s, ((done + k) / F::SLOTS) & 1);
                         if (!ok) break;
-                        clean_values<HD>(base + F::RING + (done + vs) % NST * F::STAGE + F::SLAB, v0, prefix, now_len, blk.bad, row);
+                        clean_values<HD>(base + F::RING + s * F::STAGE + F::SLAB, v0, prefix, now_len, blk.bad, row);
                         fence_async_smem();
                     }
                 }
@@ -593,7 +602,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 mbar_arrive(bar(F::P_READY + 2 * t + bf));
             }
             if (ok) ok = wait_bar_warp(ctx, F::O_DONE + t, count & 1);
-            done += ns;
+            done += mine;
             steps_done += nh;
             ++count;
             prevs += nh > 1;
@@ -624,36 +633,48 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             float* part = a.part + (size_t)part_at * F::PART;
             const int rows = min(F::ROWS, a.R - r0), live_nodes = bad_tree ? 0 : now_n;
             const bool full = ok && nh > 0 && m_ref != -INFINITY;
+            // a thread takes one 16-byte piece of every 32nd row
+            constexpr int K = F::ROWS / 32;
+            const int c = st_id & 7, rr0 = st_id >> 3;
+            int at[K];                  // elements from the batch's, or the part's, first; below 0: nothing to write
+            uint32_t alive = 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int rg = r0 + rr0 + 32 * k, rn = node_of(sh, rg);
+                const bool l_ = rn < live_nodes;
+                alive |= (uint32_t)l_ << k;
+                at[k] = rr0 + 32 * k >= rows || !ok || !(whole || l_) ? -1 : (whole ? (rn * a.Hq + rg - rn * a.G) * HD : (rr0 + 32 * k) * HD) + 4 * c;
+            }
+            __nv_bfloat16* out_at = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD;
 #pragma unroll 1
             for (int ch = 0; ch < HD / 32; ++ch) {
                 uint32_t o[32];
                 if (ok && nh > 0) tmem_ld_x32_sync(o_addr + ch * 32, o);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const uint4 v = make_uint4(__float_as_uint(__uint_as_float(o[4 * c]) * w), __float_as_uint(__uint_as_float(o[4 * c + 1]) * w),
-                                               __float_as_uint(__uint_as_float(o[4 * c + 2]) * w), __float_as_uint(__uint_as_float(o[4 * c + 3]) * w));
-                    sts128(base + st_id * 128 + ((c ^ (st_id & 7)) << 4), full ? v : make_uint4(0u, 0u, 0u, 0u));
+                for (int e = 0; e < 8; ++e) {
+                    const uint4 v = make_uint4(__float_as_uint(__uint_as_float(o[4 * e]) * w), __float_as_uint(__uint_as_float(o[4 * e + 1]) * w),
+                                               __float_as_uint(__uint_as_float(o[4 * e + 2]) * w), __float_as_uint(__uint_as_float(o[4 * e + 3]) * w));
+                    sts128(base + st_id * 128 + ((e ^ (st_id & 7)) << 4), full ? v : make_uint4(0u, 0u, 0u, 0u));
                 }
                 meet();
-                if (ok)
-                    for (int idx = st_id; idx < rows * 8; idx += 256) {
-                        const int rr = idx >> 3, c = idx & 7, rg = r0 + rr, rnode = rg / a.G;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (rnode < live_nodes) {
 #pragma unroll
-                            for (int x = 0; x < F::STREAMS; ++x) {
-                                const uint4 u = lds128(base + (x * F::ROWS + rr) * 128 + ((c ^ (rr & 7)) << 4));
-                                v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
-                            }
-                        }
-                        if (whole) {
-                            const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
-                            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + rnode) * a.Hq + kvh * a.G + rg % a.G) * HD;
-                            reinterpret_cast<uint2*>(out + ch * 32)[c] = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
-                        } else if (rnode < live_nodes) {
-                            reinterpret_cast<float4*>(part + (size_t)rr * HD + ch * 32)[c] = v;
+                for (int k = 0; k < K; ++k) {
+                    if (at[k] < 0) continue;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (alive >> k & 1u) {
+#pragma unroll
+                        for (int x = 0; x < F::STREAMS; ++x) {
+                            const uint4 u = lds128(base + (x * F::ROWS + rr0 + 32 * k) * 128 + ((c ^ (rr0 & 7)) << 4));
+                            v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
                         }
                     }
+                    if (whole) {
+                        const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
+                        *reinterpret_cast<uint2*>(out_at + at[k] + ch * 32) = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
+                    } else {
+                        *reinterpret_cast<float4*>(part + at[k] + ch * 32) = v;
+                    }
+                }
                 meet();
             }
             const bool owner = st_id < F::ROWS && st_id < rows;         // of row r in the results
@@ -694,88 +715,96 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (warp == WARP_MMA0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
 }
 
-// Joins the parts of heads that several CTAs have worked on, a warp a row: their sums at their common maximum.  Rows of sequences
-// without nodes are written here too where the batch is cut into shares.  grid (B * Hkv * groups, rows / 32)
+// Joins the parts of heads that several CTAs have worked on, a warp a row at a time: the parts' sums at their common maximum, eight parts on
+// their way at once.  With equal shares a CTA looks at one cut of the batch (blockIdx.x < ctas - 1), and takes the head there if it is the head's
+// first cut, or at one sequence (blockIdx.x - ctas + 1), whose rows it clears if it has no nodes.  It knows all that before the kernel ahead of it ends,
+// whose lengths are those of the call.
+constexpr int kJoinRows = 16;       // of a CTA
 template <int HD>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Share sh, int piece_rows) {
     __shared__ Block blk;
-    const int hgs = a.Hkv * sh.groups, b = blockIdx.x / hgs, hg = blockIdx.x % hgs, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait();
+    const int hgs = a.Hkv * sh.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int b = blockIdx.x / hgs, hg = blockIdx.x % hgs, c0 = 0, parts = a.n_splits;
+    bool dense = true, clear = false;
+    if (sh.ctas && warp == 0) scan_batch(a, blk, false);
+    __syncthreads();
+    pdl_wait();                 // every CTA, or the kernel behind this one could start before the one ahead of it has ended
     pdl_trigger();
-    int c0 = 0, parts = a.n_splits;
     if (sh.ctas) {
-        if (warp == 0) scan_batch(a, blk, false);
-        __syncthreads();
-        const int stages = blk.before[b + 1] - blk.before[b];
-        const long long all = (long long)blk.before[kMaxShared] * hgs, first = (long long)blk.before[b] * hgs + hg * stages;
-        parts = 0;
-        if (stages > 0) {
+        const int all = blk.before[kMaxShared] * hgs;
+        if ((int)blockIdx.x < sh.ctas - 1) {
+            const int cut = share_begin(blk, a, sh, blockIdx.x + 1), prev = share_begin(blk, a, sh, blockIdx.x);
+            if (cut >= all) return;
+            b = sequence_at(blk, hgs, cut);
+            const int stages = blk.before[b + 1] - blk.before[b], rem = cut - blk.before[b] * hgs;
+            hg = rem / stages;
+            const int first = cut - (rem - hg * stages);
+            if (first == cut || prev > first || prev == cut) return;     // between heads, or not the head's first cut
             // the last CTA whose share begins at or before a stage has it
-            c0 = (int)(((first + 1) * sh.ctas - 1) / all);
-            parts = (int)(((first + stages) * sh.ctas - 1) / all) - c0 + 1;
-            if (parts == 1) return;         // written by its CTA
+            c0 = blockIdx.x;
+            parts = (int)(((long long)(first + stages) * sh.ctas - 1) / all) - c0 + 1;
+            dense = all >= sh.ctas;
+        } else {
+            b = blockIdx.x - (sh.ctas - 1);
+            if (blk.nodes[b]) return;
+            clear = true;
+            parts = 0;
         }
     }
-    const size_t stride = (size_t)piece_rows * (HD + 2);
     constexpr int V = HD / 32;              // columns of a lane
-    // part i: where, and whether there is one (a share may be empty where there are fewer stages than CTAs)
-    auto part_of = [&](int i) -> const float* {
-        if (!sh.ctas) return a.part + ((size_t)blockIdx.x * a.n_splits + i) * stride;
-        if (share_begin(blk, a, sh, c0 + i) == share_begin(blk, a, sh, c0 + i + 1)) return nullptr;
-        return a.part + ((size_t)(c0 + i) * 2 + (i == 0)) * stride;
-    };
-    for (int e = 0; e < 4; ++e) {
-        const int rr = blockIdx.y * 32 + warp * 4 + e, r = hg % sh.groups * piece_rows + rr;
-        if (rr >= piece_rows || r >= a.R) return;
-        float m = -INFINITY;
-        for (int i = lane; i < parts; i += 32) {
-            const float* p = part_of(i);
-            const float2 v = p ? __ldcg(reinterpret_cast<const float2*>(p + (size_t)piece_rows * HD) + rr) : make_float2(-INFINITY, 0.f);
-            if (v.y != 0.f) m = fmaxf(m, v.x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float l = 0.f, acc[V];
+    if (clear) {
+        const size_t n = (size_t)a.T * a.Hq * HD / 8;
+        uint4* out = reinterpret_cast<uint4*>(a.out) + b * n;
+        for (size_t i = (size_t)blockIdx.y * 256 + threadIdx.x; i < n; i += (size_t)gridDim.y * 256) out[i] = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
+    const size_t stride = (size_t)piece_rows * (HD + 2);
+    const float* first_part = a.part + (sh.ctas ? (size_t)c0 * 2 : (size_t)blockIdx.x * a.n_splits) * stride;
+    const int kvh = hg / sh.groups, r0 = hg % sh.groups * piece_rows, rows = min(piece_rows, a.R - r0);
+    for (int rr = blockIdx.y * kJoinRows + warp; rr < min(rows, (int)(blockIdx.y + 1) * kJoinRows); rr += 8) {
+        float m = -INFINITY, l = 0.f, acc[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) acc[c] = 0.f;
-        for (int i0 = 0; i0 < parts; i0 += 32) {
-            const float* mine = i0 + lane < parts ? part_of(i0 + lane) : nullptr;
-            const float2 v = mine ? __ldcg(reinterpret_cast<const float2*>(mine + (size_t)piece_rows * HD) + rr) : make_float2(-INFINITY, 0.f);
-            const float w = v.y != 0.f ? exp2f(v.x - m) : 0.f;
-            l = fmaf(w, v.y, l);
-            uint32_t have = __ballot_sync(0xffffffffu, v.y != 0.f);         // a part that has seen nothing has no O
-            while (have) {
-                float x[4][V], ws[4];
+        for (int i0 = 0; i0 < parts; i0 += 8) {
+            float2 ml[8];
+            float o[8][V];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = have ? __ffs(have) - 1 : 0;
-                    ws[j] = __shfl_sync(0xffffffffu, w, i);
-                    const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i));
-                    if (!have) ws[j] = 0.f;
-#pragma unroll
-                    for (int c = 0; c < V; ++c) x[j][c] = 0.f;
-                    if (have) {
-                        if constexpr (V == 4) {
-                            const float4 f = __ldcg(reinterpret_cast<const float4*>(p + (size_t)rr * HD) + lane);
-                            x[j][0] = f.x; x[j][1] = f.y; x[j][2] = f.z; x[j][3] = f.w;
-                        } else {
-                            const float2 f = __ldcg(reinterpret_cast<const float2*>(p + (size_t)rr * HD) + lane);
-                            x[j][0] = f.x; x[j][1] = f.y;
-                        }
-                    }
-                    have &= have - 1;
+            for (int j = 0; j < 8; ++j) {
+                const int i = i0 + j;
+                ml[j] = make_float2(-INFINITY, 0.f);
+                if (i >= parts || (!dense && share_begin(blk, a, sh, c0 + i) == share_begin(blk, a, sh, c0 + i + 1))) continue;
+                // shares: the part that begins the head is its CTA's second place, the others are their CTAs' first
+                const float* p = first_part + (sh.ctas ? (size_t)2 * i + (i == 0) : (size_t)i) * stride;
+                ml[j] = __ldcg(reinterpret_cast<const float2*>(p + (size_t)piece_rows * HD) + rr);
+                if constexpr (V == 4) {
+                    const float4 f = __ldcg(reinterpret_cast<const float4*>(p + (size_t)rr * HD) + lane);
+                    o[j][0] = f.x; o[j][1] = f.y; o[j][2] = f.z; o[j][3] = f.w;
+                } else {
+                    const float2 f = __ldcg(reinterpret_cast<const float2*>(p + (size_t)rr * HD) + lane);
+                    o[j][0] = f.x; o[j][1] = f.y;
                 }
+            }
+            float m_new = m;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 8; ++j)
+                if (ml[j].y != 0.f) m_new = fmaxf(m_new, ml[j].x);
+            const float f = m == -INFINITY ? 0.f : exp2f(m - m_new);
+            l *= f;
 #pragma unroll
-                    for (int c = 0; c < V; ++c) acc[c] = fmaf(ws[j], x[j][c], acc[c]);
+            for (int c = 0; c < V; ++c) acc[c] *= f;
+            m = m_new;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (ml[j].y == 0.f) continue;       // a part that has seen nothing has no O
+                const float w = exp2f(ml[j].x - m);
+                l = fmaf(w, ml[j].y, l);
+#pragma unroll
+                for (int c = 0; c < V; ++c) acc[c] = fmaf(w, o[j][c], acc[c]);
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int kvh = hg / sh.groups;
-        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + r / a.G) * a.Hq + kvh * a.G + r % a.G) * HD;
+        const int r = r0 + rr, node = node_of(sh, r);
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r - node * a.G) * HD;
         if constexpr (V == 4) {
             const __nv_bfloat162 p0 = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), p1 = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
             reinterpret_cast<uint2*>(out)[lane] = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
@@ -807,7 +836,7 @@ static int launch(grl_device* dev, const CUtensorMap& tk, const CUtensorMap& tv,
     GRL_CUDA(launch_pdl(tree_sm100_kernel<HD, MODE>, grid, kThreads, F::TOTAL, dev->stream, tk, tv, a, sh));
     GRL_LAUNCHED("tree_sm100_kernel");
     if (!sh.ctas && a.n_splits == 1) return GRL_OK;
-    GRL_CUDA(launch_pdl(tree_join_kernel<HD>, dim3(a.B * a.Hkv * sh.groups, (F::ROWS + 31) / 32), 256, 0, dev->stream, a, sh, F::ROWS));
+    GRL_CUDA(launch_pdl(tree_join_kernel<HD>, dim3(sh.ctas ? sh.ctas - 1 + a.B : a.B * a.Hkv * sh.groups, (min(F::ROWS, a.R) + kJoinRows - 1) / kJoinRows), 256, 0, dev->stream, a, sh, F::ROWS));
     GRL_LAUNCHED("tree_join_kernel");
     return GRL_OK;
 }
@@ -846,7 +875,7 @@ int tree_sm100_launch(grl_device* dev, const TreeArgs& a, const TreeTensorPlan& 
     int rc = make_pool_map(dev, &tk, a.k_pages, a);
     if (!rc) rc = make_pool_map(dev, &tv, a.v_pages, a);
     if (rc) return rc;
-    const Share sh{plan.ctas, plan.groups};
+    const Share sh{a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G), plan.ctas, plan.groups};
     const Mode mode = mode_of(a.R);
     if (a.D == 128)
         return mode == PAIR ? launch<128, PAIR>(dev, tk, tv, a, sh) : mode == SPLIT ? launch<128, SPLIT>(dev, tk, tv, a, sh) : launch<128, FOLD>(dev, tk, tv, a, sh);
