@@ -39,9 +39,30 @@ struct TreeTensorPlan {
 TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int capacity, int asked);
 int tree_sm100_launch(grl_device* dev, const TreeArgs& a, const TreeTensorPlan& plan);
 
+// The parts of n_splits splits of every (sequence, kv head), `rows` rows each (tree_sm100.cu).
+int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows);
+// How the kernel for few rows lays a call out (tree_mma.cu): up to kTreeFewRows rows of a (sequence, kv head).
+constexpr int kTreeFewRows = 32;
+struct TreeMmaPlan {
+    int splits, cluster;
+    size_t workspace;
+};
+TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked);
+int tree_mma_launch(grl_device* dev, const TreeArgs& a, const TreeMmaPlan& plan);
+
 inline size_t tree_part_stride(size_t rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }
 
 #ifdef __CUDACC__
+// A look at a barrier that does not suspend the thread; it costs a third of a wait where the phase is over.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void tree_fail(int32_t* status, int what, int b, int value) {
     if (status && atomicCAS(status, 0, GRL_ERR_INVALID) == 0) {
         status[1] = (6 << 28) | what;

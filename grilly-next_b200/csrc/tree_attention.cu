@@ -225,14 +225,23 @@ struct TreePlan {
     bool tensor;
     int splits;
     size_t workspace;
+    bool few;
     TreeTensorPlan t;
+    TreeMmaPlan m;
 };
-static TreePlan tree_plan(const grl_device* dev, const grl_tree_params* p) {
+static TreePlan tree_plan(grl_device* dev, const grl_tree_params* p) {
     const grl_kv_layout& kv = p->kv;
     const int cap = kv.max_pages * kv.page_tokens, longest = p->max_seq_len > 0 && p->max_seq_len < cap ? p->max_seq_len : cap;
     const int R = p->n_tree * (p->num_q_heads / kv.num_kv_heads);
     TreePlan t{};
     t.tensor = p->kernel != GRL_KERNEL_SIMT_F32 && tensor_cores_apply(p);
+    t.few = t.tensor && R <= kTreeFewRows;
+    if (t.few) {
+        t.m = tree_mma_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, p->n_splits);
+        t.splits = t.m.splits;
+        t.workspace = t.m.workspace;
+        return t;
+    }
     if (t.tensor) {
         t.t = tree_sm100_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, cap, p->n_splits);
         t.splits = t.t.splits;
@@ -285,6 +294,7 @@ int grl_tree_attention(grl_device* dev, const grl_tree_params* p) {
     DeviceGuard g(dev->ordinal);
     dev->status_dirty = true;
     const bool c32 = kv.cache_dtype == GRL_F32, io32 = p->io_dtype == GRL_F32;
+    if (plan.few) return tree_mma_launch(dev, a, plan.m);
     if (plan.tensor) return tree_sm100_launch(dev, a, plan.t);
     rc = io32 ? (c32 ? launch_rows_d<float, float>(dev, a) : launch_rows_d<float, __nv_bfloat16>(dev, a))
        : (c32 ? launch_rows_d<__nv_bfloat16, float>(dev, a) : launch_rows_d<__nv_bfloat16, __nv_bfloat16>(dev, a));

@@ -95,16 +95,6 @@ struct Ctx {
     int32_t* status;
     long long limit;
 };
-// A look at a barrier that does not suspend the thread; it costs a third of a wait where the phase is over.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
 __device__ __forceinline__ bool wait_bar(const Ctx& c, int bar, uint32_t parity) {
     const uint32_t addr = c.bars + bar * 8;
     if (mbar_test(addr, parity)) return true;
@@ -845,6 +835,15 @@ static Mode mode_of(int R) { return R > BM ? PAIR : R > 64 ? SPLIT : FOLD; }
 static int piece_rows(Mode m) { return m == PAIR ? 256 : m == SPLIT ? 128 : 64; }
 
 }  // namespace tree
+
+int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows) {
+    using namespace tree;
+    const Share sh{a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G), 0, 1};
+    GRL_CUDA(launch_pdl(a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv, (a.R + kJoinRows - 1) / kJoinRows), 256, 0, dev->stream, a,
+                        sh, rows));
+    GRL_LAUNCHED("tree_join_kernel");
+    return GRL_OK;
+}
 
 // asked: the caller's number of splits, or 0.
 TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int capacity, int asked) {

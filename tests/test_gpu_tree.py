@@ -191,6 +191,12 @@ TREES = {
     "shares_of_wide": tree_case(70, 8, 2, 128, 32, [70 + 64 * (5 * i % 11) for i in range(30)], [70 - i for i in range(30)]),
     "shares_of_three_groups": tree_case(128, 16, 2, 64, 64, [900, 128, 300]),
     "shares_of_one_tile": tree_case(30, 8, 2, 128, 64, [30 + 100 * (5 * i % 11) for i in range(30)]),
+    "few_rows_one_split": tree_case(4, 8, 2, 128, 64, [700, 65, 4], kw_splits=1),
+    "few_rows_joined": tree_case(4, 8, 2, 128, 16, [3000, 65, 4], [4, 2, 0], kw_splits=17),
+    "few_rows_clusters": tree_case(8, 8, 2, 128, 32, [1500, 65, 8], [8, 2, 0], kw_splits=5),
+    "few_rows_64": tree_case(5, 6, 2, 64, 16, [2500, 200]), "few_rows_64_wide": tree_case(10, 6, 2, 64, 64, [2500, 200], [10, 0]),
+    "few_rows_32": tree_case(32, 2, 2, 128, 64, [600, 40], [32, 30]), "few_rows_17": tree_case(17, 1, 1, 128, 64, [333]),
+    "few_rows_star": tree_case(16, 2, 1, 128, 64, [16, 80], kind="star"),
     "hint_too_short": tree_case(8, 8, 2, 128, 64, [700, 64], kw_max_seq_len=100),
     "f32": tree_case(11, 6, 2, 64, 24, [300, 97, 11], cache="f32"),
     "f32_dim_32": tree_case(11, 6, 2, 32, 7, [100, 50], cache="f32"),
@@ -234,7 +240,7 @@ def test_float32_arithmetic_on_request(dev, name):
     cache.free()
 
 
-@pytest.mark.parametrize("T,kind,cache_type", [(6, "tree", "bf16"), (70, "tree", "bf16"), (2, "star", "bf16"), (6, "tree", "f32")])
+@pytest.mark.parametrize("T,kind,cache_type", [(4, "tree", "bf16"), (6, "tree", "bf16"), (30, "tree", "bf16"), (15, "tree", "bf16"), (70, "tree", "bf16"), (2, "star", "bf16"), (6, "tree", "f32")])
 def test_what_a_row_does_not_see_may_be_anything(dev, T, kind, cache_type):
     """Keys and values of other branches hold NaN and infinities: rows that do not see them are as if they were not there; the rest of the
     pools, past every sequence's end, is NaN in all of these tests."""
@@ -256,7 +262,7 @@ def test_what_a_row_does_not_see_may_be_anything(dev, T, kind, cache_type):
         cache.free()
 
 
-@pytest.mark.parametrize("T", [4, 30, 64])
+@pytest.mark.parametrize("T", [2, 8, 12, 30, 64])
 def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(T):
     """A budget of one cycle for the waits of long streams (a wait that the hardware suspends may still succeed, so the call is made until one runs
     out): the kernel returns, the failure is reported, and the call after it gives what the call before gave."""
