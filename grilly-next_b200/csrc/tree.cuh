@@ -31,23 +31,26 @@ struct TreeArgs {
 
 // How the tensor-core kernel lays a call out (tree_sm100.cu).
 struct TreeTensorPlan {
-    int splits;         // CTAs of a (sequence, kv head, group of rows), where ctas is 0
-    int ctas;           // > 0: CTAs that take equal shares of the batch
+    int splits;         // CTAs of a (sequence, kv head, group of rows)
     int groups;         // of rows of a (sequence, kv head)
     size_t workspace;
 };
-TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int capacity, int asked);
+TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked);
 int tree_sm100_launch(grl_device* dev, const TreeArgs& a, const TreeTensorPlan& plan);
 
 // The parts of n_splits splits of every (sequence, kv head), `rows` rows each (tree_sm100.cu).
 int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows);
 // How the kernel for few rows lays a call out (tree_mma.cu): up to kTreeFewRows rows of a (sequence, kv head).
-constexpr int kTreeFewRows = 32;
+// us, 16 rows of 8 kv heads, this kernel / the one of 128-row tiles: 1 x 300 tokens 8.8 / 9.9, 1 x 1001 9.8 / 12.9, 4 x 600 10.0 / 12.8, 4 x 4096
+// 18.5 / 24.9, 16 x 4096 46.2 / 56.1, 32 x 600 17.9 / 31.3, 32 x 4096 82.6 / 109, 1 x 131072 106 / 102.  With 32 rows as two operands of a warp,
+// one CTA an SM: 10.6 / 9.6, 11.6 / 11.8, 17.8 / 12.9, 32 / 25, 78 / 56, 33 / 31.5, 136 / 109; so it takes 16.
+constexpr int kTreeFewRows = 16;
 struct TreeMmaPlan {
     int splits, cluster;
+    bool alone;         // CTAs that must not share an SM
     size_t workspace;
 };
-TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked);
+TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int D, int longest, int asked);
 int tree_mma_launch(grl_device* dev, const TreeArgs& a, const TreeMmaPlan& plan);
 
 inline size_t tree_part_stride(size_t rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }

@@ -237,13 +237,13 @@ static TreePlan tree_plan(grl_device* dev, const grl_tree_params* p) {
     t.tensor = p->kernel != GRL_KERNEL_SIMT_F32 && tensor_cores_apply(p);
     t.few = t.tensor && R <= kTreeFewRows;
     if (t.few) {
-        t.m = tree_mma_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, p->n_splits);
+        t.m = tree_mma_plan(dev, kv.batch, kv.num_kv_heads, kv.head_dim, longest, p->n_splits);
         t.splits = t.m.splits;
         t.workspace = t.m.workspace;
         return t;
     }
     if (t.tensor) {
-        t.t = tree_sm100_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, cap, p->n_splits);
+        t.t = tree_sm100_plan(dev, kv.batch, kv.num_kv_heads, R, kv.head_dim, longest, p->n_splits);
         t.splits = t.t.splits;
         t.workspace = t.t.workspace;
         return t;

@@ -1,10 +1,10 @@
-// Attention of drafted trees of few rows over the bf16 cache: up to 32 rows (nodes x heads of the group) of a (sequence, kv head), head_dim 128 or
+// Attention of drafted trees of few rows over the bf16 cache: up to 16 rows (nodes x heads of the group) of a (sequence, kv head), head_dim 128 or
 // 64, pages of 64, 32 or 16 tokens.
 //
 // Bound by HBM where there is much to read, by latency where there is little, so 128-row tiles (tree_sm100.cu) are the wrong tool: their
 // set-up and epilogue take longer than a short cache.  One CTA is a split of a (sequence, kv head): a producer warp brings stages of 64 tokens
-// by TMA (boxes of 64 columns, 128-byte swizzle) into a ring; four compute warps take 16 tokens of each stage, with 16 or 32 rows as
-// one or two operands of mma.sync m16n8k16, and a running maximum and sum of their own for every row.  Two CTAs an SM.  The warps' sums meet in
+// by TMA (boxes of 64 columns, 128-byte swizzle) into a ring; four compute warps take 16 tokens of each stage, with the rows as
+// an operand of mma.sync m16n8k16, and a running maximum and sum of their own for every row.  Two CTAs an SM.  The warps' sums meet in
 // shared memory, those of splits in the shared memory of a cluster where the splits of a head are one, else in tree_join_kernel.
 // The predicate, and the cleaning of what lies past a sequence's end, concern the last stages only, as in tree_sm100.cu.
 #include <cuda.h>
@@ -31,8 +31,9 @@ using sm100::tma_load_2d;
 
 constexpr int BN = 64;                  // tokens of a stage
 constexpr int kThreads = 160;           // four compute warps and the producer
-constexpr int kRows = 32;               // rows of a CTA at most
+constexpr int kRows = kTreeFewRows;     // rows of a CTA: one operand
 constexpr long long kDrainCycles = 200000000;
+constexpr int kAloneSmem = 120 * 1024;  // more than half of an SM's: CTAs that must not share one
 template <int HD> struct Form {
     static constexpr int SLAB = BN * HD * 2, STAGE = 2 * SLAB, NST = 96 * 1024 / STAGE;
     static constexpr int Q = NST * STAGE;               // query rows, 16-byte pieces XOR-swizzled by row
@@ -98,12 +99,12 @@ struct Args {
     int cluster;                // > 1: the splits of a head are one cluster
 };
 
-// grid (splits, Hkv, B); RT operands of 16 rows
-template <int HD, int RT>
-__global__ void __launch_bounds__(kThreads, HD * RT > 128 ? 1 : 2)
+// grid (splits, Hkv, B)
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 2)
 tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Args args) {
     using F = Form<HD>;
-    constexpr int NST = F::NST, ROWS = 16 * RT;
+    constexpr int NST = F::NST;
     const TreeArgs& a = args.a;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw), base = (raw_addr + 1023u) & ~1023u;
@@ -187,7 +188,7 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const bool bad_tree = blk.bad_tree != 0;
     if (bad_tree && tid == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
     const int live_nodes = bad_tree ? 0 : n;
-    if (tid < ROWS) {
+    if (tid < kRows) {
         const int node = node_of(tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
         if (tid < a.R && node < live_nodes) {
@@ -206,14 +207,11 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __syncthreads();
 
     const int g = lane >> 2, t4 = lane & 3;
-    float o[RT][HD / 8][4], m_ref[RT][2], l[RT][2];
+    float o[HD / 8][4], m_ref[2], l[2];
 #pragma unroll
-    for (int x = 0; x < RT; ++x) {
-#pragma unroll
-        for (int j = 0; j < HD / 8; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
-        m_ref[x][0] = m_ref[x][1] = -INFINITY;
-        l[x][0] = l[x][1] = 0.f;
-    }
+    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    m_ref[0] = m_ref[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
     bool ok = true;
     if (warp == 4) {
         for (int p = p_begin + NST; p < p_end; ++p) {
@@ -233,6 +231,9 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const int q_row = (lane & 7) + ((mat & 1) << 3), q_col = mat >> 1;
         const int k_row = 16 * warp + (lane & 7) + ((mat >> 1) << 3), k_col = (mat & 1) << 3;
         const int v_row = 16 * warp + (lane & 7) + ((mat & 1) << 3), v_col = (mat >> 1) << 3;
+        uint32_t qf[HD / 16][4];
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) ldmatrix_x4(base + F::Q + q_row * (HD * 2) + (((2 * ks + q_col) ^ (q_row & 7)) << 4), qf[ks]);
         for (int p = p_begin; p < p_end && ok; ++p) {
             const int i = p - p_begin, s = i % NST;
             ok = __all_sync(0xffffffffu, wait_bar(full(s), (i / NST) & 1, blk, a, s));
@@ -269,69 +270,55 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     __syncwarp();
                 }
                 // ---- S = Q K^T, 16 tokens in two tiles of 8
-                float sc[RT][2][4];
+                float sc[2][4];
 #pragma unroll
-                for (int x = 0; x < RT; ++x)
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) sc[x][nt][0] = sc[x][nt][1] = sc[x][nt][2] = sc[x][nt][3] = 0.f;
+                for (int nt = 0; nt < 2; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     uint32_t kf[4];
                     ldmatrix_x4(kb + slab_off(k_row, 16 * ks + k_col), kf);
-#pragma unroll
-                    for (int x = 0; x < RT; ++x) {
-                        uint32_t qf[4];
-                        const int row = 16 * x + q_row;
-                        ldmatrix_x4(base + F::Q + row * (HD * 2) + (((2 * ks + q_col) ^ (row & 7)) << 4), qf);
-                        mma_bf16(sc[x][0], qf, kf[0], kf[1]);
-                        mma_bf16(sc[x][1], qf, kf[2], kf[3]);
-                    }
+                    mma_bf16(sc[0], qf[ks], kf[0], kf[1]);
+                    mma_bf16(sc[1], qf[ks], kf[2], kf[3]);
                 }
-                uint32_t pf[RT][4];
+                uint32_t pf[4];
 #pragma unroll
-                for (int x = 0; x < RT; ++x) {
+                for (int h = 0; h < 2; ++h) {           // rows g and g + 8
+                    float v[4] = {sc[0][2 * h], sc[0][2 * h + 1], sc[1][2 * h], sc[1][2 * h + 1]};
+                    if (nodes) {
+                        const uint4 seen = blk.seen[8 * h + g];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {           // rows g and g + 8
-                        float v[4] = {sc[x][0][2 * h], sc[x][0][2 * h + 1], sc[x][1][2 * h], sc[x][1][2 * h + 1]};
-                        if (nodes) {
-                            const uint4 seen = blk.seen[16 * x + 8 * h + g];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int key = tok0 + (e >> 1) * 8 + 2 * t4 + (e & 1), u = key - prefix;
-                                const uint32_t w = u < 64 ? (u < 32 ? seen.x : seen.y) : (u < 96 ? seen.z : seen.w);
-                                if (key >= len || (u >= 0 && !(w >> (u & 31) & 1u))) v[e] = -INFINITY;
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = tok0 + (e >> 1) * 8 + 2 * t4 + (e & 1), u = key - prefix;
+                            const uint32_t w = u < 64 ? (u < 32 ? seen.x : seen.y) : (u < 96 ? seen.z : seen.w);
+                            if (key >= len || (u >= 0 && !(w >> (u & 31) & 1u))) v[e] = -INFINITY;
                         }
-                        const float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) * a.scale_log2;
-                        // a new maximum, by more than 2^8: seldom, after the first few tiles
-                        if (__any_sync(0xffffffffu, mx > m_ref[x][h] + 8.f)) {
-                            float top = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                            const float m_new = top > m_ref[x][h] + 8.f ? top : m_ref[x][h];
-                            const float f = m_new == m_ref[x][h] ? 1.f : ex2(m_ref[x][h] - m_new);
-                            m_ref[x][h] = m_new;
-                            l[x][h] *= f;
-#pragma unroll
-                            for (int j = 0; j < HD / 8; ++j) { o[x][j][2 * h] *= f; o[x][j][2 * h + 1] *= f; }
-                        }
-                        const float off = m_ref[x][h] == -INFINITY ? 0.f : -m_ref[x][h];       // a row that has seen nothing yet
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = ex2(fmaf(v[e], a.scale_log2, off));
-                        l[x][h] += (v[0] + v[1]) + (v[2] + v[3]);
-                        pf[x][h] = pack_bf16(v[0], v[1]);
-                        pf[x][2 + h] = pack_bf16(v[2], v[3]);
                     }
+                    const float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) * a.scale_log2;
+                    // a new maximum, by more than 2^8: seldom, after the first few tiles
+                    if (__any_sync(0xffffffffu, mx > m_ref[h] + 8.f)) {
+                        float top = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const float m_new = top > m_ref[h] + 8.f ? top : m_ref[h];
+                        const float f = m_new == m_ref[h] ? 1.f : ex2(m_ref[h] - m_new);
+                        m_ref[h] = m_new;
+                        l[h] *= f;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; ++j) { o[j][2 * h] *= f; o[j][2 * h + 1] *= f; }
+                    }
+                    const float off = m_ref[h] == -INFINITY ? 0.f : -m_ref[h];       // a row that has seen nothing yet
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = ex2(fmaf(v[e], a.scale_log2, off));
+                    l[h] += (v[0] + v[1]) + (v[2] + v[3]);
+                    pf[h] = pack_bf16(v[0], v[1]);
+                    pf[2 + h] = pack_bf16(v[2], v[3]);
                 }
                 // ---- O += P V
 #pragma unroll
                 for (int dn = 0; dn < HD / 16; ++dn) {
                     uint32_t vf[4];
                     ldmatrix_x4_trans(vb + slab_off(v_row, 16 * dn + v_col), vf);
-#pragma unroll
-                    for (int x = 0; x < RT; ++x) {
-                        mma_bf16(o[x][2 * dn], pf[x], vf[0], vf[1]);
-                        mma_bf16(o[x][2 * dn + 1], pf[x], vf[2], vf[3]);
-                    }
+                    mma_bf16(o[2 * dn], pf, vf[0], vf[1]);
+                    mma_bf16(o[2 * dn + 1], pf, vf[2], vf[3]);
                 }
             }
             if (tok0 + 16 > prefix) fence_async_smem();         // cleaned rows, ahead of the copy that takes their place
@@ -339,12 +326,10 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (lane == 0) mbar_arrive(empty(s));
         }
 #pragma unroll
-        for (int x = 0; x < RT; ++x)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], 1);
-                l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], 2);
-            }
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
     }
     __syncthreads();            // the ring is free: every copy has come in and been read
     pdl_trigger();
@@ -356,15 +341,13 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     // blocks of eight columns XOR-swizzled by row, so that neither the stores nor the reads meet in a bank
     if (warp < 4) {
 #pragma unroll
-        for (int x = 0; x < RT; ++x)
+        for (int h = 0; h < 2; ++h) {
+            const int row = warp * kRows + 8 * h + g;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = warp * ROWS + 16 * x + 8 * h + g;
-#pragma unroll
-                for (int j = 0; j < HD / 8; ++j)
-                    *reinterpret_cast<float2*>(warp_o + row * HD + ((j ^ g) << 3) + 2 * t4) = make_float2(o[x][j][2 * h], o[x][j][2 * h + 1]);
-                if (t4 == 0) warp_ml[row] = make_float2(m_ref[x][h], l[x][h]);
-            }
+            for (int j = 0; j < HD / 8; ++j)
+                *reinterpret_cast<float2*>(warp_o + row * HD + ((j ^ g) << 3) + 2 * t4) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+            if (t4 == 0) warp_ml[row] = make_float2(m_ref[h], l[h]);
+        }
     }
     __syncthreads();
     // who writes row r, its columns 4 c..: v un-normalised
@@ -377,19 +360,19 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         reinterpret_cast<uint2*>(out)[c] = w;
     };
     const uint4 bad = make_uint4(blk.bad[0], blk.bad[1], blk.bad[2], blk.bad[3]);
-    float* part = a.part + (((size_t)b * a.Hkv + kvh) * a.n_splits + split) * (size_t)(ROWS * (HD + 2));
+    float* part = a.part + (((size_t)b * a.Hkv + kvh) * a.n_splits + split) * (size_t)(kRows * (HD + 2));
     for (int idx = tid; idx < a.R * (HD / 4); idx += kThreads) {
         const int r = idx / (HD / 4), c = idx % (HD / 4);
         float m = -INFINITY, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, warp_ml[w * ROWS + r].x);
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, warp_ml[w * kRows + r].x);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float2 ml = warp_ml[w * ROWS + r];
+            const float2 ml = warp_ml[w * kRows + r];
             if (ml.x == -INFINITY) continue;
             const float f = ex2(ml.x - m);
-            const float4 u = *reinterpret_cast<const float4*>(warp_o + (w * ROWS + r) * HD + (((c >> 1) ^ (r & 7)) << 3) + ((c & 1) << 2));
+            const float4 u = *reinterpret_cast<const float4*>(warp_o + (w * kRows + r) * HD + (((c >> 1) ^ (r & 7)) << 3) + ((c & 1) << 2));
             v.x = fmaf(f, u.x, v.x); v.y = fmaf(f, u.y, v.y); v.z = fmaf(f, u.z, v.z); v.w = fmaf(f, u.w, v.w);
             sum = fmaf(f, ml.y, sum);
         }
@@ -416,7 +399,7 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (c == 0) cta_ml[r] = make_float2(m, sum);
         } else {
             reinterpret_cast<float4*>(part)[r * (HD / 4) + c] = v;
-            if (c == 0) reinterpret_cast<float2*>(part + ROWS * HD)[r] = node_of(r) < live_nodes ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+            if (c == 0) reinterpret_cast<float2*>(part + kRows * HD)[r] = node_of(r) < live_nodes ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
         }
     }
     if (args.cluster > 1) {
@@ -471,19 +454,16 @@ static int make_pool_map(grl_device* dev, CUtensorMap* tm, const void* pool, con
 }
 
 using Kernel = void (*)(CUtensorMap, CUtensorMap, Args);
-static Kernel kernel_of(int D, int R) {
-    return D == 128 ? (R > 16 ? tree_mma_kernel<128, 2> : tree_mma_kernel<128, 1>) : (R > 16 ? tree_mma_kernel<64, 2> : tree_mma_kernel<64, 1>);
-}
+static Kernel kernel_of(int D) { return D == 128 ? tree_mma_kernel<128> : tree_mma_kernel<64>; }
 static int smem_of(int D) { return D == 128 ? Form<128>::TOTAL : Form<64>::TOTAL; }
 
 static int set_attributes(grl_device* dev) {
     static bool attr_set[64] = {};
     if (!attr_set[dev->ordinal & 63]) {      // a function attribute belongs to the device that was current
-        for (int D : {64, 128})
-            for (int R : {16, 32}) {
-                GRL_CUDA(cudaFuncSetAttribute(kernel_of(D, R), cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(D)));
-                GRL_CUDA(cudaFuncSetAttribute(kernel_of(D, R), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            }
+        for (int D : {64, 128}) {
+            GRL_CUDA(cudaFuncSetAttribute(kernel_of(D), cudaFuncAttributeMaxDynamicSharedMemorySize, kAloneSmem));
+            GRL_CUDA(cudaFuncSetAttribute(kernel_of(D), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
         attr_set[dev->ordinal & 63] = true;
     }
     return GRL_OK;
@@ -493,7 +473,7 @@ static int set_attributes(grl_device* dev) {
 
 // The split of a decode of as many heads and stages (decode_plan.h); the splits of a head are a cluster while they are short and clusters fit the GPU
 // at once.
-TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked) {
+TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int D, int longest, int asked) {
     using namespace treemma;
     DecodeShape d;
     d.heads = B * Hkv;
@@ -502,13 +482,14 @@ TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int R, int D, int lon
     d.mma = true;
     const auto fits = [&](bool, int c) {
         DeviceGuard g(dev->ordinal);
-        return set_attributes(dev) != GRL_OK ? 0 : max_active_clusters(dev, (const void*)kernel_of(D, R), kThreads, smem_of(D), c);
+        return set_attributes(dev) != GRL_OK ? 0 : max_active_clusters(dev, (const void*)kernel_of(D), kThreads, smem_of(D), c);
     };
     TreeMmaPlan p{};
     p.splits = asked > 0 ? asked : decode_splits(d, fits);
     p.cluster = 1;
     if (p.splits > 1 && p.splits <= kMaxCluster && (d.stages + p.splits - 1) / p.splits <= kClusterStages && d.heads <= fits(false, p.splits)) p.cluster = p.splits;
-    p.workspace = p.splits > 1 && p.cluster == 1 ? sizeof(float) * (size_t)d.heads * p.splits * (R > 16 ? 32 : 16) * (D + 2) : 0;
+    p.workspace = p.splits > 1 && p.cluster == 1 ? sizeof(float) * (size_t)d.heads * p.splits * kRows * (D + 2) : 0;
+    p.alone = p.splits > 1 && p.cluster == 1 && (long long)d.heads * p.splits <= d.sms;
     return p;
 }
 
@@ -520,9 +501,9 @@ int tree_mma_launch(grl_device* dev, const TreeArgs& a, const TreeMmaPlan& plan)
     if (!rc) rc = set_attributes(dev);
     if (rc) return rc;
     const Args args{a, a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G), plan.cluster};
-    GRL_CUDA(launch_pdl_cluster(kernel_of(a.D, a.R), dim3(a.n_splits, a.Hkv, a.B), kThreads, smem_of(a.D), dev->stream, plan.cluster, tk, tv, args));
+    GRL_CUDA(launch_pdl_cluster(kernel_of(a.D), dim3(a.n_splits, a.Hkv, a.B), kThreads, plan.alone ? kAloneSmem : smem_of(a.D), dev->stream, plan.cluster, tk, tv, args));
     GRL_LAUNCHED("tree_mma_kernel");
-    return a.n_splits > 1 && plan.cluster == 1 ? tree_join_launch(dev, a, a.R > 16 ? 32 : 16) : GRL_OK;
+    return a.n_splits > 1 && plan.cluster == 1 ? tree_join_launch(dev, a, kRows) : GRL_OK;
 }
 
 }  // namespace grl

@@ -11,10 +11,7 @@
 //   SPLIT   the even and the odd stages of one row tile, joined in the epilogue
 //   FOLD    up to 64 rows, twice in the tile: the first half of a chain's threads takes one stage of a pair, the second half the other.  P has zeros
 //           where a half's rows meet the other's keys, so that one product sums both; four streams are joined in the epilogue
-// The work is a list of pieces, runs of stages of one (sequence, kv head, group of rows): one for every CTA of the grid where the caller names the
-// number of splits or there are many sequences, else an equal share of all stages of the batch for every CTA, which may end one head, hold some
-// whole and begin another.  Whole heads are written by their CTA, the parts of others meet in tree_join_kernel (a CTA's own two merges would have to wait for its neighbours).  The loads of the next
-// piece run under the epilogue of the one before.
+// A CTA takes one split of the stages of one (sequence, kv head, group of rows); the rows of several splits meet in tree_join_kernel.
 // The predicate is applied to the last stages only, those with nodes in them: a row has one bit for each of 128 nodes.  There, rows
 // of V past the sequence's end, which may hold anything, are cleared in shared memory ahead of the product, and so are elements
 // that are no finite number; rows that see such an element get it added behind the epilogue, so that it reaches nobody else.
@@ -43,17 +40,13 @@ constexpr uint32_t TMEM_COLS = 512, TMEM_CHAIN = 256, TMEM_O = 128;     // a cha
 
 enum Mode { SPLIT, PAIR, FOLD };
 constexpr long long kDrainCycles = 200000000;       // 0.1 s: how long a CTA that gives up waits for its copies and products
-constexpr int kMaxShared = 128;             // sequences of a batch that is cut into equal shares
-// Behind the ring: barriers, flags and the lengths of the batch.
+// Behind the ring: barriers and flags.
 struct Block {
     uint64_t bars[32];
     uint32_t tmem;
-    int abort, stop, bad_tree;
+    int abort, bad_tree;
     uint32_t bad[4];                        // nodes with elements of V that are no finite number
     int8_t up[GRL_MAX_TREE];                // parents
-    int before[kMaxShared + 1];             // stages of the sequences before each one (of one head and group)
-    int len[kMaxShared];
-    uint8_t nodes[kMaxShared];
 };
 template <int HD, Mode MODE> struct Form {
     static constexpr int BOXES = HD / 64;
@@ -61,7 +54,7 @@ template <int HD, Mode MODE> struct Form {
     static constexpr int STAGE = 2 * SLAB;
     static constexpr int Q_TILE = BOXES * Q_BOX;
     static constexpr int STREAMS = MODE == FOLD ? 4 : MODE == SPLIT ? 2 : 1;        // of a row
-    static constexpr int ROWS = 256 / STREAMS;              // of a piece
+    static constexpr int ROWS = 256 / STREAMS;              // of a group
     static constexpr int Q_BYTES = MODE == PAIR ? 2 * Q_TILE : Q_TILE;
     static constexpr int OUT_BYTES = 256 * 32 * 4;          // 32 columns of 256 accumulator rows, where the queries were
     static constexpr int RING = Q_BYTES > OUT_BYTES ? Q_BYTES : OUT_BYTES;
@@ -72,15 +65,14 @@ template <int HD, Mode MODE> struct Form {
     static constexpr int BLOCK = RING + NST * STAGE;
     static constexpr int TOTAL = BLOCK + (int)sizeof(Block) + 1024;     // + slack for 1024-byte alignment
     static_assert(TOTAL <= 227 * 1024, "shared memory");
-    static constexpr size_t PART = (size_t)ROWS * (HD + 2);             // floats of a piece in the workspace: O, then (m, l)
+    static constexpr size_t PART = (size_t)ROWS * (HD + 2);             // floats of a CTA in the workspace: O, then (m, l)
     // barriers
     static constexpr int FULL = 0, EMPTY = NST, S_FULL = 2 * NST, P_READY = S_FULL + 4, O_PREV = P_READY + 4, O_DONE = O_PREV + 2, Q_READY = O_DONE + 2,
                          DRAIN = Q_READY + 1, NUM = DRAIN + 2;
     static_assert(NUM <= 32, "barrier block");
 };
-struct Share {
+struct Groups {
     uint32_t per_group;     // 2^32 / G rounded up: row / G is its product's upper half (rows and G below 2^15; 0: G is 1)
-    int ctas;               // > 0: equal shares of all stages; 0: one piece a CTA, grid (splits, Hkv * groups, B)
     int groups;             // of rows of a (sequence, kv head)
 };
 
@@ -163,87 +155,12 @@ __device__ __forceinline__ void clean_values(uint32_t slab, int k0, int prefix, 
 }
 
 
-__device__ __forceinline__ int node_of(const Share& sh, int r) { return sh.per_group ? (int)__umulhi((uint32_t)r, sh.per_group) : r; }
-struct Piece {
-    int b, hg, st0, ns;     // sequence, kv head * groups + group, first stage and stages
-    bool whole;
-    int part;               // where it goes in the workspace, where it is not whole
-};
-
-// Nodes and length of a sequence (0, 0 where they do not fit).
-__device__ __forceinline__ int fitting(const TreeArgs& a, int b, int* n, bool tell) {
-    int prefix;
-    const int k = tree_nodes(a, b, &prefix, tell);
-    *n = k < 0 ? 0 : k;
-    return k > 0 ? prefix + k : 0;
-}
-// Stages of the sequences before each one, by one warp; four sequences a lane.
-__device__ __forceinline__ void scan_batch(const TreeArgs& a, Block& k, bool tell) {
-    const int lane = threadIdx.x & 31;
-    int len[4], n[4], sum = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        len[e] = n[e] = 0;
-        if (4 * lane + e < a.B) len[e] = fitting(a, 4 * lane + e, &n[e], tell);
-    }
-    int at[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { at[e] = sum; sum += (len[e] + BN - 1) / BN; }
-    int before = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-    }
-    before -= sum;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        k.before[4 * lane + e] = before + at[e];
-        k.len[4 * lane + e] = len[e];
-        k.nodes[4 * lane + e] = (uint8_t)n[e];
-    }
-    if (lane == 31) k.before[kMaxShared] = before + sum;
-}
-// The share of CTA `cta` of the stages of the batch, which are fewer than 2^31 (tree_sm100_plan).
-__device__ __forceinline__ int share_begin(const Block& k, const TreeArgs& a, const Share& sh, int cta) {
-    return (int)((long long)k.before[kMaxShared] * a.Hkv * sh.groups * cta / sh.ctas);
-}
-// The sequence of a stage of the batch.
-__device__ __forceinline__ int sequence_at(const Block& k, int hgs, int stage) {
-    int lo = 0, hi = kMaxShared;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (k.before[mid] * hgs <= stage) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-// Walks the pieces of a CTA; every role does so for itself.
-struct Pieces {
-    int at, end;
-    __device__ __forceinline__ void start(const Block& k, const TreeArgs& a, const Share& sh) {
-        at = share_begin(k, a, sh, blockIdx.x);
-        end = share_begin(k, a, sh, blockIdx.x + 1);
-    }
-    __device__ __forceinline__ bool take(const Block& k, const TreeArgs& a, const Share& sh, Piece* p) {
-        if (at >= end) return false;
-        const int hgs = a.Hkv * sh.groups;
-        p->b = sequence_at(k, hgs, at);
-        const int stages = k.before[p->b + 1] - k.before[p->b], rem = at - k.before[p->b] * hgs;
-        p->hg = (int)((unsigned)rem / (unsigned)stages);
-        p->st0 = rem - p->hg * stages;
-        p->ns = min(stages - p->st0, end - at);
-        p->whole = p->ns == stages;
-        p->part = (int)blockIdx.x * 2 + (p->st0 == 0);       // a CTA goes on with one head at most, and begins one at most
-        at += p->ns;
-        return true;
-    }
-};
+__device__ __forceinline__ int node_of(const Groups& sh, int r) { return sh.per_group ? (int)__umulhi((uint32_t)r, sh.per_group) : r; }
 
 template <int HD, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeArgs a,
-                  const __grid_constant__ Share sh) {
+                  const __grid_constant__ Groups sh) {
     using F = Form<HD, MODE>;
     constexpr bool PAIR = MODE == tree::PAIR, FOLD = MODE == tree::FOLD;
     constexpr int NST = F::NST;
@@ -272,7 +189,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             mbar_init(bar(F::DRAIN + t), 1);
         }
         mbar_init(bar(F::Q_READY), 256);
-        blk.abort = blk.stop = blk.bad_tree = 0;
+        blk.abort = blk.bad_tree = 0;
         blk.bad[0] = blk.bad[1] = blk.bad[2] = blk.bad[3] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
@@ -283,47 +200,22 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     // all of the above beside the tail of the kernel before this one, nothing below
     pdl_wait();
-    if (sh.ctas && warp == WARP_TMA0) scan_batch(a, blk, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&blk.tmem);
-    // the piece of a CTA that has one only
-    Piece only{};
-    int only_len = 0, only_n = 0;
-    if (!sh.ctas) {
-        only.b = blockIdx.z;
-        only.hg = blockIdx.y;
-        only_len = fitting(a, only.b, &only_n, tid == 0);
-        const int stages = (only_len + BN - 1) / BN, per = (stages + a.n_splits - 1) / a.n_splits;
-        only.st0 = min(stages, (int)blockIdx.x * per);
-        only.ns = min(stages, ((int)blockIdx.x + 1) * per) - only.st0;
-        only.whole = a.n_splits == 1;
-        only.part = (only.b * gridDim.y + only.hg) * a.n_splits + blockIdx.x;
-    }
-    Pieces pieces{};
-    if (sh.ctas) pieces.start(blk, a, sh);
-    bool taken = false;
-    auto take = [&](Piece* p, int* len, int* n) -> bool {
-        if (sh.ctas) {
-            if (!pieces.take(blk, a, sh, p)) return false;
-            *len = blk.len[p->b];
-            *n = blk.nodes[p->b];
-            return true;
-        }
-        if (taken) return false;
-        taken = true;
-        *p = only;
-        *len = only_len;
-        *n = only_n;
-        return true;
-    };
+    // nodes and length of the sequence (0, 0 where they do not fit); this CTA's stages
+    const int b = blockIdx.z, kvh = blockIdx.y / sh.groups, r0 = blockIdx.y % sh.groups * F::ROWS;
+    int cached;
+    const int fits = tree_nodes(a, b, &cached, tid == 0), n = max(fits, 0), len = fits > 0 ? cached + fits : 0;
+    const int stages = (len + BN - 1) / BN, per = (stages + a.n_splits - 1) / a.n_splits;
+    const int st0 = min(stages, (int)blockIdx.x * per), ns = min(stages, ((int)blockIdx.x + 1) * per) - st0;
     // stages of chain t of ns, and its k-th one: all, or every second one, or every second pair
-    auto count_of = [&](int t, int ns) { return PAIR ? ns : FOLD ? ns / 4 * 2 + max(0, min(2, ns % 4 - 2 * t)) : (ns - t + 1) / 2; };
+    auto count_of = [&](int t) { return PAIR ? ns : FOLD ? ns / 4 * 2 + max(0, min(2, ns % 4 - 2 * t)) : (ns - t + 1) / 2; };
     auto stage_of = [&](int t, int k) { return PAIR ? k : FOLD ? 4 * (k >> 1) + 2 * t + (k & 1) : 2 * k + t; };
-    auto slot_of = [&](int t, int x) { return (PAIR ? 0 : t * F::SLOTS) + x % F::SLOTS; };        // of the x-th stage of a chain since the start
+    auto slot_of = [&](int t, int x) { return (PAIR ? 0 : t * F::SLOTS) + x % F::SLOTS; };        // of the x-th stage of a chain
     // steps of chain t over ns stages: one for each, or for two; a tile without rows takes none
-    auto steps_of = [&](int t, int ns, int r0) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : FOLD ? ((ns + 1) / 2 - t + 1) / 2 : (ns - t + 1) / 2; };
+    auto steps_of = [&](int t) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : FOLD ? ((ns + 1) / 2 - t + 1) / 2 : (ns - t + 1) / 2; };
 
     if (warp < WARP_SOFTMAX) {
       reg_dec<REGS_MISC>();
@@ -331,38 +223,33 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         // ------------------------------------------------------------------ TMA: a warp the stages of a chain (PAIR: the even or the odd ones)
         // A lane a copy: one lane's chain of waits and copies took some 1700 cycles a stage, longer than HBM takes to bring it.
         const int ppt = BN / a.P, t = uniform(warp == WARP_TMA1);
-        int done = 0, last = -1, len, n;        // stages of earlier pieces; the last one this warp has asked for
-        Piece pc;
-        bool ok = true;
-        while (ok && take(&pc, &len, &n)) {
-            const int32_t* table = a.block_table + (size_t)pc.b * a.max_pages;
-            const int kvh = pc.hg / sh.groups, count = count_of(t, pc.ns);
-            int first = pc.st0 * ppt;
-            int entry = table[min(first + lane, a.max_pages - 1)], next = table[min(first + 32 + lane, a.max_pages - 1)];
-            for (int k = PAIR ? (done ^ t) & 1 : 0; k < count; k += PAIR ? 2 : 1) {
-                const int p = pc.st0 + stage_of(t, k), s = slot_of(t, done + k), it = (done + k) / F::SLOTS;
-                if (p * ppt - first >= 32) {
-                    first += 32;
-                    entry = next;
-                    next = table[min(first + 32 + lane, a.max_pages - 1)];
-                }
-                if (it > 0 && !wait_bar_warp(ctx, F::EMPTY + s, (it - 1) & 1)) { ok = false; break; }
-                const int np = min(ppt, (len - p * BN + a.P - 1) / a.P);       // pages of the stage that hold tokens
-                if (lane == 0) mbar_expect_tx(bar(F::FULL + s), (uint32_t)(np * a.P * HD * 4));
-                __syncwarp();
-                // lane: page j, then K or V, then the box
-                constexpr int COPIES = 2 * F::BOXES;
-                const int j = lane / COPIES, v = lane / F::BOXES & 1, x = lane % F::BOXES;
-                int page = __shfl_sync(0xffffffffu, entry, (p * ppt - first + j) & 31);
-                if (j < np) {
-                    if ((unsigned)page >= (unsigned)a.num_pages) { tree_fail(a.status, TREE_BAD_PAGE, pc.b, page); page = 0; }
-                    tma_load_2d(base + F::RING + s * F::STAGE + v * F::SLAB + x * KV_BOX + j * a.P * 128, v ? &tmV : &tmK, x * 64,
-                                (page * a.Hkv + kvh) * a.P, bar(F::FULL + s));
-                }
-                __syncwarp();
-                last = done + k;
+        int last = -1;          // the last stage this warp has asked for
+        const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+        const int count = count_of(t);
+        int first = st0 * ppt;
+        int entry = table[min(first + lane, a.max_pages - 1)], next = table[min(first + 32 + lane, a.max_pages - 1)];
+        for (int k = PAIR ? t : 0; k < count; k += PAIR ? 2 : 1) {
+            const int p = st0 + stage_of(t, k), s = slot_of(t, k), it = k / F::SLOTS;
+            if (p * ppt - first >= 32) {
+                first += 32;
+                entry = next;
+                next = table[min(first + 32 + lane, a.max_pages - 1)];
             }
-            if (ok) done += count;
+            if (it > 0 && !wait_bar_warp(ctx, F::EMPTY + s, (it - 1) & 1)) break;
+            const int np = min(ppt, (len - p * BN + a.P - 1) / a.P);       // pages of the stage that hold tokens
+            if (lane == 0) mbar_expect_tx(bar(F::FULL + s), (uint32_t)(np * a.P * HD * 4));
+            __syncwarp();
+            // lane: page j, then K or V, then the box
+            constexpr int COPIES = 2 * F::BOXES;
+            const int j = lane / COPIES, v = lane / F::BOXES & 1, x = lane % F::BOXES;
+            int page = __shfl_sync(0xffffffffu, entry, (p * ppt - first + j) & 31);
+            if (j < np) {
+                if ((unsigned)page >= (unsigned)a.num_pages) { tree_fail(a.status, TREE_BAD_PAGE, b, page); page = 0; }
+                tma_load_2d(base + F::RING + s * F::STAGE + v * F::SLAB + x * KV_BOX + j * a.P * 128, v ? &tmV : &tmK, x * 64,
+                            (page * a.Hkv + kvh) * a.P, bar(F::FULL + s));
+            }
+            __syncwarp();
+            last = k;
         }
         if (*ctx.abort) {       // copies in flight land before the shared memory is given back
             const long long t0 = clock64();
@@ -375,61 +262,50 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const uint32_t qa = desc_lo(base + (PAIR ? t * F::Q_TILE : 0), 16);
         const uint32_t k_lo = desc_lo(base + F::RING, 16), v_lo = desc_lo(base + F::RING + F::SLAB, KV_BOX);
         const uint32_t s_tmem = (uint32_t)uniform((int)tmem_base) + (uint32_t)t * TMEM_CHAIN, o_tmem = s_tmem + TMEM_O;
-        int done = 0, steps_done = 0, count = 0, len, n;        // this chain's stages and steps, and pieces so far
-        Piece pc;
+        const int steps = uniform(steps_of(t)), others = PAIR ? uniform(steps_of(t ^ 1)) : 1, mine = uniform(count_of(t));
         bool ok = true;
-        while (ok && take(&pc, &len, &n)) {
-            const int ns = uniform(pc.ns), r0 = pc.hg % sh.groups * (PAIR ? 2 * BM : BM);
-            const int steps = uniform(steps_of(t, ns, r0)), others = PAIR ? uniform(steps_of(t ^ 1, ns, r0)) : 1;
-            const int mine = uniform(count_of(t, ns));
-            // S of a step: 64 columns of the buffers in turn; FOLD: both buffers, a stage each
-            auto issue_qk = [&](int i) -> bool {
-                const int ci = steps_done + i;
+        // S of a step: 64 columns of the buffers in turn; FOLD: both buffers, a stage each
+        auto issue_qk = [&](int i) -> bool {
 #pragma unroll
-                for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int k = FOLD ? 2 * i + half : i, s = slot_of(t, done + k);
-                    if (FOLD && k >= mine) break;
-                    if (!wait_bar_warp(ctx, F::FULL + s, ((done + k) / F::SLOTS) & 1)) return false;
-                    tc_fence_after();
-                    const uint32_t kb = k_lo + (uint32_t)s * (F::STAGE >> 4), d = s_tmem + (uint32_t)(FOLD ? half : ci & 1) * BN;
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        mma_ss2(d, qa + (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4), kb + (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4),
-                                IDESC_QK, ks != 0);
-                }
-                mma_commit(bar(F::S_FULL + 2 * t + (FOLD ? 0 : ci & 1)));
-                return true;
-            };
-            ok = wait_bar_warp(ctx, F::Q_READY, count & 1);
-            if (ok) tc_fence_after();
-            for (int i = 0; i < (FOLD ? 1 : 2) && i < steps && ok; ++i) ok = issue_qk(i);
-            for (int i = 0; i < steps && ok; ++i) {
-                const int ci = steps_done + i;
-                ok = wait_bar_warp(ctx, F::P_READY + 2 * t + (FOLD ? 0 : ci & 1), (FOLD ? ci : ci >> 1) & 1);
-                if (!ok) break;
+            for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
+                const int k = FOLD ? 2 * i + half : i, s = slot_of(t, k);
+                if (FOLD && k >= mine) break;
+                if (!wait_bar_warp(ctx, F::FULL + s, (k / F::SLOTS) & 1)) return false;
                 tc_fence_after();
+                const uint32_t kb = k_lo + (uint32_t)s * (F::STAGE >> 4), d = s_tmem + (uint32_t)(FOLD ? half : i & 1) * BN;
 #pragma unroll
-                for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int k = FOLD ? 2 * i + half : i, s = slot_of(t, done + k);
-                    if (FOLD && k >= mine) break;
-                    const uint32_t p_tmem = s_tmem + (FOLD ? (uint32_t)half * (BN / 2) : (uint32_t)(ci & 1) * BN), vb = v_lo + (uint32_t)s * (F::STAGE >> 4);
-#pragma unroll
-                    for (int ks = 0; ks < BN / 16; ++ks)
-                        mma_ts2(o_tmem, p_tmem + ks * 8, vb + (uint32_t)ks * (2048 >> 4), IdescPV<HD>::value, i > 0 || half > 0 || ks > 0);
-                    mma_commit(bar(F::EMPTY + s));
-                    // a stage that the other tile does not read is released for it too
-                    if (PAIR && others == 0) mma_commit(bar(F::EMPTY + s));
-                }
-                if (!FOLD && i + 2 == steps) mma_commit(bar(F::O_PREV + t));
-                // overwrites the buffer of P(i): in order behind its product
-                if (i + (FOLD ? 1 : 2) < steps) ok = issue_qk(i + (FOLD ? 1 : 2));
+                for (int ks = 0; ks < HD / 16; ++ks)
+                    mma_ss2(d, qa + (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4), kb + (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4),
+                            IDESC_QK, ks != 0);
             }
-            // for a chain without steps too, so that nobody falls two pieces behind
-            if (ok) mma_commit(bar(F::O_DONE + t));
-            done += mine;
-            steps_done += steps;
-            ++count;
+            mma_commit(bar(F::S_FULL + 2 * t + (FOLD ? 0 : i & 1)));
+            return true;
+        };
+        ok = wait_bar_warp(ctx, F::Q_READY, 0);
+        if (ok) tc_fence_after();
+        for (int i = 0; i < (FOLD ? 1 : 2) && i < steps && ok; ++i) ok = issue_qk(i);
+        for (int i = 0; i < steps && ok; ++i) {
+            ok = wait_bar_warp(ctx, F::P_READY + 2 * t + (FOLD ? 0 : i & 1), (FOLD ? i : i >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
+                const int k = FOLD ? 2 * i + half : i, s = slot_of(t, k);
+                if (FOLD && k >= mine) break;
+                const uint32_t p_tmem = s_tmem + (FOLD ? (uint32_t)half * (BN / 2) : (uint32_t)(i & 1) * BN), vb = v_lo + (uint32_t)s * (F::STAGE >> 4);
+#pragma unroll
+                for (int ks = 0; ks < BN / 16; ++ks)
+                    mma_ts2(o_tmem, p_tmem + ks * 8, vb + (uint32_t)ks * (2048 >> 4), IdescPV<HD>::value, i > 0 || half > 0 || ks > 0);
+                mma_commit(bar(F::EMPTY + s));
+                // a stage that the other tile does not read is released for it too
+                if (PAIR && others == 0) mma_commit(bar(F::EMPTY + s));
+            }
+            if (!FOLD && i + 2 == steps) mma_commit(bar(F::O_PREV + t));
+            // overwrites the buffer of P(i): in order behind its product
+            if (i + (FOLD ? 1 : 2) < steps) ok = issue_qk(i + (FOLD ? 1 : 2));
         }
+        // for a chain without steps too
+        if (ok) mma_commit(bar(F::O_DONE + t));
         if (!ok) {              // products in flight end before the tensor memory and the operands are given back
             mma_commit(bar(F::DRAIN + t));
             const long long t0 = clock64();
@@ -445,256 +321,238 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_addr = lane_addr + (uint32_t)t * TMEM_CHAIN, o_addr = s_addr + TMEM_O;
         constexpr int CH = HD / 8, PER = F::ROWS * CH / 256;     // 16-byte pieces of a query row, of a thread
-        int done = 0, steps_done = 0, count = 0, prevs = 0, len = 0, n = 0;
-        Piece pc{};
         auto meet = [] {        // both warpgroups; the barrier is for converged warps
             __syncwarp();
             asm volatile("bar.sync 1, 256;" ::: "memory");
         };
-        while (take(&pc, &len, &n)) {
-            const int b = pc.b, kvh = pc.hg / sh.groups, r0 = pc.hg % sh.groups * (PAIR ? 2 * BM : BM), ns = pc.ns, st0 = pc.st0, now_len = len, now_n = n,
-                      prefix = len - n;
-            const bool whole = pc.whole;
-            const int part_at = pc.part;
-            const int r = r0 + (PAIR ? t * BM : 0) + (FOLD ? row & 63 : row), node = node_of(sh, r);
-            {   // query rows as the K-major operand, rows past the last one zero; parents
-                const int up = a.parents && st_id < now_n ? a.parents[(size_t)b * a.T + st_id] : -1;
-                const int c = st_id % CH, first = st_id / CH;
-                const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD) + c;
-                uint4 v[PER];
+        const int prefix = len - n;
+        const bool whole = a.n_splits == 1;
+        const int r = r0 + (PAIR ? t * BM : 0) + (FOLD ? row & 63 : row), node = node_of(sh, r);
+        {   // query rows as the K-major operand, rows past the last one zero; parents
+            const int up = a.parents && st_id < n ? a.parents[(size_t)b * a.T + st_id] : -1;
+            const int c = st_id % CH, first = st_id / CH;
+            const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD) + c;
+            uint4 v[PER];
 #pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    const int g = r0 + first + e * (256 / CH), at = node_of(sh, g);
-                    v[e] = make_uint4(0u, 0u, 0u, 0u);
-                    if (g < a.R) v[e] = __ldg(q + (at * a.Hq + g - at * a.G) * CH);
-                }
+            for (int e = 0; e < PER; ++e) {
+                const int g = r0 + first + e * (256 / CH), at = node_of(sh, g);
+                v[e] = make_uint4(0u, 0u, 0u, 0u);
+                if (g < a.R) v[e] = __ldg(q + (at * a.Hq + g - at * a.G) * CH);
+            }
 #pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    const int qr = first + e * (256 / CH);
-                    const uint32_t to = base + (qr >> 7) * F::Q_TILE + (c >> 3) * Q_BOX + (qr & 127) * 128 + (((c & 7) ^ (qr & 7)) << 4);
-                    sts128(to, v[e]);
-                    if (FOLD) sts128(to + 64 * 128, v[e]);
+            for (int e = 0; e < PER; ++e) {
+                const int qr = first + e * (256 / CH);
+                const uint32_t to = base + (qr >> 7) * F::Q_TILE + (c >> 3) * Q_BOX + (qr & 127) * 128 + (((c & 7) ^ (qr & 7)) << 4);
+                sts128(to, v[e]);
+                if (FOLD) sts128(to + 64 * 128, v[e]);
+            }
+            if (a.parents && st_id < n) {
+                if (up < -1 || up >= st_id) blk.bad_tree = 1;
+                blk.up[st_id] = (int8_t)up;
+            }
+        }
+        fence_async_smem();
+        mbar_arrive(bar(F::Q_READY));
+        meet();
+        const bool bad_tree = *reinterpret_cast<volatile int*>(&blk.bad_tree) != 0;
+        if (bad_tree && st_id == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
+        const bool live = r < a.R && node < n && !bad_tree;
+        uint4 seen = make_uint4(0u, 0u, 0u, 0u);
+        if (live) {
+            if (!a.parents) seen = low_bits(node + 1);
+            else
+                for (int u = node; u >= 0; u = blk.up[u]) {         // up to the cached tokens: a tree's depth
+                    const uint32_t bit = 1u << (u & 31);
+                    seen.x |= u < 32 ? bit : 0u;
+                    seen.y |= u >> 5 == 1 ? bit : 0u;
+                    seen.z |= u >> 5 == 2 ? bit : 0u;
+                    seen.w |= u >> 5 == 3 ? bit : 0u;
                 }
-                if (a.parents && st_id < now_n) {
-                    if (up < -1 || up >= st_id) blk.bad_tree = 1;
-                    blk.up[st_id] = (int8_t)up;
+        }
+        __syncwarp();
+        const int nh = steps_of(t), mine = count_of(t);
+        float m_ref = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int i = 0; i < nh && ok; ++i) {
+            const int bf = FOLD ? 0 : i & 1, own = FOLD ? 2 * i + sub : i, k0 = (st0 + stage_of(t, own)) * BN;
+            const bool none = FOLD && own >= mine, nodes = none || k0 + BN > prefix;       // none: the pair's second stage is another CTA's, or past the end
+            // stages with nodes in them: their values are there when their scores are
+#pragma unroll
+            for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
+                const int k = FOLD ? 2 * i + half : i, v0 = (st0 + stage_of(t, k)) * BN, s = slot_of(t, k);
+                if (k < mine && v0 + BN > prefix) {
+                    ok = ok && wait_bar_warp(ctx, F::FULL + s, (k / F::SLOTS) & 1);
+                    if (!ok) break;
+                    clean_values<HD>(base + F::RING + s * F::STAGE + F::SLAB, v0, prefix, len, blk.bad, row);
+                    fence_async_smem();
                 }
             }
-            fence_async_smem();
-            mbar_arrive(bar(F::Q_READY));
-            meet();
-            const bool bad_tree = *reinterpret_cast<volatile int*>(&blk.bad_tree) != 0;
-            if (bad_tree && st_id == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
-            const bool live = r < a.R && node < n && !bad_tree;
-            uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-            if (live) {
-                if (!a.parents) seen = low_bits(node + 1);
-                else
-                    for (int u = node; u >= 0; u = blk.up[u]) {         // up to the cached tokens: a tree's depth
-                        const uint32_t bit = 1u << (u & 31);
-                        seen.x |= u < 32 ? bit : 0u;
-                        seen.y |= u >> 5 == 1 ? bit : 0u;
-                        seen.z |= u >> 5 == 2 ? bit : 0u;
-                        seen.w |= u >> 5 == 3 ? bit : 0u;
-                    }
-            }
-            __syncwarp();
-            const int nh = steps_of(t, ns, r0), mine = count_of(t, ns);
-            float m_ref = -INFINITY, l = 0.f;
-            bool ok = true;
-            for (int i = 0; i < nh && ok; ++i) {
-                const int ci = steps_done + i, bf = FOLD ? 0 : ci & 1, own = FOLD ? 2 * i + sub : i, k0 = (st0 + stage_of(t, own)) * BN;
-                const bool none = FOLD && own >= mine, nodes = none || k0 + BN > prefix;       // none: the pair's second stage is another CTA's, or past the end
-                // stages with nodes in them: their values are there when their scores are
-#pragma unroll
-                for (int half = 0; half < (FOLD ? 2 : 1); ++half) {
-                    const int k = FOLD ? 2 * i + half : i, v0 = (st0 + stage_of(t, k)) * BN, s = slot_of(t, done + k);
-                    if (k < mine && v0 + BN > prefix) {
-                        ok = ok && wait_bar_warp(ctx, F::FULL + s, ((done + k) / F::SLOTS) & 1);
-                        if (!ok) break;
-                        clean_values<HD>(base + F::RING + s * F::STAGE + F::SLAB, v0, prefix, now_len, blk.bad, row);
-                        fence_async_smem();
-                    }
-                }
-                if (!ok) break;
-                ok = wait_bar_warp(ctx, F::S_FULL + 2 * t + bf, (FOLD ? ci : ci >> 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                uint32_t sr[BN];
-                tmem_ld_x64_sync(s_addr + (FOLD ? sub : bf) * BN, sr);
-                if (nodes) {
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint32_t vis = none ? 0u : window32(seen, k0 + 32 * w - prefix);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (!(vis >> c & 1u)) sr[32 * w + c] = 0xff800000u;
-                    }
-                }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < BN; c += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(sr[c + 2 * e]), __uint_as_float(sr[c + 2 * e + 1]));
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                const float m_new = fmaxf(m_ref, mx * a.scale_log2);
-                if (i == 0) {
-                    m_ref = m_new;
-                } else {
-                    const bool need = m_new > m_ref + 8.f;
-                    if (__any_sync(0xffffffffu, need)) {
-                        // P V of the step before must be in O: it is once S of the next step is there (FOLD: of this one), issued behind it
-                        if constexpr (!FOLD)
-                            ok = i + 1 < nh ? wait_bar_warp(ctx, F::S_FULL + 2 * t + (bf ^ 1), ((ci + 1) >> 1) & 1)
-                                            : wait_bar_warp(ctx, F::O_PREV + t, prevs & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const float f = need ? ex2(m_ref - m_new) : 1.f;
-                        if (need) m_ref = m_new;
-                        l *= f;
-#pragma unroll
-                        for (int ch = 0; ch < HD / 32; ++ch) {
-                            uint32_t o[32];
-                            tmem_ld_x32_sync(o_addr + ch * 32, o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st_x32(o_addr + ch * 32, o);
-                        }
-                        tmem_st_wait();
-                    }
-                }
-                const float off = m_ref == -INFINITY ? 0.f : -m_ref;       // a row that has seen nothing yet
-                const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(off, off);
-                float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int ch = 0; ch < BN / 32; ++ch) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        float2 x = make_float2(__uint_as_float(sr[ch * 32 + c]), __uint_as_float(sr[ch * 32 + c + 1]));
-                        x = __ffma2_rn(x, sc2, nm2);
-                        const float2 pe = make_float2(ex2(x.x), ex2(x.y));
-                        rs[(c >> 1) & 3] = __fadd2_rn(rs[(c >> 1) & 3], pe);
-                        const __nv_bfloat162 pp = __floats2bfloat162_rn(pe.x, pe.y);
-                        pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&pp);
-                    }
-                    tmem_st_x16(s_addr + (FOLD ? sub * (BN / 2) : bf * BN) + ch * 16, pk);
-                }
-                if constexpr (FOLD) {
-                    uint32_t zero[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) zero[e] = 0u;
-                    tmem_st_x32(s_addr + (sub ^ 1) * (BN / 2), zero);
-                }
-                l += ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(bar(F::P_READY + 2 * t + bf));
-            }
-            if (ok) ok = wait_bar_warp(ctx, F::O_DONE + t, count & 1);
-            done += mine;
-            steps_done += nh;
-            ++count;
-            prevs += nh > 1;
-
-            // Epilogue.  The streams of a row meet at their common maximum; 32 columns at a time go through the queries' place, which both chains
-            // have done with, so that rows leave in whole pieces.
-            tc_fence_before();
-            meet();
-            ok = __all_sync(0xffffffffu, ok && !*ctx.abort);
+            if (!ok) break;
+            ok = wait_bar_warp(ctx, F::S_FULL + 2 * t + bf, (FOLD ? i : i >> 1) & 1);
+            if (!ok) break;
             tc_fence_after();
-            float m = m_ref, sum = l;
-            if constexpr (F::STREAMS > 1) {
-                float2* ml = reinterpret_cast<float2*>(smem);
-                ml[t * BM + row] = make_float2(m_ref, l);
-                meet();
-                m = -INFINITY;
-                sum = 0.f;
+            uint32_t sr[BN];
+            tmem_ld_x64_sync(s_addr + (FOLD ? sub : bf) * BN, sr);
+            if (nodes) {
 #pragma unroll
-                for (int x = 0; x < F::STREAMS; ++x) m = fmaxf(m, ml[x * F::ROWS + row % F::ROWS].x);
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t vis = none ? 0u : window32(seen, k0 + 32 * w - prefix);
 #pragma unroll
-                for (int x = 0; x < F::STREAMS; ++x) {
-                    const float2 v = ml[x * F::ROWS + row % F::ROWS];
-                    if (v.x != -INFINITY) sum = fmaf(ex2(v.x - m), v.y, sum);
+                    for (int c = 0; c < 32; ++c)
+                        if (!(vis >> c & 1u)) sr[32 * w + c] = 0xff800000u;
                 }
-                meet();
             }
-            const float w = (m_ref == -INFINITY ? 0.f : ex2(m_ref - m)) * (whole ? 1.f / sum : 1.f);
-            float* part = a.part + (size_t)part_at * F::PART;
-            const int rows = min(F::ROWS, a.R - r0), live_nodes = bad_tree ? 0 : now_n;
-            const bool full = ok && nh > 0 && m_ref != -INFINITY;
-            // a thread takes one 16-byte piece of every 32nd row
-            constexpr int K = F::ROWS / 32;
-            const int c = st_id & 7, rr0 = st_id >> 3;
-            int at[K];                  // elements from the batch's, or the part's, first; below 0: nothing to write
-            uint32_t alive = 0;
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < BN; c += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(sr[c + 2 * e]), __uint_as_float(sr[c + 2 * e + 1]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            const float m_new = fmaxf(m_ref, mx * a.scale_log2);
+            if (i == 0) {
+                m_ref = m_new;
+            } else {
+                const bool need = m_new > m_ref + 8.f;
+                if (__any_sync(0xffffffffu, need)) {
+                    // P V of the step before must be in O: it is once S of the next step is there (FOLD: of this one), issued behind it
+                    if constexpr (!FOLD)
+                        ok = i + 1 < nh ? wait_bar_warp(ctx, F::S_FULL + 2 * t + (bf ^ 1), ((i + 1) >> 1) & 1)
+                                        : wait_bar_warp(ctx, F::O_PREV + t, 0);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float f = need ? ex2(m_ref - m_new) : 1.f;
+                    if (need) m_ref = m_new;
+                    l *= f;
+#pragma unroll
+                    for (int ch = 0; ch < HD / 32; ++ch) {
+                        uint32_t o[32];
+                        tmem_ld_x32_sync(o_addr + ch * 32, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st_x32(o_addr + ch * 32, o);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            const float off = m_ref == -INFINITY ? 0.f : -m_ref;       // a row that has seen nothing yet
+            const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(off, off);
+            float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int ch = 0; ch < BN / 32; ++ch) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    float2 x = make_float2(__uint_as_float(sr[ch * 32 + c]), __uint_as_float(sr[ch * 32 + c + 1]));
+                    x = __ffma2_rn(x, sc2, nm2);
+                    const float2 pe = make_float2(ex2(x.x), ex2(x.y));
+                    rs[(c >> 1) & 3] = __fadd2_rn(rs[(c >> 1) & 3], pe);
+                    const __nv_bfloat162 pp = __floats2bfloat162_rn(pe.x, pe.y);
+                    pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&pp);
+                }
+                tmem_st_x16(s_addr + (FOLD ? sub * (BN / 2) : bf * BN) + ch * 16, pk);
+            }
+            if constexpr (FOLD) {
+                uint32_t zero[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) zero[e] = 0u;
+                tmem_st_x32(s_addr + (sub ^ 1) * (BN / 2), zero);
+            }
+            l += ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar(F::P_READY + 2 * t + bf));
+        }
+        if (ok) ok = wait_bar_warp(ctx, F::O_DONE + t, 0);
+
+        // Epilogue.  The streams of a row meet at their common maximum; 32 columns at a time go through the queries' place, which both chains
+        // have done with, so that rows leave in whole pieces.
+        tc_fence_before();
+        meet();
+        ok = __all_sync(0xffffffffu, ok && !*ctx.abort);
+        tc_fence_after();
+        float m = m_ref, sum = l;
+        if constexpr (F::STREAMS > 1) {
+            float2* ml = reinterpret_cast<float2*>(smem);
+            ml[t * BM + row] = make_float2(m_ref, l);
+            meet();
+            m = -INFINITY;
+            sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < F::STREAMS; ++x) m = fmaxf(m, ml[x * F::ROWS + row % F::ROWS].x);
+#pragma unroll
+            for (int x = 0; x < F::STREAMS; ++x) {
+                const float2 v = ml[x * F::ROWS + row % F::ROWS];
+                if (v.x != -INFINITY) sum = fmaf(ex2(v.x - m), v.y, sum);
+            }
+            meet();
+        }
+        const float w = (m_ref == -INFINITY ? 0.f : ex2(m_ref - m)) * (whole ? 1.f / sum : 1.f);
+        float* part = a.part + ((size_t)(b * gridDim.y + blockIdx.y) * a.n_splits + blockIdx.x) * F::PART;
+        const int rows = min(F::ROWS, a.R - r0), live_nodes = bad_tree ? 0 : n;
+        const bool full = ok && nh > 0 && m_ref != -INFINITY;
+        // a thread takes one 16-byte piece of every 32nd row
+        constexpr int K = F::ROWS / 32;
+        const int c = st_id & 7, rr0 = st_id >> 3;
+        int at[K];                  // elements from the batch's, or the part's, first; below 0: nothing to write
+        uint32_t alive = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int rg = r0 + rr0 + 32 * k, rn = node_of(sh, rg);
+            const bool l_ = rn < live_nodes;
+            alive |= (uint32_t)l_ << k;
+            at[k] = rr0 + 32 * k >= rows || !ok || !(whole || l_) ? -1 : (whole ? (rn * a.Hq + rg - rn * a.G) * HD : (rr0 + 32 * k) * HD) + 4 * c;
+        }
+        __nv_bfloat16* out_at = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD;
+#pragma unroll 1
+        for (int ch = 0; ch < HD / 32; ++ch) {
+            uint32_t o[32];
+            if (ok && nh > 0) tmem_ld_x32_sync(o_addr + ch * 32, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint4 v = make_uint4(__float_as_uint(__uint_as_float(o[4 * e]) * w), __float_as_uint(__uint_as_float(o[4 * e + 1]) * w),
+                                           __float_as_uint(__uint_as_float(o[4 * e + 2]) * w), __float_as_uint(__uint_as_float(o[4 * e + 3]) * w));
+                sts128(base + st_id * 128 + ((e ^ (st_id & 7)) << 4), full ? v : make_uint4(0u, 0u, 0u, 0u));
+            }
+            meet();
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int rg = r0 + rr0 + 32 * k, rn = node_of(sh, rg);
-                const bool l_ = rn < live_nodes;
-                alive |= (uint32_t)l_ << k;
-                at[k] = rr0 + 32 * k >= rows || !ok || !(whole || l_) ? -1 : (whole ? (rn * a.Hq + rg - rn * a.G) * HD : (rr0 + 32 * k) * HD) + 4 * c;
-            }
-            __nv_bfloat16* out_at = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)b * a.T * a.Hq + kvh * a.G) * HD;
-#pragma unroll 1
-            for (int ch = 0; ch < HD / 32; ++ch) {
-                uint32_t o[32];
-                if (ok && nh > 0) tmem_ld_x32_sync(o_addr + ch * 32, o);
+                if (at[k] < 0) continue;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (alive >> k & 1u) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint4 v = make_uint4(__float_as_uint(__uint_as_float(o[4 * e]) * w), __float_as_uint(__uint_as_float(o[4 * e + 1]) * w),
-                                               __float_as_uint(__uint_as_float(o[4 * e + 2]) * w), __float_as_uint(__uint_as_float(o[4 * e + 3]) * w));
-                    sts128(base + st_id * 128 + ((e ^ (st_id & 7)) << 4), full ? v : make_uint4(0u, 0u, 0u, 0u));
-                }
-                meet();
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (at[k] < 0) continue;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (alive >> k & 1u) {
-#pragma unroll
-                        for (int x = 0; x < F::STREAMS; ++x) {
-                            const uint4 u = lds128(base + (x * F::ROWS + rr0 + 32 * k) * 128 + ((c ^ (rr0 & 7)) << 4));
-                            v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
-                        }
-                    }
-                    if (whole) {
-                        const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
-                        *reinterpret_cast<uint2*>(out_at + at[k] + ch * 32) = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
-                    } else {
-                        *reinterpret_cast<float4*>(part + at[k] + ch * 32) = v;
+                    for (int x = 0; x < F::STREAMS; ++x) {
+                        const uint4 u = lds128(base + (x * F::ROWS + rr0 + 32 * k) * 128 + ((c ^ (rr0 & 7)) << 4));
+                        v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
                     }
                 }
-                meet();
-            }
-            const bool owner = st_id < F::ROWS && st_id < rows;         // of row r in the results
-            if (!whole && owner)
-                reinterpret_cast<float2*>(part + (size_t)F::ROWS * HD)[st_id] = live && ok && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
-            if ((blk.bad[0] | blk.bad[1] | blk.bad[2] | blk.bad[3]) != 0u) {         // rare: what is no finite number, for the rows that see it
-                if (owner && live && ok)
-                    for (int u = 0; u < now_n; ++u) {
-                        const uint32_t sees = u < 64 ? (u < 32 ? seen.x : seen.y) : (u < 96 ? seen.z : seen.w);
-                        if (!(blk.bad[u >> 5] & sees & (1u << (u & 31)))) continue;
-                        const int at = prefix + u, page = a.block_table[(size_t)b * a.max_pages + at / a.P];
-                        if ((unsigned)page >= (unsigned)a.num_pages) continue;
-                        const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v_pages) + (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * HD;
-                        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r % a.G) * HD;
-                        for (int d = 0; d < HD; ++d) {
-                            const float x = __bfloat162float(v[d]);
-                            if (isfinite(x)) continue;
-                            if (whole) out[d] = __float2bfloat16_rn(__bfloat162float(out[d]) + x);
-                            else part[(size_t)st_id * HD + d] += x;
-                        }
-                    }
-                meet();
-                if (st_id < 4) blk.bad[st_id] = 0u;
-            }
-            if (st_id == 0) {
-                blk.bad_tree = 0;
-                blk.stop = blk.abort;
+                if (whole) {
+                    const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
+                    *reinterpret_cast<uint2*>(out_at + at[k] + ch * 32) = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
+                } else {
+                    *reinterpret_cast<float4*>(part + at[k] + ch * 32) = v;
+                }
             }
             meet();
-            if (*reinterpret_cast<volatile int*>(&blk.stop)) break;
+        }
+        const bool owner = st_id < F::ROWS && st_id < rows;         // of row r in the results
+        if (!whole && owner)
+            reinterpret_cast<float2*>(part + (size_t)F::ROWS * HD)[st_id] = live && ok && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+        if ((blk.bad[0] | blk.bad[1] | blk.bad[2] | blk.bad[3]) != 0u) {         // rare: what is no finite number, for the rows that see it
+            if (owner && live && ok)
+                for (int u = 0; u < n; ++u) {
+                    const uint32_t sees = u < 64 ? (u < 32 ? seen.x : seen.y) : (u < 96 ? seen.z : seen.w);
+                    if (!(blk.bad[u >> 5] & sees & (1u << (u & 31)))) continue;
+                    const int at = prefix + u, page = a.block_table[(size_t)b * a.max_pages + at / a.P];
+                    if ((unsigned)page >= (unsigned)a.num_pages) continue;
+                    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v_pages) + (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * HD;
+                    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r % a.G) * HD;
+                    for (int d = 0; d < HD; ++d) {
+                        const float x = __bfloat162float(v[d]);
+                        if (isfinite(x)) continue;
+                        if (whole) out[d] = __float2bfloat16_rn(__bfloat162float(out[d]) + x);
+                        else part[(size_t)st_id * HD + d] += x;
+                    }
+                }
         }
     }
     pdl_trigger();
@@ -706,66 +564,37 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 }
 
 // Joins the parts of heads that several CTAs have worked on, a warp a row at a time: the parts' sums at their common maximum, eight parts on
-// their way at once.  With equal shares a CTA looks at one cut of the batch (blockIdx.x < ctas - 1), and takes the head there if it is the head's
-// first cut, or at one sequence (blockIdx.x - ctas + 1), whose rows it clears if it has no nodes.  It knows all that before the kernel ahead of it ends,
-// whose lengths are those of the call.
+// their way at once.
 constexpr int kJoinRows = 16;       // of a CTA
+// The fewest stages of a split.  us, split into 1 / 2 / 3 / 4: 4 x 8 heads x 700 tokens, 124 rows 15.2 / 15.9 / 15.2 / 15.0, 64 rows 14.2 / 15.7 /
+// 13.3 / 13.5; 1500 tokens, 64 rows 21.4 / 18.1 / - / 17.7.  More heads than SMs are not split: 20 x 8 x 4096, 124 rows 98.7 / 106 / 110, 64 rows
+// 106 / 102 / 105, 20 x 8 x 1024 40.4 / 49.3 / 57.2, 24 x 8 x 4096 101 / 121.  Equal shares of all stages for every CTA, heads cut where they fall, are no
+// faster anywhere: 32 x 8 x 4096, 64 rows 118 for 106, 4 x 8 x 1500 27.1 for 17.7, 1 x 8 x 131072 of 244 rows 172 for 163.
+constexpr int kSplitStages = 4;
 template <int HD>
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Share sh, int piece_rows) {
-    __shared__ Block blk;
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Groups sh, int part_rows) {
     const int hgs = a.Hkv * sh.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int b = blockIdx.x / hgs, hg = blockIdx.x % hgs, c0 = 0, parts = a.n_splits;
-    bool dense = true, clear = false;
-    if (sh.ctas && warp == 0) scan_batch(a, blk, false);
-    __syncthreads();
+    const int b = blockIdx.x / hgs, hg = blockIdx.x % hgs;
     pdl_wait();                 // every CTA, or the kernel behind this one could start before the one ahead of it has ended
     pdl_trigger();
-    if (sh.ctas) {
-        const int all = blk.before[kMaxShared] * hgs;
-        if ((int)blockIdx.x < sh.ctas - 1) {
-            const int cut = share_begin(blk, a, sh, blockIdx.x + 1), prev = share_begin(blk, a, sh, blockIdx.x);
-            if (cut >= all) return;
-            b = sequence_at(blk, hgs, cut);
-            const int stages = blk.before[b + 1] - blk.before[b], rem = cut - blk.before[b] * hgs;
-            hg = rem / stages;
-            const int first = cut - (rem - hg * stages);
-            if (first == cut || prev > first || prev == cut) return;     // between heads, or not the head's first cut
-            // the last CTA whose share begins at or before a stage has it
-            c0 = blockIdx.x;
-            parts = (int)(((long long)(first + stages) * sh.ctas - 1) / all) - c0 + 1;
-            dense = all >= sh.ctas;
-        } else {
-            b = blockIdx.x - (sh.ctas - 1);
-            if (blk.nodes[b]) return;
-            clear = true;
-            parts = 0;
-        }
-    }
     constexpr int V = HD / 32;              // columns of a lane
-    if (clear) {
-        const size_t n = (size_t)a.T * a.Hq * HD / 8;
-        uint4* out = reinterpret_cast<uint4*>(a.out) + b * n;
-        for (size_t i = (size_t)blockIdx.y * 256 + threadIdx.x; i < n; i += (size_t)gridDim.y * 256) out[i] = make_uint4(0u, 0u, 0u, 0u);
-        return;
-    }
-    const size_t stride = (size_t)piece_rows * (HD + 2);
-    const float* first_part = a.part + (sh.ctas ? (size_t)c0 * 2 : (size_t)blockIdx.x * a.n_splits) * stride;
-    const int kvh = hg / sh.groups, r0 = hg % sh.groups * piece_rows, rows = min(piece_rows, a.R - r0);
+    const size_t stride = (size_t)part_rows * (HD + 2);
+    const float* first_part = a.part + (size_t)blockIdx.x * a.n_splits * stride;
+    const int kvh = hg / sh.groups, r0 = hg % sh.groups * part_rows, rows = min(part_rows, a.R - r0);
     for (int rr = blockIdx.y * kJoinRows + warp; rr < min(rows, (int)(blockIdx.y + 1) * kJoinRows); rr += 8) {
         float m = -INFINITY, l = 0.f, acc[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) acc[c] = 0.f;
-        for (int i0 = 0; i0 < parts; i0 += 8) {
+        for (int i0 = 0; i0 < a.n_splits; i0 += 8) {
             float2 ml[8];
             float o[8][V];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int i = i0 + j;
                 ml[j] = make_float2(-INFINITY, 0.f);
-                if (i >= parts || (!dense && share_begin(blk, a, sh, c0 + i) == share_begin(blk, a, sh, c0 + i + 1))) continue;
-                // shares: the part that begins the head is its CTA's second place, the others are their CTAs' first
-                const float* p = first_part + (sh.ctas ? (size_t)2 * i + (i == 0) : (size_t)i) * stride;
-                ml[j] = __ldcg(reinterpret_cast<const float2*>(p + (size_t)piece_rows * HD) + rr);
+                if (i >= a.n_splits) continue;
+                const float* p = first_part + (size_t)i * stride;
+                ml[j] = __ldcg(reinterpret_cast<const float2*>(p + (size_t)part_rows * HD) + rr);
                 if constexpr (V == 4) {
                     const float4 f = __ldcg(reinterpret_cast<const float4*>(p + (size_t)rr * HD) + lane);
                     o[j][0] = f.x; o[j][1] = f.y; o[j][2] = f.z; o[j][3] = f.w;
@@ -814,57 +643,45 @@ static int make_pool_map(grl_device* dev, CUtensorMap* tm, const void* pool, con
     return get_tensor_map(dev, k, tm);
 }
 
+static int join(grl_device* dev, const TreeArgs& a, const Groups& sh, int part_rows) {
+    const dim3 grid(a.B * a.Hkv * sh.groups, (min(part_rows, a.R) + kJoinRows - 1) / kJoinRows);
+    GRL_CUDA(launch_pdl(a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<64>, grid, 256, 0, dev->stream, a, sh, part_rows));
+    GRL_LAUNCHED("tree_join_kernel");
+    return GRL_OK;
+}
+
 template <int HD, Mode MODE>
-static int launch(grl_device* dev, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a, const Share& sh) {
+static int launch(grl_device* dev, const CUtensorMap& tk, const CUtensorMap& tv, const TreeArgs& a, const Groups& sh) {
     using F = Form<HD, MODE>;
     static bool attr_set[64] = {};
     if (!attr_set[dev->ordinal & 63]) {      // a function attribute belongs to the device that was current
         GRL_CUDA(cudaFuncSetAttribute(tree_sm100_kernel<HD, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::TOTAL));
         attr_set[dev->ordinal & 63] = true;
     }
-    const dim3 grid = sh.ctas ? dim3(sh.ctas) : dim3(a.n_splits, a.Hkv * sh.groups, a.B);
-    GRL_CUDA(launch_pdl(tree_sm100_kernel<HD, MODE>, grid, kThreads, F::TOTAL, dev->stream, tk, tv, a, sh));
+    GRL_CUDA(launch_pdl(tree_sm100_kernel<HD, MODE>, dim3(a.n_splits, a.Hkv * sh.groups, a.B), kThreads, F::TOTAL, dev->stream, tk, tv, a, sh));
     GRL_LAUNCHED("tree_sm100_kernel");
-    if (!sh.ctas && a.n_splits == 1) return GRL_OK;
-    GRL_CUDA(launch_pdl(tree_join_kernel<HD>, dim3(sh.ctas ? sh.ctas - 1 + a.B : a.B * a.Hkv * sh.groups, (min(F::ROWS, a.R) + kJoinRows - 1) / kJoinRows), 256, 0, dev->stream, a, sh, F::ROWS));
-    GRL_LAUNCHED("tree_join_kernel");
-    return GRL_OK;
+    return a.n_splits == 1 ? GRL_OK : join(dev, a, sh, F::ROWS);
 }
 
 static Mode mode_of(int R) { return R > BM ? PAIR : R > 64 ? SPLIT : FOLD; }
-static int piece_rows(Mode m) { return m == PAIR ? 256 : m == SPLIT ? 128 : 64; }
+static int rows_of(Mode m) { return m == PAIR ? 256 : m == SPLIT ? 128 : 64; }
+static Groups groups_of(int G, int groups) { return {G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G), groups}; }
 
 }  // namespace tree
 
-int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows) {
-    using namespace tree;
-    const Share sh{a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G), 0, 1};
-    GRL_CUDA(launch_pdl(a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<64>, dim3(a.B * a.Hkv, (a.R + kJoinRows - 1) / kJoinRows), 256, 0, dev->stream, a,
-                        sh, rows));
-    GRL_LAUNCHED("tree_join_kernel");
-    return GRL_OK;
-}
+int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows) { return tree::join(dev, a, tree::groups_of(a.G, 1), rows); }
 
 // asked: the caller's number of splits, or 0.
-TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int capacity, int asked) {
+TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked) {
     using namespace tree;
-    const int rows = piece_rows(mode_of(R)), groups = (R + rows - 1) / rows, sms = dev->prop.multiProcessorCount;
-    const long long heads = (long long)B * Hkv * groups, stages = (longest + BN - 1) / BN;
+    const int rows = rows_of(mode_of(R)), sms = dev->prop.multiProcessorCount;
     TreeTensorPlan p{};
-    p.groups = groups;
-    const size_t part = sizeof(float) * (size_t)rows * (D + 2);
-    if (asked > 0 || B > kMaxShared || heads * (capacity / BN + 1) >= (1LL << 31)) {
-        long long s = asked > 0 ? asked : sms / heads;
-        if (asked <= 0 && s > stages / 2) s = stages / 2;
-        p.splits = (int)(s < 1 ? 1 : s > 4096 ? 4096 : s);
-        p.workspace = p.splits == 1 ? 0 : part * heads * p.splits;
-        return p;
-    }
-    // equal shares of at least two stages a CTA
-    const long long ctas = (heads * stages + 1) / 2;
-    p.splits = 1;
-    p.ctas = (int)(ctas < 1 ? 1 : ctas < sms ? ctas : sms);
-    p.workspace = part * 2 * p.ctas;
+    p.groups = (R + rows - 1) / rows;
+    const long long heads = (long long)B * Hkv * p.groups, stages = (longest + BN - 1) / BN;
+    long long s = asked > 0 ? asked : sms / heads;
+    if (asked <= 0 && s > stages / kSplitStages) s = stages / kSplitStages;
+    p.splits = (int)(s < 1 ? 1 : s);
+    p.workspace = p.splits == 1 ? 0 : sizeof(float) * (size_t)rows * (D + 2) * heads * p.splits;
     return p;
 }
 
@@ -874,7 +691,7 @@ int tree_sm100_launch(grl_device* dev, const TreeArgs& a, const TreeTensorPlan& 
     int rc = make_pool_map(dev, &tk, a.k_pages, a);
     if (!rc) rc = make_pool_map(dev, &tv, a.v_pages, a);
     if (rc) return rc;
-    const Share sh{a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G), plan.ctas, plan.groups};
+    const Groups sh = groups_of(a.G, plan.groups);
     const Mode mode = mode_of(a.R);
     if (a.D == 128)
         return mode == PAIR ? launch<128, PAIR>(dev, tk, tv, a, sh) : mode == SPLIT ? launch<128, SPLIT>(dev, tk, tv, a, sh) : launch<128, FOLD>(dev, tk, tv, a, sh);
