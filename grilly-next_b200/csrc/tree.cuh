@@ -98,15 +98,10 @@ __device__ __forceinline__ uint4 low_bits(int n) {      // bits 0 .. n-1 of 128
     const auto word = [n](int w) { const int k = n - 32 * w; return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
     return make_uint4(word(0), word(1), word(2), word(3));
 }
-// The whole CTA (at least GRL_MAX_TREE threads) calls it; returns whether the parents are a tree.
-__device__ __forceinline__ bool tree_masks(TreeMasks& m, const int32_t* parents, int n) {
+// The whole CTA (at least GRL_MAX_TREE threads) calls it, thread t with the parent of node t; returns whether the parents are a tree.
+__device__ __forceinline__ bool tree_masks(TreeMasks& m, int p, int n) {
     const int t = threadIdx.x;
-    if (!parents) {
-        if (t < n) m.seen[t] = low_bits(t + 1);
-        __syncthreads();
-        return true;
-    }
-    int p = t < n ? parents[t] : -1;
+    if (t >= n) p = -1;
     const bool bad = t < n && (p < -1 || p >= t);
     if (bad) p = -1;
     uint4 own = make_uint4(0u, 0u, 0u, 0u);

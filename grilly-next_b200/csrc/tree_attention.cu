@@ -5,7 +5,9 @@
 namespace grl {
 
 constexpr int kTreeKeys = 32;       // keys of a tile of the float32 kernel
-constexpr int kTreeRows = 8;        // rows of a CTA of it, a warp each
+constexpr int kTreeRun = 4;         // rows of a warp of it
+constexpr int kTreeWarps = 8;       // of a CTA
+inline int tree_chunks(int R) { return (R + kTreeWarps * kTreeRun - 1) / (kTreeWarps * kTreeRun); }
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -17,22 +19,35 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
     return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-// grid (splits, Hkv x chunks of rows, B).  A tile of 32 keys lies in shared memory as float32; a lane forms the score of one key, then
-// the warp's lanes share out the columns of the output.
+// grid (splits, Hkv x chunks of rows, B), the fours of rows shared out evenly.  A tile of 32 keys lies in shared memory as float32; a
+// lane forms the scores of one key with the four rows of its warp, then the warp's lanes share out the columns of the output: a key, or a value,
+// that has been read from shared memory meets four rows.  The next tile is on its way to registers meanwhile.
+// Bound by shared-memory reads where there are many rows (8 x 8 heads x 4000 tokens, 64 rows of 128: 468 us, 18 TFLOP/s), by the chain of length, page
+// and tile where there are few.  us, a row a warp / four: 5 x 2 heads x 777 tokens, 33 rows of 64 24.0 / 18.5; one row, 1 x 8 x 4000, 108 with a warp's
+// loads to a CTA, 26 with eight.
 template <typename TIO, typename TC, int D>
-__global__ void __launch_bounds__(32 * kTreeRows) tree_rows_kernel(const __grid_constant__ TreeArgs a) {
-    extern __shared__ float smem[];
-    __shared__ TreeMasks masks;
-    float* ks = smem;                               // [32][D + 1]
-    float* vs = ks + kTreeKeys * (D + 1);           // [32][D]
-    float* qs = vs + kTreeKeys * D;                 // [8][D]
-    const int chunks = (a.R + kTreeRows - 1) / kTreeRows;
-    const int split = blockIdx.x, kvh = blockIdx.y / chunks, b = blockIdx.z;
+__global__ void __launch_bounds__(32 * kTreeWarps) tree_rows_kernel(const __grid_constant__ TreeArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    __shared__ int up[GRL_MAX_TREE];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int r = blockIdx.y % chunks * kTreeRows + warp, t = r / a.G, g = r % a.G;
+    float* ks = smem;                               // [32][D + 4]
+    float* vs = ks + kTreeKeys * (D + 4);           // [32][D]
+    float* qs = vs + kTreeKeys * D + warp * kTreeRun * D;                                        // this warp's [4][D]
+    float* ps = vs + kTreeKeys * D + kTreeWarps * kTreeRun * D + warp * kTreeRun * kTreeKeys;   // and its weights [4][32]
+    const int chunks = (a.R + kTreeWarps * kTreeRun - 1) / (kTreeWarps * kTreeRun), fours = ((a.R + kTreeRun - 1) / kTreeRun + chunks - 1) / chunks;
+    const int split = blockIdx.x, kvh = blockIdx.y / chunks, b = blockIdx.z;
+    const int r0 = warp < fours ? (blockIdx.y % chunks * fours + warp) * kTreeRun : a.R;
+    pdl_wait();
+    pdl_trigger();
     int prefix;
     int n = tree_nodes(a, b, &prefix, tid == 0);
-    if (n > 0 && !tree_masks(masks, a.parents ? a.parents + (size_t)b * a.T : nullptr, n)) {
+    bool bad = false;
+    if (a.parents)
+        for (int t = tid; t < n; t += 32 * kTreeWarps) {
+            up[t] = a.parents[(size_t)b * a.T + t];
+            bad |= up[t] < -1 || up[t] >= t;
+        }
+    if (__syncthreads_or(bad)) {
         if (tid == 0) tree_fail(a.status, TREE_BAD_PARENT, b, n);
         n = 0;
     }
@@ -40,77 +55,148 @@ __global__ void __launch_bounds__(32 * kTreeRows) tree_rows_kernel(const __grid_
     const int len = n ? prefix + n : 0;
     const int tiles = (len + kTreeKeys - 1) / kTreeKeys, per = (tiles + a.n_splits - 1) / a.n_splits;
     const int k_begin = min(len, split * per * kTreeKeys), k_end = min(len, (split + 1) * per * kTreeKeys);
-    const bool live = r < a.R && t < n;
-    const size_t io = (((size_t)b * a.T + t) * a.Hq + kvh * a.G + g) * D;
-    for (int d = lane; d < D; d += 32) qs[warp * D + d] = live ? load_as_float<TIO>(reinterpret_cast<const TIO*>(a.q) + io + d) * a.scale_log2 : 0.f;
-    const uint4 seen = live ? masks.seen[t] : make_uint4(0u, 0u, 0u, 0u);
-    float m = -INFINITY, l = 0.f, acc[D / 32];
+    // row x of the warp: element of the first of its head in q and out, whether it is a node's, and the nodes it sees
+    size_t io[kTreeRun];
+    bool live[kTreeRun], some = false;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+    for (int x = 0; x < kTreeRun; ++x) {
+        const int r = r0 + x, t = r / a.G;
+        live[x] = r < a.R && t < n;
+        some |= live[x];
+        io[x] = (((size_t)b * a.T + t) * a.Hq + kvh * a.G + r - t * a.G) * D;
+        for (int d = lane; d < D; d += 32) qs[x * D + d] = live[x] ? load_as_float<TIO>(reinterpret_cast<const TIO*>(a.q) + io[x] + d) * a.scale_log2 : 0.f;
+    }
+    uint4 seen = make_uint4(0u, 0u, 0u, 0u);        // lane x: of row x
+    if (lane < kTreeRun && r0 + lane < a.R && (r0 + lane) / a.G < n) {
+        const int node = (r0 + lane) / a.G;
+        if (!a.parents) seen = low_bits(node + 1);
+        else
+            for (int u = node; u >= 0; u = up[u]) {
+                const uint32_t bit = 1u << (u & 31);
+                seen.x |= u < 32 ? bit : 0u;
+                seen.y |= u >> 5 == 1 ? bit : 0u;
+                seen.z |= u >> 5 == 2 ? bit : 0u;
+                seen.w |= u >> 5 == 3 ? bit : 0u;
+            }
+    }
+    __syncwarp();
+    float m[kTreeRun], l[kTreeRun], acc[kTreeRun][D / 32];
+#pragma unroll
+    for (int x = 0; x < kTreeRun; ++x) {
+        m[x] = -INFINITY;
+        l[x] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[x][i] = 0.f;
+    }
     const TC* kp = reinterpret_cast<const TC*>(a.k_pages);
     const TC* vp = reinterpret_cast<const TC*>(a.v_pages);
     const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+    constexpr int PER = kTreeKeys * (D / 4) / (32 * kTreeWarps);       // 16-byte pieces of a tile of keys, of a thread
+    float4 kx[PER], vx[PER];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int idx = tid + e * 32 * kTreeWarps, d = idx % (D / 4) * 4, at = k0 + idx / (D / 4);
+            kx[e] = vx[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at >= k_end) continue;
+            const int page = table[at / a.P];
+            if ((unsigned)page < (unsigned)a.num_pages) {
+                const size_t off = (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * D + d;
+                kx[e] = load4<TC>(kp + off);
+                vx[e] = load4<TC>(vp + off);
+            } else if (d == 0) {
+                tree_fail(a.status, TREE_BAD_PAGE, b, page);
+            }
+        }
+    };
+    if (k_begin < k_end) fetch(k_begin);
     for (int k0 = k_begin; k0 < k_end; k0 += kTreeKeys) {
         __syncthreads();
-        for (int idx = tid; idx < kTreeKeys * (D / 4); idx += 32 * kTreeRows) {
-            const int key = idx / (D / 4), d = idx % (D / 4) * 4, at = k0 + key;
-            float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
-            if (at < k_end) {
-                const int page = table[at / a.P];
-                if ((unsigned)page < (unsigned)a.num_pages) {
-                    const size_t off = (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * D + d;
-                    kx = load4<TC>(kp + off);
-                    vx = load4<TC>(vp + off);
-                } else if (d == 0) {
-                    tree_fail(a.status, TREE_BAD_PAGE, b, page);
-                }
-            }
-            float* kd = ks + key * (D + 1) + d;
-            kd[0] = kx.x; kd[1] = kx.y; kd[2] = kx.z; kd[3] = kx.w;
-            *reinterpret_cast<float4*>(vs + key * D + d) = vx;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int idx = tid + e * 32 * kTreeWarps, key = idx / (D / 4), d = idx % (D / 4) * 4;
+            *reinterpret_cast<float4*>(ks + key * (D + 4) + d) = kx[e];
+            *reinterpret_cast<float4*>(vs + key * D + d) = vx[e];
         }
         __syncthreads();
-        if (!live) continue;
-        const int u = k0 + lane - prefix;       // node of this key, below 0 a cached token
-        const uint32_t word = u < 64 ? (u < 32 ? seen.x : seen.y) : (u < 96 ? seen.z : seen.w);
-        const bool vis = k0 + lane < k_end && (u < 0 || (word >> (u & 31) & 1u));
-        float s = 0.f;
-#pragma unroll 16
-        for (int d = 0; d < D; ++d) s = fmaf(qs[warp * D + d], ks[lane * (D + 1) + d], s);
-        float mx = vis ? s : -INFINITY;
+        if (k0 + kTreeKeys < k_end) fetch(k0 + kTreeKeys);
+        if (!some) continue;
+        float s[kTreeRun] = {};
+#pragma unroll 8
+        for (int d = 0; d < D; d += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(ks + lane * (D + 4) + d);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const uint32_t any = __ballot_sync(0xffffffffu, vis);
-        if (!any) continue;
-        const float m_new = fmaxf(m, mx), f = exp2f(m - m_new), p = vis ? exp2f(s - m_new) : 0.f;
-        float sum = p;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l = fmaf(l, f, sum);
-        m = m_new;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] *= f;
-        for (int key = 0; key < kTreeKeys; ++key) {
-            const float w = __shfl_sync(0xffffffffu, p, key);
-            if (any >> key & 1u) {      // a row that is not seen may hold anything
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, vs[key * D + lane + 32 * i], acc[i]);
+            for (int x = 0; x < kTreeRun; ++x) {
+                const float4 q = *reinterpret_cast<const float4*>(qs + x * D + d);
+                s[x] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[x]))));
             }
         }
-    }
-    if (r >= a.R) return;
-    if (a.n_splits == 1) {
-        TIO* out = reinterpret_cast<TIO*>(a.out) + io;
-        const float inv = live ? 1.f / l : 0.f;
+        const bool nodes = k0 + kTreeKeys > prefix;
+        uint32_t vis[kTreeRun];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) store_from_float<TIO>(out + lane + 32 * i, live ? acc[i] * inv : 0.f);
-        return;
+        for (int x = 0; x < kTreeRun; ++x) {
+            vis[x] = 0xffffffffu;
+            if (nodes) {
+                const int u = k0 + lane - prefix;       // node of this key, below 0 a cached token
+                const uint32_t s0 = __shfl_sync(0xffffffffu, seen.x, x), s1 = __shfl_sync(0xffffffffu, seen.y, x), s2 = __shfl_sync(0xffffffffu, seen.z, x),
+                               s3 = __shfl_sync(0xffffffffu, seen.w, x);
+                const uint32_t word = u < 64 ? (u < 32 ? s0 : s1) : (u < 96 ? s2 : s3);
+                vis[x] = __ballot_sync(0xffffffffu, k0 + lane < k_end && (u < 0 || (word >> (u & 31) & 1u)));
+            }
+            if (!(vis[x] >> lane & 1u)) s[x] = -INFINITY;
+            float mx = s[x];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float m_new = fmaxf(m[x], mx), off = m_new == -INFINITY ? 0.f : m_new;       // a row that has seen nothing yet
+            const float f = exp2f(m[x] - off), p = vis[x] >> lane & 1u ? exp2f(s[x] - off) : 0.f;
+            l[x] = fmaf(l[x], f, p);
+            m[x] = m_new;
+            ps[x * kTreeKeys + lane] = p;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) acc[x][i] *= f;
+        }
+        __syncwarp();
+#pragma unroll 2
+        for (int k4 = 0; k4 < kTreeKeys; k4 += 4) {
+            float4 w[kTreeRun];
+#pragma unroll
+            for (int x = 0; x < kTreeRun; ++x) w[x] = *reinterpret_cast<const float4*>(ps + x * kTreeKeys + k4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v[D / 32];
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) v[i] = vs[(k4 + e) * D + lane + 32 * i];
+#pragma unroll
+                for (int x = 0; x < kTreeRun; ++x) {
+                    if (nodes && !(vis[x] >> (k4 + e) & 1u)) continue;       // a row that is not seen may hold anything
+                    const float y = e == 0 ? w[x].x : e == 1 ? w[x].y : e == 2 ? w[x].z : w[x].w;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) acc[x][i] = fmaf(y, v[i], acc[x][i]);
+                }
+            }
+        }
+        __syncwarp();
     }
-    const size_t rows = (size_t)a.B * a.Hkv * a.R, row = ((size_t)b * a.Hkv + kvh) * a.R + r;
+    const size_t rows = (size_t)a.B * a.Hkv * a.R;
     float* part = a.part + split * a.part_stride;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) part[row * D + lane + 32 * i] = acc[i];
-    if (lane == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * row) = make_float2(m, l);
+    for (int x = 0; x < kTreeRun; ++x) {
+        float sum = l[x];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (r0 + x >= a.R) continue;
+        if (a.n_splits == 1) {
+            TIO* out = reinterpret_cast<TIO*>(a.out) + io[x];
+            const float inv = live[x] ? 1.f / sum : 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) store_from_float<TIO>(out + lane + 32 * i, live[x] ? acc[x][i] * inv : 0.f);
+            continue;
+        }
+        const size_t row = ((size_t)b * a.Hkv + kvh) * a.R + r0 + x;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) part[row * D + lane + 32 * i] = acc[x][i];
+        if (lane == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * row) = live[x] ? make_float2(m[x], sum) : make_float2(-INFINITY, 0.f);
+    }
 }
 
 // A warp a row: the splits' sums at their common maximum.
@@ -122,25 +208,40 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     pdl_trigger();
     if (row >= rows) return;
     const float* ml = a.part + rows * a.D + 2 * row;
-    float m = -INFINITY;
-    for (int s = lane; s < a.n_splits; s += 32) {
-        const float2 v = *reinterpret_cast<const float2*>(ml + s * stride);
-        if (v.y != 0.f) m = fmaxf(m, v.x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, acc[8];
+    const float* o_at = a.part + row * a.D + lane;
+    float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-    for (int s = 0; s < a.n_splits; ++s) {
-        const float2 v = *reinterpret_cast<const float2*>(ml + s * stride);
-        if (v.y == 0.f) continue;       // saw nothing: its O is not written
-        const float w = exp2f(v.x - m);
-        l = fmaf(w, v.y, l);
-        const float* o = a.part + s * stride + row * a.D;
+    constexpr int AT_ONCE = 8;
+    for (int s0 = 0; s0 < a.n_splits; s0 += AT_ONCE) {
+        float2 v[AT_ONCE];
+        float o[AT_ONCE][8], top = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < a.D) acc[i] = fmaf(w, o[lane + 32 * i], acc[i]);
+        for (int j = 0; j < AT_ONCE; ++j) {
+            v[j] = make_float2(-INFINITY, 0.f);
+            if (s0 + j >= a.n_splits) continue;
+            v[j] = *reinterpret_cast<const float2*>(ml + (s0 + j) * stride);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < a.D) o[j][i] = o_at[(s0 + j) * stride + 32 * i];
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+            if (v[j].y != 0.f) top = fmaxf(top, v[j].x);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - top);
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] *= f;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            if (v[j].y == 0.f) continue;       // saw nothing
+            const float w = exp2f(v[j].x - m);
+            l = fmaf(w, v[j].y, l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < a.D) acc[i] = fmaf(w, o[j][i], acc[i]);
+        }
     }
     const int r = (int)(row % a.R), kvh = (int)(row / a.R % a.Hkv);
     const size_t b = row / a.R / a.Hkv;
@@ -153,14 +254,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
 
 template <typename TIO, typename TC, int D>
 static int launch_rows(grl_device* dev, const TreeArgs& a) {
-    const int smem = (kTreeKeys * (2 * D + 1) + kTreeRows * D) * (int)sizeof(float);
+    const int smem = (kTreeKeys * (2 * D + 4) + kTreeWarps * kTreeRun * (D + kTreeKeys)) * (int)sizeof(float);
     static bool attr_set[64] = {};
     if (!attr_set[dev->ordinal & 63]) {
         GRL_CUDA(cudaFuncSetAttribute(tree_rows_kernel<TIO, TC, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         attr_set[dev->ordinal & 63] = true;
     }
-    dim3 grid(a.n_splits, a.Hkv * ((a.R + kTreeRows - 1) / kTreeRows), a.B);
-    tree_rows_kernel<TIO, TC, D><<<grid, 32 * kTreeRows, smem, dev->stream>>>(a);
+    GRL_CUDA(launch_pdl(tree_rows_kernel<TIO, TC, D>, dim3(a.n_splits, a.Hkv * tree_chunks(a.R), a.B), 32 * kTreeWarps, smem, dev->stream, a));
     GRL_LAUNCHED("tree_rows_kernel");
     return GRL_OK;
 }
@@ -216,7 +316,7 @@ static int check_tree(const grl_tree_params* p) {
         return set_error(GRL_ERR_UNSUPPORTED, "the tensor-core kernel takes bf16 queries over a bf16 cache, head_dim 128 or 64, pages of 64, 32 or 16 tokens");
     GRL_REQUIRE((uintptr_t)kv.k_pages % 16 == 0 && (uintptr_t)kv.v_pages % 16 == 0, "page pools must be 16-byte aligned");
     GRL_REQUIRE((uintptr_t)p->q % 16 == 0 && (uintptr_t)p->out % 16 == 0, "q and out must be 16-byte aligned");
-    const long long chunks = ((long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads) + kTreeRows - 1) / kTreeRows;
+    const long long chunks = ((long long)p->n_tree * (p->num_q_heads / kv.num_kv_heads) + 7) / 8;
     GRL_REQUIRE(chunks * kv.num_kv_heads <= 65535, "too many query heads");
     return GRL_OK;
 }
@@ -248,9 +348,10 @@ static TreePlan tree_plan(grl_device* dev, const grl_tree_params* p) {
         t.workspace = t.t.workspace;
         return t;
     }
-    // some four CTAs an SM, every split at least four tiles
-    const long long ctas = (long long)kv.batch * kv.num_kv_heads * ((R + kTreeRows - 1) / kTreeRows);
-    long long s = 4LL * dev->prop.multiProcessorCount / ctas, most = longest / (4 * kTreeKeys);
+    // Some two CTAs an SM, every split at least two tiles.  us, splits: 5 x 2 x 777 tokens, 33 rows 1: 90, 3: 37, 6: 23.1, 12: 19.3; 1 x 8 x 4000, one row
+    // 4: 114, 16: 34.7, 37: 26.3, 62: 38, 124: 43; 1 x 8 x 16000, 128 rows 4: 613, 8: 465, 9: 415, 16: 475.
+    const long long ctas = (long long)kv.batch * kv.num_kv_heads * tree_chunks(R);
+    long long s = 2LL * dev->prop.multiProcessorCount / ctas, most = longest / (2 * kTreeKeys);
     if (s > most) s = most;
     t.splits = p->n_splits > 0 ? p->n_splits : (int)(s < 1 ? 1 : s > 256 ? 256 : s);
     t.workspace = t.splits == 1 ? 0 : sizeof(float) * t.splits * tree_part_stride((size_t)kv.batch * p->n_tree * p->num_q_heads, kv.head_dim);
