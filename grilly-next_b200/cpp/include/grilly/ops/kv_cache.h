@@ -9,6 +9,7 @@
 #include "grilly/buffer_pool.h"
 #include "grilly/command_batch.h"
 #include "grilly/ops/attention.h"
+#include "grilly/ops/rope.h"
 #include "grilly/pipeline_cache.h"
 
 namespace grilly {
@@ -59,6 +60,7 @@ struct KVCache {
     GrillyBuffer seqLens;             // int32 [B]
     std::vector<int32_t> hostBlockTable;
     std::vector<int32_t> hostSeqLens; // host mirror (lengths advance deterministically)
+    std::vector<int32_t> draftNodes;  // nodes of every sequence in the last draftStep; empty once anything else has changed the lengths
     uint32_t maxPages = 0;            // per sequence
     uint32_t numPages = 0;            // in the pool
     uint32_t nextFreePage = 0;        // bump allocator over the pool (no eviction => no free list churn)
@@ -132,6 +134,21 @@ void gqaAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& k
 void decodeStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, const GrillyBuffer& q,
                       const GrillyBuffer& kNew, const GrillyBuffer& vNew, GrillyBuffer& qRotated, GrillyBuffer& out,
                       uint32_t numQHeads, RopeMode mode, float theta, float scaling, float scale, GrillyBuffer& ws);
+
+// Steps of several drafted tokens, a tree or a chain for each sequence.  No counterpart in the reference; beside decodeStep.
+/// parents: empty for chains, else (B, n), a node's parent among the nodes before it or -1; counts: nodes of each sequence, empty for n each.
+/// q, out (B,n,Hq,D), kNew, vNew (B,n,Hkv,D): device buffers of `dtype`.  Keys and queries are normalised and rotated at cached tokens + depth,
+/// keys and values appended, and every node attends to the cached tokens, its ancestors and itself.  Rows of padding are written as 0.
+/// Asynchronous but for the upload of parents and counts; the buffers in `scratch` are the caller's to release behind the launch.
+void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, const GrillyBuffer& q, const GrillyBuffer& kNew,
+                     const GrillyBuffer& vNew, GrillyBuffer& out, int dtype, uint32_t n, uint32_t numQHeads,
+                     const std::vector<int32_t>& parents, const std::vector<int32_t>& counts, const HeadNorm& norm, const HeadRope& rope,
+                     float scale, std::vector<GrillyBuffer>& scratch);
+/// The attention of the last draftStep's nodes over the cache for queries that are rotated already (another head count, another scale).
+void treeAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& kvCache, const GrillyBuffer& q, GrillyBuffer& out, int dtype,
+                         uint32_t n, uint32_t numQHeads, const std::vector<int32_t>& parents, float scale, std::vector<GrillyBuffer>& scratch);
+/// Keeps the accepted path of the last draftStep, ascending node numbers of each sequence, and drops its other nodes.
+void kvCacheKeep(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, const std::vector<std::vector<int32_t>>& paths);
 
 // Eviction family of the reference (kv_cache.h:186-229) on the paged cache.
 /// attentionScores: nullptr, or host (T, T) probabilities of sequence 0 -- (B, T, T) for a batched cache

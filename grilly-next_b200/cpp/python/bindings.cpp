@@ -811,6 +811,213 @@ PYBIND11_MODULE(grilly_core, m) {
         py::arg("scale") = 0.0f, py::arg("out") = py::none(), py::arg("accumulate_scores") = false,
         "RoPE(q,k) at the current position, append k/v, attend over the cache");
 
+    // ---- normalised heads and steps of several drafted tokens.  Host arrays are uploaded (rounded to bf16 where dtype is "bf16") and come
+    // back as float32; DeviceTensors of one dtype stay on the device and nothing is waited for.
+    struct Operand {
+        TensorPtr t;
+        bool host = false;
+    };
+    const auto operand = [](const ContextPtr& ctx, const py::object& o, const char* name, int dtype) -> Operand {
+        if (py::isinstance<DeviceTensor>(o)) {
+            Operand x{o.cast<TensorPtr>(), false};
+            if (x.t->ctx.get() != ctx.get()) throw std::runtime_error("tensor lives on another Device");
+            if (dtype >= 0 && x.t->dtype != dtype) throw std::runtime_error(std::string(name) + " has another dtype");
+            return x;
+        }
+        FArr a;
+        try {
+            a = o.cast<FArr>();
+        } catch (const py::cast_error&) {
+            throw std::runtime_error(std::string(name) + " must be a float32 array or a DeviceTensor");
+        }
+        Operand x{std::make_shared<DeviceTensor>(ctx, std::vector<py::ssize_t>(a.shape(), a.shape() + a.ndim()), dtype < 0 ? GRL_F32 : dtype), true};
+        const size_t n = x.t->numel();
+        grl_device* dev = ctx->device.handle();
+        if (n == 0) return x;
+        if (x.t->dtype == GRL_F32) {
+            check(grl_memcpy_h2d(dev, x.t->buf.dptr, a.data(), n * 4), name);
+            check(grl_sync(dev, 0), name);          // the source array may go away
+        } else {
+            Pooled tmp(ctx->pool, std::max<size_t>(n * 4, 16));
+            check(grl_memcpy_h2d(dev, tmp.buf.dptr, a.data(), n * 4), name);
+            check(grl_cast(dev, tmp.buf.dptr, GRL_F32, x.t->buf.dptr, GRL_BF16, n), name);
+            check(grl_sync(dev, 0), name);
+        }
+        return x;
+    };
+    const auto result = [](const TensorPtr& t, bool host) -> py::object {
+        if (!host) return py::cast(t);
+        py::array_t<float> out(t->shape);
+        const size_t n = t->numel();
+        grl_device* dev = t->ctx->device.handle();
+        if (t->dtype == GRL_F32) {
+            check(grl_memcpy_d2h(dev, out.mutable_data(), t->buf.dptr, n * 4), "download");
+            check(grl_sync(dev, 0), "download");
+        } else {
+            Pooled tmp(t->ctx->pool, std::max<size_t>(n * 4, 16));
+            check(grl_cast(dev, t->buf.dptr, GRL_BF16, tmp.buf.dptr, GRL_F32, n), "download");
+            check(grl_memcpy_d2h(dev, out.mutable_data(), tmp.buf.dptr, n * 4), "download");
+            check(grl_sync(dev, 0), "download");
+        }
+        return out;
+    };
+    // the dtype of a call: that of its first tensor, or the dtype argument for host arrays
+    const auto dtypeOf = [](const py::object& first, const std::string& dtype) {
+        return py::isinstance<DeviceTensor>(first) ? first.cast<TensorPtr>()->dtype : parseDtype(dtype);
+    };
+    const auto weight = [operand](const ContextPtr& ctx, const py::object& o, const char* name, py::ssize_t D) -> TensorPtr {
+        if (o.is_none()) return nullptr;
+        TensorPtr t = operand(ctx, o, name, GRL_F32).t;
+        if (t->shape.size() != 1 || t->shape[0] != D) throw std::runtime_error(std::string(name) + " must be (head_dim)");
+        return t;
+    };
+    const auto headRope = [](const std::string& mode, uint32_t rotaryDim, float theta, float scaling, float gain) {
+        ops::HeadRope r;
+        r.mode = theta != 0.0f ? parseRopeMode(mode, false) : ops::RopeMode::None;
+        r.rotaryDim = rotaryDim; r.theta = theta != 0.0f ? theta : 10000.0f; r.scaling = scaling; r.gain = gain;
+        return r;
+    };
+    const auto bufferOf = [](const TensorPtr& t) { return t ? t->buf : GrillyBuffer{}; };
+    const auto headShape = [](const TensorPtr& q, const TensorPtr& k) {
+        if (q->shape.size() != 4) throw std::runtime_error("q must be 4D (batch, seq_len, heads, head_dim)");
+        if (k && (k->shape.size() != 4 || k->shape[0] != q->shape[0] || k->shape[1] != q->shape[1] || k->shape[3] != q->shape[3]))
+            throw std::runtime_error("k must be (batch, seq_len, kv_heads, head_dim)");
+        return ops::HeadShape{uint32_t(q->shape[0]), uint32_t(q->shape[1]), uint32_t(q->shape[2]), k ? uint32_t(k->shape[2]) : 0, uint32_t(q->shape[3])};
+    };
+    const auto positionsOf = [](const ContextPtr& ctx, const std::optional<IArr>& positions, const ops::HeadShape& s, GrillyBuffer& buf) {
+        if (!positions) return;
+        if (positions->ndim() != 2 || positions->shape(0) != s.batch || positions->shape(1) != s.seqLen)
+            throw std::runtime_error("positions must be (batch, seq_len)");
+        const size_t bytes = size_t(s.batch) * s.seqLen * 4;
+        buf = ctx->pool.acquire(std::max<size_t>(bytes, 16));
+        check(grl_memcpy_h2d(ctx->device.handle(), buf.dptr, positions->data(), bytes), "positions");
+        check(grl_sync(ctx->device.handle(), 0), "positions");
+    };
+    struct Released {           // buffers that go back to the pool on every way out; stream order protects them
+        BufferPool& pool;
+        std::vector<GrillyBuffer> bufs;
+        ~Released() { for (auto& b : bufs) pool.release(b); }
+    };
+
+    m.def(
+        "qk_norm_rope",
+        [=](ContextPtr ctx, py::object qIn, py::object kIn, py::object qWeight, py::object kWeight, float eps, float ropeTheta, float ropeScaling,
+            const std::string& ropeMode, uint32_t rotaryDim, float ropeGain, std::optional<IArr> positions, int32_t posBase,
+            const std::string& dtype) -> py::object {
+            const int dt = dtypeOf(qIn, dtype);
+            const Operand q = operand(ctx, qIn, "q", dt), k = kIn.is_none() ? Operand{} : operand(ctx, kIn, "k", dt);
+            const ops::HeadShape s = headShape(q.t, k.t);
+            const TensorPtr qw = weight(ctx, qWeight, "q_weight", s.headDim), kw = weight(ctx, kWeight, "k_weight", s.headDim);
+            auto qo = std::make_shared<DeviceTensor>(ctx, q.t->shape, dt);
+            auto ko = k.t ? std::make_shared<DeviceTensor>(ctx, k.t->shape, dt) : nullptr;
+            Released tmp{ctx->pool, std::vector<GrillyBuffer>(1)};
+            positionsOf(ctx, positions, s, tmp.bufs[0]);
+            GrillyBuffer koBuf = bufferOf(ko);
+            ops::qkNormRopeDevice(ctx->pool, ctx->cache, q.t->buf, bufferOf(k.t), qo->buf, koBuf, dt, s, {bufferOf(qw), bufferOf(kw), eps},
+                                  headRope(ropeMode, rotaryDim, ropeTheta, ropeScaling, ropeGain), tmp.bufs[0], posBase);
+            if (!ko) return result(qo, q.host);
+            return py::make_tuple(result(qo, q.host), result(ko, k.host));
+        },
+        py::arg("device"), py::arg("q"), py::arg("k") = py::none(), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(),
+        py::arg("eps") = 1e-6f, py::arg("rope_theta") = 10000.0f, py::arg("rope_scaling") = 1.0f, py::arg("rope_mode") = "interleaved",
+        py::arg("rotary_dim") = 0, py::arg("rope_gain") = 1.0f, py::arg("positions") = py::none(), py::arg("pos_base") = 0, py::arg("dtype") = "fp32",
+        "Normalise every (batch, seq_len, heads, head_dim) head of q (and k) by its root mean square, scale by the weights and rotate");
+
+    m.def(
+        "qk_norm_rope_backward",
+        [=](ContextPtr ctx, py::object gradQ, py::object gradK, py::object qIn, py::object kIn, py::object qWeight, py::object kWeight, float eps,
+            float ropeTheta, float ropeScaling, const std::string& ropeMode, uint32_t rotaryDim, float ropeGain, std::optional<IArr> positions,
+            int32_t posBase, const std::string& dtype) {
+            if (gradK.is_none() != kIn.is_none()) throw std::runtime_error("grad_k and k go together");
+            const int dt = dtypeOf(qIn, dtype);
+            const Operand q = operand(ctx, qIn, "q", dt), gq = operand(ctx, gradQ, "grad_q", dt);
+            const Operand k = kIn.is_none() ? Operand{} : operand(ctx, kIn, "k", dt), gk = kIn.is_none() ? Operand{} : operand(ctx, gradK, "grad_k", dt);
+            const ops::HeadShape s = headShape(q.t, k.t);
+            if (gq.t->shape != q.t->shape || (k.t && gk.t->shape != k.t->shape)) throw std::runtime_error("a gradient differs from its input in shape");
+            const TensorPtr qw = weight(ctx, qWeight, "q_weight", s.headDim), kw = weight(ctx, kWeight, "k_weight", s.headDim);
+            const auto make = [&](const std::vector<py::ssize_t>& shape, int t) { return std::make_shared<DeviceTensor>(ctx, shape, t); };
+            const TensorPtr dq = make(q.t->shape, dt), dk = k.t ? make(k.t->shape, dt) : nullptr;
+            const TensorPtr dqw = qw ? make(qw->shape, GRL_F32) : nullptr, dkw = kw && k.t ? make(kw->shape, GRL_F32) : nullptr;
+            Released tmp{ctx->pool, std::vector<GrillyBuffer>(2)};
+            positionsOf(ctx, positions, s, tmp.bufs[0]);
+            GrillyBuffer dkBuf = bufferOf(dk), dqwBuf = bufferOf(dqw), dkwBuf = bufferOf(dkw);
+            ops::qkNormRopeBackwardDevice(ctx->pool, ctx->cache, gq.t->buf, bufferOf(gk.t), q.t->buf, bufferOf(k.t), dq->buf, dkBuf, dqwBuf, dkwBuf, dt, s,
+                                          {bufferOf(qw), bufferOf(kw), eps}, headRope(ropeMode, rotaryDim, ropeTheta, ropeScaling, ropeGain),
+                                          tmp.bufs[0], posBase, tmp.bufs[1]);
+            py::dict d;
+            d["grad_q"] = result(dq, q.host);
+            if (dk) d["grad_k"] = result(dk, k.host);
+            if (dqw) d["grad_q_weight"] = result(dqw, q.host);
+            if (dkw) d["grad_k_weight"] = result(dkw, q.host);
+            return d;
+        },
+        py::arg("device"), py::arg("grad_q"), py::arg("grad_k"), py::arg("q"), py::arg("k"), py::arg("q_weight") = py::none(),
+        py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6f, py::arg("rope_theta") = 10000.0f, py::arg("rope_scaling") = 1.0f,
+        py::arg("rope_mode") = "interleaved", py::arg("rotary_dim") = 0, py::arg("rope_gain") = 1.0f, py::arg("positions") = py::none(),
+        py::arg("pos_base") = 0, py::arg("dtype") = "fp32",
+        "Gradients of qk_norm_rope: {grad_q, grad_k, grad_q_weight, grad_k_weight}, those of weights that were given");
+
+    const auto intsOf = [](const std::optional<IArr>& a, const char* name, py::ssize_t rows, py::ssize_t cols) {
+        std::vector<int32_t> v;
+        if (!a) return v;
+        if (cols ? a->ndim() != 2 || a->shape(0) != rows || a->shape(1) != cols : a->ndim() != 1 || a->shape(0) != rows)
+            throw std::runtime_error(std::string(name) + (cols ? " must be (batch, n)" : " must be (batch)"));
+        v.assign(a->data(), a->data() + a->size());
+        return v;
+    };
+    const auto checkStep = [](const ops::KVCache& kv, const TensorPtr& t, const char* name, py::ssize_t n, py::ssize_t heads) {
+        if (t->shape.size() != 4 || t->shape[0] != kv.config.batchSize || (n && t->shape[1] != n) || (heads && t->shape[2] != heads) ||
+            t->shape[3] != kv.config.headDim)
+            throw std::runtime_error(std::string(name) + " must be (batch, n, heads, head_dim) of the cache");
+    };
+
+    m.def(
+        "draft_step",
+        [=](ContextPtr ctx, ops::KVCache& kv, py::object qIn, py::object kIn, py::object vIn, std::optional<IArr> parents, std::optional<IArr> nNodes,
+            py::object qWeight, py::object kWeight, float eps, float ropeTheta, float ropeScaling, const std::string& ropeMode, uint32_t rotaryDim,
+            float ropeGain, float scale, const std::string& dtype) -> py::object {
+            const auto& c = kv.config;
+            const int dt = dtypeOf(qIn, dtype);
+            const Operand q = operand(ctx, qIn, "q", dt), k = operand(ctx, kIn, "k_new", dt), v = operand(ctx, vIn, "v_new", dt);
+            checkStep(kv, q.t, "q", 0, 0);
+            const py::ssize_t n = q.t->shape[1];
+            checkStep(kv, k.t, "k_new", n, c.numHeads);
+            checkStep(kv, v.t, "v_new", n, c.numHeads);
+            const TensorPtr qw = weight(ctx, qWeight, "q_weight", c.headDim), kw = weight(ctx, kWeight, "k_weight", c.headDim);
+            auto out = std::make_shared<DeviceTensor>(ctx, q.t->shape, dt);
+            Released tmp{ctx->pool, {}};
+            ops::draftStepDevice(ctx->pool, ctx->cache, kv, q.t->buf, k.t->buf, v.t->buf, out->buf, dt, uint32_t(n), uint32_t(q.t->shape[2]),
+                                 intsOf(parents, "parents", c.batchSize, n), intsOf(nNodes, "n_nodes", c.batchSize, 0), {bufferOf(qw), bufferOf(kw), eps},
+                                 headRope(ropeMode, rotaryDim, ropeTheta, ropeScaling, ropeGain), scale, tmp.bufs);
+            return result(out, q.host);
+        },
+        py::arg("device"), py::arg("kv_cache"), py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("parents") = py::none(),
+        py::arg("n_nodes") = py::none(), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6f,
+        py::arg("rope_theta") = 10000.0f, py::arg("rope_scaling") = 1.0f, py::arg("rope_mode") = "interleaved", py::arg("rotary_dim") = 0,
+        py::arg("rope_gain") = 1.0f, py::arg("scale") = 0.0f, py::arg("dtype") = "fp32",
+        "A step of several drafted tokens: normalise and rotate q and k at the nodes' depths, append k/v, attend to the cache and the ancestors");
+
+    m.def(
+        "tree_attention",
+        [=](ContextPtr ctx, py::object qIn, ops::KVCache& kv, std::optional<IArr> parents, float scale, const std::string& dtype) -> py::object {
+            const int dt = dtypeOf(qIn, dtype);
+            const Operand q = operand(ctx, qIn, "q", dt);
+            checkStep(kv, q.t, "q", 0, 0);
+            auto out = std::make_shared<DeviceTensor>(ctx, q.t->shape, dt);
+            Released tmp{ctx->pool, {}};
+            ops::treeAttentionDevice(ctx->pool, ctx->cache, kv, q.t->buf, out->buf, dt, uint32_t(q.t->shape[1]), uint32_t(q.t->shape[2]),
+                                     intsOf(parents, "parents", kv.config.batchSize, q.t->shape[1]), scale, tmp.bufs);
+            return result(out, q.host);
+        },
+        py::arg("device"), py::arg("q"), py::arg("kv_cache"), py::arg("parents") = py::none(), py::arg("scale") = 0.0f, py::arg("dtype") = "fp32",
+        "Attention of rotated queries of the last draft_step's nodes over the cache");
+
+    m.def(
+        "kv_cache_keep",
+        [](ContextPtr ctx, ops::KVCache& kv, const std::vector<std::vector<int32_t>>& paths) { ops::kvCacheKeep(ctx->pool, ctx->cache, kv, paths); },
+        py::arg("device"), py::arg("kv_cache"), py::arg("paths"),
+        "Keep the accepted nodes of the last draft_step (ascending node numbers of each sequence) and drop the others");
+
     // ---- KV-sharded decode across processes (one per GPU): NCCL behind the C ABI
     struct PyShardGroup {
         ContextPtr ctx;

@@ -383,6 +383,52 @@ void rope(CommandBatch& batch, BufferPool& pool, PipelineCache& cache, const flo
     batch.submit();
 }
 
+static grl_qk_norm_params normParams(const GrillyBuffer& q, const GrillyBuffer& k, int dtype, const HeadShape& h, const HeadNorm& norm,
+                                     const HeadRope& rope, const GrillyBuffer& positions, int32_t posBase) {
+    const size_t elem = dtype == GRL_BF16 ? 2 : 4, rows = size_t(h.batch) * h.seqLen;
+    if (!q.valid()) throw std::runtime_error("qkNormRope: null tensor");
+    if (q.size < rows * h.numQHeads * h.headDim * elem || (k.valid() && k.size < rows * h.numKvHeads * h.headDim * elem))
+        throw std::runtime_error("qkNormRope: buffer too small");
+    grl_qk_norm_params p{};
+    p.q = q.dptr; p.k = k.valid() ? k.dptr : nullptr;
+    p.q_weight = static_cast<const float*>(norm.qWeight.dptr); p.k_weight = static_cast<const float*>(norm.kWeight.dptr);
+    p.in_dtype = p.out_dtype = dtype;
+    p.batch = int(h.batch); p.seq_len = int(h.seqLen); p.num_q_heads = int(h.numQHeads); p.num_kv_heads = k.valid() ? int(h.numKvHeads) : 0;
+    p.head_dim = int(h.headDim); p.eps = norm.eps; p.rope = rope.spec();
+    p.positions = static_cast<const int32_t*>(positions.dptr); p.pos_base = posBase;
+    return p;
+}
+
+void qkNormRopeDevice(BufferPool& pool, PipelineCache& cache, const GrillyBuffer& q, const GrillyBuffer& k, GrillyBuffer& qOut,
+                      GrillyBuffer& kOut, int dtype, const HeadShape& shape, const HeadNorm& norm, const HeadRope& rope,
+                      const GrillyBuffer& positions, int32_t posBase) {
+    grl_qk_norm_params p = normParams(q, k, dtype, shape, norm, rope, positions, posBase);
+    if (qOut.size < q.size || (k.valid() && kOut.size < k.size)) throw std::runtime_error("qkNormRope: result buffer too small");
+    cache.getOrCreate("qk-norm-rope/" + std::to_string(shape.headDim));
+    p.q_out = qOut.dptr; p.k_out = k.valid() ? kOut.dptr : nullptr;
+    check(grl_qk_norm_rope(pool.device().handle(), &p), "qkNormRope");
+}
+
+void qkNormRopeBackwardDevice(BufferPool& pool, PipelineCache& cache, const GrillyBuffer& qOutGrad, const GrillyBuffer& kOutGrad,
+                              const GrillyBuffer& q, const GrillyBuffer& k, GrillyBuffer& qGrad, GrillyBuffer& kGrad,
+                              GrillyBuffer& qWeightGrad, GrillyBuffer& kWeightGrad, int dtype, const HeadShape& shape,
+                              const HeadNorm& norm, const HeadRope& rope, const GrillyBuffer& positions, int32_t posBase, GrillyBuffer& ws) {
+    grl_qk_norm_grad_params p{};
+    p.fwd = normParams(q, k, dtype, shape, norm, rope, positions, posBase);
+    if (qOutGrad.size < q.size || qGrad.size < q.size || (k.valid() && (kOutGrad.size < k.size || kGrad.size < k.size)))
+        throw std::runtime_error("qkNormRopeBackward: buffer too small");
+    cache.getOrCreate("qk-norm-rope-backward/" + std::to_string(shape.headDim));
+    p.q_out_grad = qOutGrad.dptr; p.q_grad = qGrad.dptr;
+    p.k_out_grad = k.valid() ? kOutGrad.dptr : nullptr; p.k_grad = k.valid() ? kGrad.dptr : nullptr;
+    p.q_weight_grad = static_cast<float*>(qWeightGrad.dptr);
+    p.k_weight_grad = k.valid() ? static_cast<float*>(kWeightGrad.dptr) : nullptr;
+    grl_device* dev = pool.device().handle();
+    check(grl_qk_norm_rope_backward_workspace_bytes(dev, &p, &p.workspace_bytes), "qkNormRopeBackward");
+    if (p.workspace_bytes) ws = pool.acquire(p.workspace_bytes);
+    p.workspace = ws.dptr;
+    check(grl_qk_norm_rope_backward(dev, &p), "qkNormRopeBackward");
+}
+
 void attentionMask(CommandBatch& batch, BufferPool& pool, PipelineCache& cache, float* scores, const float* keyMask,
                    uint32_t B, uint32_t H, uint32_t S, bool causal, float maskValue) {
     if (!scores) throw std::runtime_error("attentionMask: null scores");

@@ -21,12 +21,12 @@ struct Recording {
     }
 };
 
-// Give every sequence pages for `extra` more tokens; uploads the block table when it changed.
-void reservePages(BufferPool& pool, KVCache& kv, uint32_t extra) {
+// Give every sequence pages for `extra` (or its own count) more tokens; uploads the block table when it changed.
+void reservePages(BufferPool& pool, KVCache& kv, uint32_t extra, const std::vector<int32_t>& counts = {}) {
     const auto& c = kv.config;
     bool changed = false;
     for (uint32_t b = 0; b < c.batchSize; ++b) {
-        const uint32_t need = (uint32_t(kv.hostSeqLens[b]) + extra + c.pageTokens - 1) / c.pageTokens;
+        const uint32_t need = (uint32_t(kv.hostSeqLens[b]) + (counts.empty() ? extra : uint32_t(counts[b])) + c.pageTokens - 1) / c.pageTokens;
         if (need > kv.maxPages)
             throw std::runtime_error("kvCacheAppend: sequence would exceed max_cache_tokens (" +
                                      std::to_string(c.maxCacheTokens) + ")");
@@ -172,6 +172,7 @@ void destroyKVCache(BufferPool& pool, KVCache& kv) {
     pool.release(kv.evicted);
     kv.hostBlockTable.clear();
     kv.hostSeqLens.clear();
+    kv.draftNodes.clear();
     kv.currentLen = 0;
     kv.nextFreePage = 0;
 }
@@ -251,6 +252,7 @@ void kvCacheAppendRope(CommandBatch& batch, BufferPool& pool, PipelineCache& cac
         throw;
     }
     pool.release(kb); pool.release(vb); pool.release(qb); pool.release(qo);
+    kv.draftNodes.clear();
     for (auto& l : kv.hostSeqLens) l += int32_t(n);
     kv.currentLen = uint32_t(kv.hostSeqLens[0]);
     kv.totalAppended += uint64_t(n) * c.batchSize;
@@ -448,6 +450,7 @@ void decodeStep(CommandBatch& batch, BufferPool& pool, PipelineCache& cache, KVC
         ap.pos_base = 0; ap.update_lens = 1;
         ap.pos_offsets = static_cast<const int32_t*>(kv.evicted.dptr);
         check(grl_kv_append(dev, &ap), "decodeStep: append");
+        kv.draftNodes.clear();
         for (auto& l : kv.hostSeqLens) l += 1;
         kv.currentLen = uint32_t(kv.hostSeqLens[0]);
         kv.totalAppended += c.batchSize;
@@ -502,10 +505,150 @@ void decodeStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kv, const
     ap.pos_base = 0; ap.update_lens = 1;
     ap.pos_offsets = static_cast<const int32_t*>(kv.evicted.dptr);
     check(grl_kv_append(dev, &ap), "decodeStep: append");
+    kv.draftNodes.clear();
     for (auto& l : kv.hostSeqLens) l += 1;
     kv.currentLen = uint32_t(kv.hostSeqLens[0]);
     kv.totalAppended += c.batchSize;
     launchDecode(dev, pool, kv, static_cast<const float*>(qRotated.dptr), static_cast<float*>(out.dptr), numQHeads, scale, 0, ws);
+}
+
+namespace {
+// Device copies of small host arrays; waits, since the arrays may go away.
+const int32_t* uploadInts(BufferPool& pool, const std::vector<int32_t>& v, std::vector<GrillyBuffer>& scratch) {
+    if (v.empty()) return nullptr;
+    scratch.push_back(pool.acquire(v.size() * 4));
+    check(grl_memcpy_h2d(pool.device().handle(), scratch.back().dptr, v.data(), v.size() * 4), "upload");
+    check(grl_sync(pool.device().handle(), 0), "upload");
+    return static_cast<const int32_t*>(scratch.back().dptr);
+}
+
+void checkDrafted(const char* op, const KVCache& kv, uint32_t n, uint32_t numQHeads, const std::vector<int32_t>& parents,
+                  const std::vector<int32_t>& counts) {
+    const std::string who(op);
+    const auto& c = kv.config;
+    if (!kv.kPages.valid()) throw std::runtime_error(who + ": cache was destroyed");
+    if (kv.mla()) throw std::runtime_error(who + ": not built for the MLA latent cache (use compression_ratio=1)");
+    if (c.dtype == GRL_FP8_INT4) throw std::runtime_error(who + ": not built for the quantised cache");
+    if (numQHeads == 0 || numQHeads % c.numHeads != 0)
+        throw std::runtime_error(who + ": num_q_heads must be a positive multiple of num_kv_heads");
+    if (n == 0 || n > GRL_MAX_TREE) throw std::runtime_error(who + ": a step has 1 to " + std::to_string(GRL_MAX_TREE) + " nodes");
+    if (!counts.empty() && counts.size() != c.batchSize) throw std::runtime_error(who + ": n_nodes must be (batch)");
+    if (!parents.empty() && parents.size() != size_t(c.batchSize) * n) throw std::runtime_error(who + ": parents must be (batch, n)");
+    for (uint32_t b = 0; b < c.batchSize; ++b) {
+        const int32_t m = counts.empty() ? int32_t(n) : counts[b];
+        if (m < 0 || m > int32_t(n)) throw std::runtime_error(who + ": n_nodes out of range");
+        for (int32_t t = 0; t < m && !parents.empty(); ++t) {
+            const int32_t p = parents[size_t(b) * n + t];
+            if (p < -1 || p >= t) throw std::runtime_error(who + ": a parent must be an earlier node or -1");
+        }
+    }
+}
+
+void launchTree(BufferPool& pool, const KVCache& kv, const void* q, void* out, int dtype, uint32_t n, uint32_t numQHeads, const int32_t* parents,
+                const int32_t* counts, float scale, std::vector<GrillyBuffer>& scratch) {
+    grl_tree_params p{};
+    p.kv = kv.layout();
+    p.q = q; p.out = out; p.io_dtype = dtype; p.num_q_heads = int(numQHeads); p.n_tree = int(n);
+    p.scale = scale; p.parents = parents; p.n_nodes = counts;
+    p.max_seq_len = *std::max_element(kv.hostSeqLens.begin(), kv.hostSeqLens.end());
+    check(grl_tree_workspace_bytes(pool.device().handle(), &p, &p.workspace_bytes), "treeAttention");
+    if (p.workspace_bytes) {
+        scratch.push_back(pool.acquire(p.workspace_bytes));
+        p.workspace = scratch.back().dptr;
+    }
+    check(grl_tree_attention(pool.device().handle(), &p), "treeAttention");
+}
+}  // namespace
+
+void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kv, const GrillyBuffer& q, const GrillyBuffer& kNew,
+                     const GrillyBuffer& vNew, GrillyBuffer& out, int dtype, uint32_t n, uint32_t numQHeads,
+                     const std::vector<int32_t>& parents, const std::vector<int32_t>& counts, const HeadNorm& norm, const HeadRope& rope,
+                     float scale, std::vector<GrillyBuffer>& scratch) {
+    checkDrafted("draftStep", kv, n, numQHeads, parents, counts);
+    const auto& c = kv.config;
+    const size_t qBytes = size_t(c.batchSize) * n * numQHeads * c.headDim * elemSize(dtype), kBytes = qBytes / numQHeads * c.numHeads;
+    if (q.size < qBytes || out.size < qBytes || kNew.size < kBytes || vNew.size < kBytes) throw std::runtime_error("draftStep: buffer too small");
+    cache.getOrCreate("draft-step/" + std::to_string(c.headDim));
+    reservePages(pool, kv, n, counts);
+    grl_append_norm_params a{};
+    a.kv = kv.layout();
+    a.parents = uploadInts(pool, parents, scratch);
+    a.n_nodes = uploadInts(pool, counts, scratch);
+    scratch.push_back(pool.acquire(qBytes));
+    const GrillyBuffer rotated = scratch.back();
+    a.k_new = kNew.dptr; a.v_new = vNew.dptr; a.q_in = q.dptr; a.q_out = rotated.dptr;
+    a.q_weight = static_cast<const float*>(norm.qWeight.dptr); a.k_weight = static_cast<const float*>(norm.kWeight.dptr);
+    a.eps = norm.eps; a.in_dtype = a.q_out_dtype = dtype;
+    a.n_new = int(n); a.num_q_heads = int(numQHeads); a.rope = rope.spec(); a.update_lens = 1;
+    a.pos_offsets = static_cast<const int32_t*>(kv.evicted.dptr);
+    check(grl_kv_append_norm(pool.device().handle(), &a), "draftStep: append");
+    kv.draftNodes = counts.empty() ? std::vector<int32_t>(c.batchSize, int32_t(n)) : counts;
+    for (uint32_t b = 0; b < c.batchSize; ++b) {
+        kv.hostSeqLens[b] += kv.draftNodes[b];
+        kv.totalAppended += uint64_t(kv.draftNodes[b]);
+    }
+    kv.currentLen = uint32_t(kv.hostSeqLens[0]);
+    launchTree(pool, kv, rotated.dptr, out.dptr, dtype, n, numQHeads, a.parents, a.n_nodes, scale, scratch);
+}
+
+void treeAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& kv, const GrillyBuffer& q, GrillyBuffer& out, int dtype,
+                         uint32_t n, uint32_t numQHeads, const std::vector<int32_t>& parents, float scale, std::vector<GrillyBuffer>& scratch) {
+    if (kv.kPages.valid() && kv.draftNodes.empty())
+        throw std::runtime_error("treeAttention: the cache does not end with the nodes of a draft step");
+    checkDrafted("treeAttention", kv, n, numQHeads, parents, kv.draftNodes);
+    const auto& c = kv.config;
+    const size_t bytes = size_t(c.batchSize) * n * numQHeads * c.headDim * elemSize(dtype);
+    if (q.size < bytes || out.size < bytes) throw std::runtime_error("treeAttention: buffer too small");
+    cache.getOrCreate("tree-attention/" + std::to_string(c.headDim));
+    const int32_t* up = uploadInts(pool, parents, scratch);
+    launchTree(pool, kv, q.dptr, out.dptr, dtype, n, numQHeads, up, uploadInts(pool, kv.draftNodes, scratch), scale, scratch);
+}
+
+void kvCacheKeep(BufferPool& pool, PipelineCache& cache, KVCache& kv, const std::vector<std::vector<int32_t>>& paths) {
+    if (!kv.kPages.valid()) throw std::runtime_error("kvCacheKeep: cache was destroyed");
+    if (kv.draftNodes.empty())
+        throw std::runtime_error("kvCacheKeep: the cache does not end with the nodes of a draft step");
+    const size_t B = kv.config.batchSize;
+    if (paths.size() != B) throw std::runtime_error("kvCacheKeep: one path a sequence");
+    size_t longest = 1;
+    for (size_t b = 0; b < B; ++b) {
+        int32_t last = -1;
+        for (const int32_t t : paths[b]) {
+            if (t <= last || t >= kv.draftNodes[b]) throw std::runtime_error("kvCacheKeep: a path is ascending node numbers of the last draft step");
+            last = t;
+        }
+        longest = std::max(longest, paths[b].size());
+    }
+    cache.getOrCreate("kv-keep/" + std::to_string(kv.config.headDim));
+    std::vector<int32_t> ints(B * (longest + 2), 0);         // paths, their lengths, the nodes
+    for (size_t b = 0; b < B; ++b) {
+        std::copy(paths[b].begin(), paths[b].end(), ints.begin() + b * longest);
+        ints[B * longest + b] = int32_t(paths[b].size());
+        ints[B * (longest + 1) + b] = kv.draftNodes[b];
+    }
+    std::vector<GrillyBuffer> scratch;
+    try {
+        const int32_t* d = uploadInts(pool, ints, scratch);
+        const grl_kv_meta meta = kv.meta();
+        grl_commit_params p{};
+        p.kv = kv.layout();
+        p.path = d; p.n_path = d + B * longest; p.n_nodes = d + B * (longest + 1);
+        p.max_path = int(longest);
+        p.n_tree = GRL_MAX_TREE;
+        p.meta = &meta;
+        check(grl_kv_commit(pool.device().handle(), &p), "kvCacheKeep");
+    } catch (...) {
+        for (auto& s : scratch) pool.release(s);
+        throw;
+    }
+    for (auto& s : scratch) pool.release(s);
+    for (size_t b = 0; b < B; ++b) {
+        const int32_t dropped = kv.draftNodes[b] - int32_t(paths[b].size());
+        kv.hostSeqLens[b] -= dropped;
+        kv.totalAppended -= uint64_t(dropped);
+    }
+    kv.draftNodes.clear();
+    kv.currentLen = uint32_t(kv.hostSeqLens[0]);
 }
 
 void kvCacheEvictH2O(CommandBatch& batch, BufferPool& pool, PipelineCache& cache, KVCache& kv,
@@ -672,6 +815,7 @@ void kvCacheCompact(CommandBatch& batch, BufferPool& pool, PipelineCache& cache,
         throw;
     }
     pool.release(scratch);
+    kv.draftNodes.clear();
     for (size_t b = 0; b < lens.size(); ++b) {
         kv.totalEvicted += uint64_t(kv.hostSeqLens[b] - lens[b]);
         kv.hostSeqLens[b] = lens[b];

@@ -84,6 +84,27 @@ def decode_step(device, kv_cache, q, k_new, v_new, **kwargs):
     return _core.decode_step(device, kv_cache, q, k_new, v_new, **kwargs)
 
 
+# ---- normalised heads, steps of several drafted tokens
+def qk_norm_rope(device, q, k=None, q_weight=None, k_weight=None, **kwargs):
+    return _core.qk_norm_rope(device, q, k, q_weight, k_weight, **kwargs)
+
+
+def qk_norm_rope_backward(device, grad_q, grad_k, q, k, q_weight=None, k_weight=None, **kwargs):
+    return _core.qk_norm_rope_backward(device, grad_q, grad_k, q, k, q_weight, k_weight, **kwargs)
+
+
+def draft_step(device, kv_cache, q, k_new, v_new, parents=None, n_nodes=None, **kwargs):
+    return _core.draft_step(device, kv_cache, q, k_new, v_new, parents, n_nodes, **kwargs)
+
+
+def tree_attention(device, q, kv_cache, parents=None, **kwargs):
+    return _core.tree_attention(device, q, kv_cache, parents, **kwargs)
+
+
+def kv_cache_keep(device, kv_cache, paths):
+    return _core.kv_cache_keep(device, kv_cache, paths)
+
+
 KVCache = getattr(_core, "KVCache", None)
 Device = getattr(_core, "Device", None)
 

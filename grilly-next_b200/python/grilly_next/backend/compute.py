@@ -68,6 +68,22 @@ class VulkanCompute:
         return _bridge.decode_step(self._device, kv_cache, q, k_new, v_new, **kwargs)
 
 
+    # ---- normalised heads, steps of several drafted tokens
+    def qk_norm_rope(self, q, k=None, q_weight=None, k_weight=None, **kwargs):
+        return _bridge.qk_norm_rope(self._device, q, k, q_weight, k_weight, **kwargs)
+
+    def qk_norm_rope_backward(self, grad_q, grad_k, q, k, q_weight=None, k_weight=None, **kwargs):
+        return _bridge.qk_norm_rope_backward(self._device, grad_q, grad_k, q, k, q_weight, k_weight, **kwargs)
+
+    def draft_step(self, kv_cache, q, k_new, v_new, parents=None, n_nodes=None, **kwargs):
+        return _bridge.draft_step(self._device, kv_cache, q, k_new, v_new, parents, n_nodes, **kwargs)
+
+    def tree_attention(self, q, kv_cache, parents=None, **kwargs):
+        return _bridge.tree_attention(self._device, q, kv_cache, parents, **kwargs)
+
+    def kv_cache_keep(self, kv_cache, paths):
+        return _bridge.kv_cache_keep(self._device, kv_cache, paths)
+
     # ---- the projections on either side of attention
     def linear(self, x, weight, bias=None, **kwargs):
         return _bridge.linear(self._device, x, weight, bias, **kwargs)

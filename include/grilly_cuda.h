@@ -333,8 +333,8 @@ int grl_qk_norm_rope_backward(grl_device* dev, const grl_qk_norm_grad_params* p)
  *   grl_tree_attention   a node attends to the cached tokens, its ancestors and itself
  *   grl_kv_commit        the rows of the accepted path close up behind the cached tokens, the others are dropped
  * A sequence whose numbers do not fit (a parent that is no earlier node, more nodes than n_new, a length past the block table, a page
- * outside the pool, a path that does not ascend) is left as it is (attention: its rows are written as 0) and the next
- * grl_sync returns GRL_ERR_KERNEL.  bf16 and float32 caches; GRL_FP8_INT4 is refused (GRL_ERR_UNSUPPORTED). */
+ * outside the pool, a path that does not ascend) is left as it is (attention: its rows are written as 0; with a page outside the pool
+ * they mean nothing) and the next grl_sync returns GRL_ERR_KERNEL.  bf16 and float32 caches; GRL_FP8_INT4 is refused (GRL_ERR_UNSUPPORTED). */
 #define GRL_MAX_TREE 128
 /* k_new, v_new (B,n_new,Hkv,D), q_in, q_out (B,n_new,Hq,D); the token strides (elements, 0 is read as H*D; of a sequence n_new
  * times that) let the parts of one packed projection be read in place; q_out is contiguous.  Rows of q_out past a sequence's nodes

@@ -223,3 +223,11 @@ def test_oracle_trees():
     assert [list(np.flatnonzero(row)) for row in s] == [[0], [0, 1], [0, 2], [0, 1, 3], [4], [0, 1, 3, 5]]
     assert list(orc.depths(parents, 6)) == [0, 1, 1, 2, 0, 3]
     assert np.array_equal(orc.ancestors(None, 4), np.tril(np.ones((4, 4), bool)))
+
+
+def test_python_operators_are_there():
+    import grilly_core
+    import grilly_next
+    from grilly_next.backend import _bridge
+    for n in ("qk_norm_rope", "qk_norm_rope_backward", "draft_step", "tree_attention", "kv_cache_keep"):
+        assert hasattr(grilly_core, n) and hasattr(_bridge, n) and hasattr(grilly_next.Compute, n)
