@@ -157,9 +157,10 @@ struct RowTables {
     float w[2][256];
 };
 __device__ __forceinline__ void row_tables(RowTables& t, const RopeArgs& r, int D, const float* w0, const float* w1) {
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
-        t.w[0][i] = w0 ? __ldg(w0 + i) : 1.f;
-        t.w[1][i] = w1 ? __ldg(w1 + i) : 1.f;
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) {
+        // zeros behind the row: threads without elements take part in its sums
+        t.w[0][i] = i >= D ? 0.f : w0 ? __ldg(w0 + i) : 1.f;
+        t.w[1][i] = i >= D ? 0.f : w1 ? __ldg(w1 + i) : 1.f;
         if (2 * i < r.rd) t.turns[i] = (r.inv_freq ? (double)__ldg(r.inv_freq + i) : r.freq.inv_freq[i]) * 0.31830988618379067;     // 1 / pi
     }
 }

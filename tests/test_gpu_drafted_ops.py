@@ -182,3 +182,20 @@ def test_refusals(gpu):
         gpu.qk_norm_rope(q, positions=np.zeros((2, 5), np.int32))
     with pytest.raises(RuntimeError, match="go together"):
         gpu.qk_norm_rope_backward(q, None, q, k)
+
+
+@pytest.mark.parametrize("mode,rotary", [("interleaved", 0), ("interleaved", 40), ("half", 0), ("half", 40)])
+@pytest.mark.parametrize("D", [40, 72, 80, 136])
+def test_rows_that_leave_threads_idle(gpu, D, mode, rotary):
+    """Head sizes between powers of two, behind a call that has left NaN in every multiprocessor's shared memory."""
+    r = np.random.default_rng(D)
+    big, nan = np.ones((4, 256, 8, 256), np.float32), np.full(256, np.nan, np.float32)
+    x, dy, w = draw(r, 4, 99, 5, D), draw(r, 4, 99, 5, D), 1 + 0.2 * draw(r, D)
+    rotary = rotary if rotary <= D else 0
+    gpu.qk_norm_rope_backward(big, None, big, None, nan)
+    g = gpu.qk_norm_rope_backward(dy, None, x, None, w, rope_mode=mode, rotary_dim=rotary)
+    pos = np.broadcast_to(np.arange(99), (4, 99))
+    want, _ = orc.norm_rope_grad(x, w, dy, pos, orc.frequencies(rotary or D), mode)
+    x64 = x.astype(np.float64)
+    size = np.abs(w).max() * np.sqrt((dy.astype(np.float64) ** 2).sum(-1, keepdims=True) / ((x64 * x64).mean(-1, keepdims=True) + 1e-6))
+    assert (np.abs(g["grad_q"] - want) <= (3 * D + 32) * U * 2 * size).all()
