@@ -199,3 +199,31 @@ def test_rows_that_leave_threads_idle(gpu, D, mode, rotary):
     x64 = x.astype(np.float64)
     size = np.abs(w).max() * np.sqrt((dy.astype(np.float64) ** 2).sum(-1, keepdims=True) / ((x64 * x64).mean(-1, keepdims=True) + 1e-6))
     assert (np.abs(g["grad_q"] - want) <= (3 * D + 32) * U * 2 * size).all()
+
+
+@pytest.mark.parametrize("T,group,dtype", [(4, 4, "bf16"), (5, 4, "bf16"), (16, 4, "bf16"), (31, 4, "bf16"), (61, 4, "bf16"), (128, 8, "bf16"),
+                                           (11, 3, "fp32")])
+def test_many_calls_give_the_same_bits(core, T, group, dtype):
+    """Ragged sequences, calls back to back without a wait between them."""
+    r = np.random.default_rng(T)
+    ctx = core.Device()
+    B, hkv, D = 6, 8, 128
+    kv = core.create_kv_cache(ctx, num_heads=hkv, head_dim=D, compression_ratio=1, max_cache_tokens=2048, use_h2o=False, batch_size=B, dtype=dtype)
+    core.kv_cache_append(ctx, kv, draw(r, B, 1501, hkv, D), draw(r, B, 1501, hkv, D))
+    q, k, v = (core.DeviceTensor.from_numpy(ctx, draw(r, B, T, h, D), dtype=dtype) for h in (hkv * group, hkv, hkv))
+    parents = np.array([[-1] + [int(r.integers(-1, t)) for t in range(1, T)] for _ in range(B)], np.int32)
+    core.draft_step(ctx, kv, q, k, v, parents, [T, 1, 0, T // 2, T, T - 1])
+    outs = [core.tree_attention(ctx, q, kv, parents) for _ in range(120)]
+    first = outs[0].to_numpy()
+    assert np.isfinite(first).all() and first[0].any() and not first[2].any()
+    assert all(np.array_equal(o.to_numpy(), first) for o in outs[1:])
+    core.destroy_kv_cache(ctx, kv)
+
+
+def test_heads_without_a_rotation(gpu):
+    """rope_theta = 0: normalised only, wherever the tokens stand."""
+    r = np.random.default_rng(3)
+    x, w = draw(r, 2, 7, 3, 64), 1 + 0.1 * draw(r, 64)
+    want = orc.norm(x, w, 1e-6)
+    got = gpu.qk_norm_rope(x, q_weight=w, rope_theta=0.0, pos_base=1000)
+    assert (np.abs(got - want) <= (64 / 2 + 8) * U * np.abs(want) + 2.0 ** -126).all()
