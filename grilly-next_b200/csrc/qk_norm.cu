@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(256) qk_norm_rows_kernel(const __grid_constant
 // factors for all heads of a token; addresses a step from head to head.  Every warp has an equal, contiguous share of the rows (token, head)
 // and walks it in segments, heads of one token and one side: its groups take the heads in turn, RUN rows of each in flight, the next one
 // asked for as soon as its registers are free.
+// 4 x 2048 tokens, 32 + 8 heads of 128, bf16: 34 us (4.9 TB/s); a warp a row 229, without packed operations 69, without segments 36.
 template <typename T> constexpr int kRunOf = sizeof(T) == 2 ? 4 : 2;
 template <typename TIn, typename TOut, int LANES, bool HALF, bool FULL>
 __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__ NormArgs a) {
@@ -143,6 +144,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_kernel(const __grid_constant__
 
 // The backward pass in the same form.  A CTA takes the queries or the keys, as many CTAs each as they have rows; a group keeps its share of the
 // weight's gradient in registers, the CTA adds them in order of its groups.
+// 2 x 2048 tokens, 32 + 8 heads of 128, bf16: 31.7 us with the launch that adds the parts; a warp a row 199, both sides in every CTA 35.
 template <typename T> constexpr int kGradRunOf = sizeof(T) == 2 ? 4 : 2;
 template <typename TIn, typename TOut, int LANES, bool HALF, bool FULL>
 __global__ void __launch_bounds__(256, 2) qk_norm_backward_kernel(const __grid_constant__ NormArgs a) {

@@ -16,6 +16,9 @@
 // of V past the sequence's end, which may hold anything, are cleared in shared memory ahead of the product, and so are elements
 // that are no finite number; rows that see such an element get it added behind the epilogue, so that it reaches nobody else.
 //
+// Measured: 32 x 8 heads x 4096 tokens, 64 rows 106 us (5.2 TB/s; HBM, and the ends of CTAs that have an SM to themselves), 1 x 8 x 131072, 244 rows
+// 147 to 163 us (800 to 900 TFLOP/s; tensor pipe 48 % busy, exponentials 53 %, the chain between them), 1 x 8 x 1001, 20 rows 10.6 us (latency).
+//
 // Every mbarrier wait is bounded; on expiry the CTA records an error, drains its copies and returns.
 #include <cuda.h>
 
@@ -563,16 +566,12 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (warp == WARP_MMA0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
 }
 
-// Joins the parts of heads that several CTAs have worked on, a warp a row at a time: the parts' sums at their common maximum, eight parts on
-// their way at once.
-constexpr int kJoinRows = 16;       // of a CTA
-// The fewest stages of a split.  us, split into 1 / 2 / 3 / 4: 4 x 8 heads x 700 tokens, 124 rows 15.2 / 15.9 / 15.2 / 15.0, 64 rows 14.2 / 15.7 /
-// 13.3 / 13.5; 1500 tokens, 64 rows 21.4 / 18.1 / - / 17.7.  More heads than SMs are not split: 20 x 8 x 4096, 124 rows 98.7 / 106 / 110, 64 rows
-// 106 / 102 / 105, 20 x 8 x 1024 40.4 / 49.3 / 57.2, 24 x 8 x 4096 101 / 121.  Equal shares of all stages for every CTA, heads cut where they fall, are no
-// faster anywhere: 32 x 8 x 4096, 64 rows 118 for 106, 4 x 8 x 1500 27.1 for 17.7, 1 x 8 x 131072 of 244 rows 172 for 163.
-constexpr int kSplitStages = 4;
+// Joins the parts of heads that several CTAs have worked on, a warp a row: the parts' sums at their common maximum, eight parts on
+// their way at once.  Latency: two rows a warp, one behind the other, take 0.9 us longer behind 1 x 8 heads of 1001 tokens (11.5 / 10.6) and 2 us
+// behind 131072 tokens of 244 rows (147.4 / 145.4).
+constexpr int kJoinRows = 8;        // of a CTA
 template <int HD>
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Groups sh, int part_rows) {
+__global__ void __launch_bounds__(32 * kJoinRows) tree_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ Groups sh, int part_rows) {
     const int hgs = a.Hkv * sh.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = blockIdx.x / hgs, hg = blockIdx.x % hgs;
     pdl_wait();                 // every CTA, or the kernel behind this one could start before the one ahead of it has ended
@@ -581,55 +580,55 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     const size_t stride = (size_t)part_rows * (HD + 2);
     const float* first_part = a.part + (size_t)blockIdx.x * a.n_splits * stride;
     const int kvh = hg / sh.groups, r0 = hg % sh.groups * part_rows, rows = min(part_rows, a.R - r0);
-    for (int rr = blockIdx.y * kJoinRows + warp; rr < min(rows, (int)(blockIdx.y + 1) * kJoinRows); rr += 8) {
-        float m = -INFINITY, l = 0.f, acc[V];
+    const int rr = blockIdx.y * kJoinRows + warp;
+    if (rr >= rows) return;
+    float m = -INFINITY, l = 0.f, acc[V];
 #pragma unroll
-        for (int c = 0; c < V; ++c) acc[c] = 0.f;
-        for (int i0 = 0; i0 < a.n_splits; i0 += 8) {
-            float2 ml[8];
-            float o[8][V];
+    for (int c = 0; c < V; ++c) acc[c] = 0.f;
+    for (int i0 = 0; i0 < a.n_splits; i0 += 8) {
+        float2 ml[8];
+        float o[8][V];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = i0 + j;
-                ml[j] = make_float2(-INFINITY, 0.f);
-                if (i >= a.n_splits) continue;
-                const float* p = first_part + (size_t)i * stride;
-                ml[j] = __ldcg(reinterpret_cast<const float2*>(p + (size_t)part_rows * HD) + rr);
-                if constexpr (V == 4) {
-                    const float4 f = __ldcg(reinterpret_cast<const float4*>(p + (size_t)rr * HD) + lane);
-                    o[j][0] = f.x; o[j][1] = f.y; o[j][2] = f.z; o[j][3] = f.w;
-                } else {
-                    const float2 f = __ldcg(reinterpret_cast<const float2*>(p + (size_t)rr * HD) + lane);
-                    o[j][0] = f.x; o[j][1] = f.y;
-                }
-            }
-            float m_new = m;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (ml[j].y != 0.f) m_new = fmaxf(m_new, ml[j].x);
-            const float f = m == -INFINITY ? 0.f : exp2f(m - m_new);
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < V; ++c) acc[c] *= f;
-            m = m_new;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (ml[j].y == 0.f) continue;       // a part that has seen nothing has no O
-                const float w = exp2f(ml[j].x - m);
-                l = fmaf(w, ml[j].y, l);
-#pragma unroll
-                for (int c = 0; c < V; ++c) acc[c] = fmaf(w, o[j][c], acc[c]);
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j;
+            ml[j] = make_float2(-INFINITY, 0.f);
+            if (i >= a.n_splits) continue;
+            const float* p = first_part + (size_t)i * stride;
+            ml[j] = __ldcg(reinterpret_cast<const float2*>(p + (size_t)part_rows * HD) + rr);
+            if constexpr (V == 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(p + (size_t)rr * HD) + lane);
+                o[j][0] = f.x; o[j][1] = f.y; o[j][2] = f.z; o[j][3] = f.w;
+            } else {
+                const float2 f = __ldcg(reinterpret_cast<const float2*>(p + (size_t)rr * HD) + lane);
+                o[j][0] = f.x; o[j][1] = f.y;
             }
         }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int r = r0 + rr, node = node_of(sh, r);
-        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r - node * a.G) * HD;
-        if constexpr (V == 4) {
-            const __nv_bfloat162 p0 = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), p1 = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
-            reinterpret_cast<uint2*>(out)[lane] = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
-        } else {
-            reinterpret_cast<__nv_bfloat162*>(out)[lane] = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+        float m_new = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (ml[j].y != 0.f) m_new = fmaxf(m_new, ml[j].x);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - m_new);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[c] *= f;
+        m = m_new;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (ml[j].y == 0.f) continue;       // a part that has seen nothing has no O
+            const float w = exp2f(ml[j].x - m);
+            l = fmaf(w, ml[j].y, l);
+#pragma unroll
+            for (int c = 0; c < V; ++c) acc[c] = fmaf(w, o[j][c], acc[c]);
         }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int r = r0 + rr, node = node_of(sh, r);
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r - node * a.G) * HD;
+    if constexpr (V == 4) {
+        const __nv_bfloat162 p0 = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), p1 = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+        reinterpret_cast<uint2*>(out)[lane] = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
+    } else {
+        reinterpret_cast<__nv_bfloat162*>(out)[lane] = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
     }
 }
 
@@ -645,7 +644,7 @@ static int make_pool_map(grl_device* dev, CUtensorMap* tm, const void* pool, con
 
 static int join(grl_device* dev, const TreeArgs& a, const Groups& sh, int part_rows) {
     const dim3 grid(a.B * a.Hkv * sh.groups, (min(part_rows, a.R) + kJoinRows - 1) / kJoinRows);
-    GRL_CUDA(launch_pdl(a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<64>, grid, 256, 0, dev->stream, a, sh, part_rows));
+    GRL_CUDA(launch_pdl(a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<64>, grid, 32 * kJoinRows, 0, dev->stream, a, sh, part_rows));
     GRL_LAUNCHED("tree_join_kernel");
     return GRL_OK;
 }
@@ -671,6 +670,11 @@ static Groups groups_of(int G, int groups) { return {G == 1 ? 0u : (uint32_t)(((
 
 int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows) { return tree::join(dev, a, tree::groups_of(a.G, 1), rows); }
 
+// The fewest stages of a split.  us, split into 1 / 2 / 3 / 4: 4 x 8 heads x 700 tokens, 124 rows 15.2 / 15.9 / 15.2 / 15.0, 64 rows 14.2 / 15.7 /
+// 13.3 / 13.5; 1500 tokens, 64 rows 21.4 / 18.1 / - / 17.7.  More heads than SMs are not split: 20 x 8 x 4096, 124 rows 98.7 / 106 / 110, 64 rows
+// 106 / 102 / 105, 20 x 8 x 1024 40.4 / 49.3 / 57.2, 24 x 8 x 4096 101 / 121.  Equal shares of all stages for every CTA, heads cut where they fall, are no
+// faster anywhere: 32 x 8 x 4096, 64 rows 118 for 106, 4 x 8 x 1500 27.1 for 17.7, 1 x 8 x 131072 of 244 rows 172 for 163.
+constexpr int kSplitStages = 4;
 // asked: the caller's number of splits, or 0.
 TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked) {
     using namespace tree;
