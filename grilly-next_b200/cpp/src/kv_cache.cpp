@@ -24,19 +24,25 @@ struct Recording {
 // Give every sequence pages for `extra` (or its own count) more tokens; uploads the block table when it changed.
 void reservePages(BufferPool& pool, KVCache& kv, uint32_t extra, const std::vector<int32_t>& counts = {}) {
     const auto& c = kv.config;
-    bool changed = false;
+    const auto pagesOf = [&](uint32_t b) {
+        return (uint32_t(kv.hostSeqLens[b]) + (counts.empty() ? extra : uint32_t(counts[b])) + c.pageTokens - 1) / c.pageTokens;
+    };
+    // looked over before any page is given out: a page given here and not uploaded would be taken for one that the device knows
+    uint32_t fresh = 0;
     for (uint32_t b = 0; b < c.batchSize; ++b) {
-        const uint32_t need = (uint32_t(kv.hostSeqLens[b]) + (counts.empty() ? extra : uint32_t(counts[b])) + c.pageTokens - 1) / c.pageTokens;
+        const uint32_t need = pagesOf(b);
         if (need > kv.maxPages)
             throw std::runtime_error("kvCacheAppend: sequence would exceed max_cache_tokens (" +
                                      std::to_string(c.maxCacheTokens) + ")");
+        for (uint32_t i = 0; i < need; ++i) fresh += kv.hostBlockTable[size_t(b) * kv.maxPages + i] < 0;
+    }
+    if (fresh > kv.numPages - kv.nextFreePage) throw std::runtime_error("kvCacheAppend: page pool exhausted");
+    const bool changed = fresh > 0;
+    for (uint32_t b = 0; b < c.batchSize; ++b) {
+        const uint32_t need = pagesOf(b);
         for (uint32_t i = 0; i < need; ++i) {
             int32_t& slot = kv.hostBlockTable[size_t(b) * kv.maxPages + i];
-            if (slot < 0) {
-                if (kv.nextFreePage >= kv.numPages) throw std::runtime_error("kvCacheAppend: page pool exhausted");
-                slot = int32_t(kv.nextFreePage++);
-                changed = true;
-            }
+            if (slot < 0) slot = int32_t(kv.nextFreePage++);
         }
     }
     if (changed) {

@@ -227,3 +227,23 @@ def test_heads_without_a_rotation(gpu):
     want = orc.norm(x, w, 1e-6)
     got = gpu.qk_norm_rope(x, q_weight=w, rope_theta=0.0, pos_base=1000)
     assert (np.abs(got - want) <= (64 / 2 + 8) * U * np.abs(want) + 2.0 ** -126).all()
+
+
+def test_a_refused_step_gives_out_no_pages(gpu):
+    """One sequence has room and the other has not: the call is refused, and the next one finds the pages as they were."""
+    r = np.random.default_rng(11)
+    kv = gpu.create_kv_cache(num_heads=1, head_dim=32, compression_ratio=1, max_cache_tokens=32, use_h2o=False, batch_size=2, page_tokens=8, dtype="fp32")
+    rows = [[], []]
+    for counts, fits in (([8, 28], True), ([8, 8], False), ([8, 2], True), ([8, 0], True)):
+        n = max(counts)
+        q, k, v = draw(r, 2, n, 2, 32), draw(r, 2, n, 1, 32), draw(r, 2, n, 1, 32)
+        if not fits:
+            with pytest.raises(RuntimeError, match="max_cache_tokens"):
+                gpu.draft_step(kv, q, k, v, None, counts)
+            continue
+        gpu.draft_step(kv, q, k, v, None, counts)
+        for b in range(2):
+            rows[b] += list(v[b, :counts[b]])
+    for b in range(2):
+        assert np.array_equal(gpu.kv_cache_decode(kv, b)["values"], np.array(rows[b]))
+    gpu.destroy_kv_cache(kv)
