@@ -221,11 +221,6 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             __syncwarp();
             issue(p);
         }
-        if (*reinterpret_cast<volatile int*>(&blk.abort)) {       // copies in flight land before the ring is used again
-            const long long t0 = clock64();
-            for (int x = last; x >= 0 && x > last - NST; --x)
-                while (!mbar_try_wait(full(x % NST), (x / NST) & 1) && clock64() - t0 < kDrainCycles) {}
-        }
     } else {
         const int mat = lane >> 3;
         // operand rows of this lane's ldmatrix addresses: queries, keys (two 8-token tiles), values (transposed)
@@ -332,7 +327,18 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         }
     }
-    __syncthreads();            // the ring is free: every copy has come in and been read
+    __syncthreads();
+    if (*reinterpret_cast<volatile int*>(&blk.abort)) {
+        // A wait ran out, maybe behind the producer's last look at the flag: copies in flight land before the ring is used again.  No wait of
+        // the stream is left, so that the whole CTA finds the flag as it is.
+        if (warp == 4) {
+            const long long t0 = clock64();
+            for (int x = last; x >= 0 && x > last - NST; --x)
+                while (!mbar_try_wait(full(x % NST), (x / NST) & 1) && clock64() - t0 < kDrainCycles) {}
+        }
+        __syncthreads();
+    }
+    // the ring is free: every copy has come in and been read
     pdl_trigger();
     float* warp_o = reinterpret_cast<float*>(smem);
     float2* warp_ml = reinterpret_cast<float2*>(smem + F::WARP_ML);

@@ -289,6 +289,42 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(T):
     dev.close()
 
 
+def single_stages_that_run_out(T, splits, B=24):
+    """Shares of one stage: all copies are on their way before any wait begins, and whoever asked for them waits no more.  With waits of one cycle
+    it is a reader that gives up, and the kernel may leave only when the copies have landed: the calls in between take the same shared memory,
+    and give what they gave before.  Many CTAs and a cold L2, so that copies take longer than the hardware suspends a wait."""
+    from grilly_next import cabi
+    dev = cabi.Device(0)
+    cache = Cache(dev, [64 * (splits - 1) + T + b % (65 - T) for b in range(B)], 8, 128, 64, "bf16", seed=12)
+    other = dev.malloc(1 << 28)
+    q = round_bf16(np.random.default_rng(12).standard_normal((B, T, 32, 128)).astype(np.float32))
+    call = lambda: attend(dev, cache, q, None, None, io="bf16", splits=splits)  # noqa: E731
+    want = call()
+    check_attention(want, cache, q, None, None, "bf16", False)
+    ran_out = 0
+    for _ in range(100):
+        cabi.check(dev.L.grl_memset(dev.h, other, 0, 1 << 28))
+        cabi.check(dev.L.grl_device_set_wait_limits(dev.h, 1, 0))
+        try:
+            assert np.array_equal(call(), want)
+        except cabi.GrlError as e:
+            assert e.code == cabi.ERR_TIMEOUT and "tree attention" in str(e)
+            ran_out += 1
+        cabi.check(dev.L.grl_device_set_wait_limits(dev.h, 0, 0))
+        assert np.array_equal(call(), want)
+        if ran_out == 8:
+            break
+    assert ran_out
+    dev.free(other)
+    cache.free()
+    dev.close()
+
+
+@pytest.mark.parametrize("T,splits", [(1, 9), (4, 6), (4, 20)])
+def test_a_reader_that_gives_up_leaves_no_copies_behind_few_rows(T, splits):
+    single_stages_that_run_out(T, splits)
+
+
 def test_refusals_of_the_tensor_core_kernel(dev):
     from grilly_next import cabi
     for c in (TREES["f32"], TREES["bf16_page_24"], TREES["bf16_dim_32"], TREES["f32_over_bf16"]):
