@@ -220,6 +220,15 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     // steps of chain t over ns stages: one for each, or for two; a tile without rows takes none
     auto steps_of = [&](int t) { return PAIR ? (r0 + t * BM < a.R ? ns : 0) : FOLD ? ((ns + 1) / 2 - t + 1) / 2 : (ns - t + 1) / 2; };
 
+    // every warp at its end; behind it nobody reads the shared or the tensor memory any more
+    auto finish = [] {
+        pdl_trigger();
+        tc_fence_before();
+        __syncwarp();
+        asm volatile("bar.sync 2, %0;" ::"n"(kThreads) : "memory");
+        tc_fence_after();
+    };
+
     if (warp < WARP_SOFTMAX) {
       reg_dec<REGS_MISC>();
       if (warp == WARP_TMA0 || warp == WARP_TMA1) {
@@ -254,7 +263,9 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             __syncwarp();
             last = k;
         }
-        if (*ctx.abort) {       // copies in flight land before the shared memory is given back
+        finish();
+        // A wait ran out, maybe behind this warp's last look at the flag: copies in flight land before the shared memory is given back.
+        if (*ctx.abort) {
             const long long t0 = clock64();
             for (int x = last; x >= 0 && x > last - F::SLOTS; x -= PAIR ? 2 : 1)
                 while (!mbar_try_wait(bar(F::FULL + slot_of(t, x)), (x / F::SLOTS) & 1) && clock64() - t0 < kDrainCycles) {}
@@ -309,11 +320,11 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         // for a chain without steps too
         if (ok) mma_commit(bar(F::O_DONE + t));
-        if (!ok) {              // products in flight end before the tensor memory and the operands are given back
+        finish();
+        if (*ctx.abort) {       // and products in flight end before the tensor memory and the operands are
             mma_commit(bar(F::DRAIN + t));
             const long long t0 = clock64();
             while (!mbar_try_wait(bar(F::DRAIN + t), 0) && clock64() - t0 < kDrainCycles) {}
-            __syncwarp();
         }
       }
     } else {
@@ -557,11 +568,9 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     }
                 }
         }
+        finish();
     }
-    pdl_trigger();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    if (*ctx.abort) __syncthreads();        // the whole CTA finds the flag as it is: no wait under the budget is left
     __syncwarp();
     if (warp == WARP_MMA0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
 }

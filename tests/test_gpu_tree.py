@@ -325,6 +325,12 @@ def test_a_reader_that_gives_up_leaves_no_copies_behind_few_rows(T, splits):
     single_stages_that_run_out(T, splits)
 
 
+@pytest.mark.parametrize("T,splits", [(8, 9), (16, 6), (20, 8), (61, 7)])
+def test_a_reader_that_gives_up_leaves_no_copies_behind_tiles(T, splits):
+    """Shares of a chain, the folded and the split tile and two tiles: products in flight end as well before the tensor memory is given back."""
+    single_stages_that_run_out(T, splits, 6)
+
+
 def test_refusals_of_the_tensor_core_kernel(dev):
     from grilly_next import cabi
     for c in (TREES["f32"], TREES["bf16_page_24"], TREES["bf16_dim_32"], TREES["f32_over_bf16"]):
