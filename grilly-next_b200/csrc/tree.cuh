@@ -21,7 +21,9 @@ struct TreeArgs {
     void* out;
     const int32_t* parents;
     const int32_t* n_nodes;
-    float* part;            // [split][ O (rows, D) | (m, l) (rows) ], rows = (sequence, kv head, node, head of the group); m in the exp2 domain
+    // [split][ O (rows, D) | (m, l) (rows) ], rows = (sequence, kv head, node, head of the group); m in the exp2 domain.  l = 0: the split has no
+    // weight in the row (nothing seen, or scores of -inf only); l < 0: no node's row, 0 in the result.
+    float* part;
     size_t part_stride;     // floats of a split, rows * (D + 2) rounded up to 16 bytes
     int32_t* status;
     int B, Hq, Hkv, G, T, R, D, P, max_pages, num_pages, n_splits;      // R = T * G rows of a (sequence, kv head)
@@ -52,6 +54,12 @@ struct TreeMmaPlan {
 };
 TreeMmaPlan tree_mma_plan(grl_device* dev, int B, int Hkv, int D, int longest, int asked);
 int tree_mma_launch(grl_device* dev, const TreeArgs& a, const TreeMmaPlan& plan);
+
+// A row that has met a score that is no number (l is NaN then) has no maximum, which such scores do not raise: 0 stands for it, so that the row is not
+// taken for one that saw nothing, whose maximum is -inf.  Its sum makes the result NaN, as the definition has it.
+#ifdef __CUDACC__
+__device__ __forceinline__ float tree_row_max(float m, float l) { return l != l ? 0.f : m; }
+#endif
 
 inline size_t tree_part_stride(size_t rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }
 

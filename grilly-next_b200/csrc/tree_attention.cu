@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(32 * kTreeWarps) tree_rows_kernel(const __grid
         const size_t row = ((size_t)b * a.Hkv + kvh) * a.R + r0 + x;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) part[row * D + lane + 32 * i] = acc[x][i];
-        if (lane == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * row) = live[x] ? make_float2(m[x], sum) : make_float2(-INFINITY, 0.f);
+        if (lane == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * row) = live[x] ? make_float2(tree_row_max(m[x], sum), sum) : make_float2(-INFINITY, -1.f);
     }
 }
 
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     const float* ml = a.part + rows * a.D + 2 * row;
     const float* o_at = a.part + row * a.D + lane;
     float m = -INFINITY, l = 0.f, acc[8];
+    bool nobody = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     constexpr int AT_ONCE = 8;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j)
-            if (v[j].y != 0.f) top = fmaxf(top, v[j].x);
+            if (!(v[j].y <= 0.f)) top = fmaxf(top, v[j].x);
         const float f = m == -INFINITY ? 0.f : exp2f(m - top);
         m = top;
         l *= f;
@@ -235,7 +236,8 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
         for (int i = 0; i < 8; ++i) acc[i] *= f;
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
-            if (v[j].y == 0.f) continue;       // saw nothing
+            nobody |= v[j].y < 0.f;
+            if (v[j].y <= 0.f) continue;       // saw nothing
             const float w = exp2f(v[j].x - m);
             l = fmaf(w, v[j].y, l);
 #pragma unroll
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     const int r = (int)(row % a.R), kvh = (int)(row / a.R % a.Hkv);
     const size_t b = row / a.R / a.Hkv;
     TIO* out = reinterpret_cast<TIO*>(a.out) + ((b * a.T + r / a.G) * a.Hq + kvh * a.G + r % a.G) * a.D;
-    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const float inv = nobody ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (lane + 32 * i < a.D) store_from_float<TIO>(out + lane + 32 * i, acc[i] * inv);

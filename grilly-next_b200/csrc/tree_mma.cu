@@ -325,6 +325,7 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            m_ref[h] = tree_row_max(m_ref[h], l[h]);
         }
     }
     __syncthreads();
@@ -406,7 +407,7 @@ tree_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (c == 0) cta_ml[r] = make_float2(m, sum);
         } else {
             reinterpret_cast<float4*>(part)[r * (HD / 4) + c] = v;
-            if (c == 0) reinterpret_cast<float2*>(part + kRows * HD)[r] = node_of(r) < live_nodes ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+            if (c == 0) reinterpret_cast<float2*>(part + kRows * HD)[r] = node_of(r) < live_nodes ? make_float2(m, sum) : make_float2(-INFINITY, -1.f);
         }
     }
     if (args.cluster > 1) {

@@ -484,6 +484,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         meet();
         ok = __all_sync(0xffffffffu, ok && !*ctx.abort);
         tc_fence_after();
+        m_ref = tree_row_max(m_ref, l);
         float m = m_ref, sum = l;
         if constexpr (F::STREAMS > 1) {
             float2* ml = reinterpret_cast<float2*>(smem);
@@ -504,6 +505,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         float* part = a.part + ((size_t)(b * gridDim.y + blockIdx.y) * a.n_splits + blockIdx.x) * F::PART;
         const int rows = min(F::ROWS, a.R - r0), live_nodes = bad_tree ? 0 : n;
         const bool full = ok && nh > 0 && m_ref != -INFINITY;
+        const uint32_t empty = whole && live && sum == 0.f ? 0x7fc00000u : 0u;      // a node without any weight, scores of -inf only: NaN
         // a thread takes one 16-byte piece of every 32nd row
         constexpr int K = F::ROWS / 32;
         const int c = st_id & 7, rr0 = st_id >> 3;
@@ -525,7 +527,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             for (int e = 0; e < 8; ++e) {
                 const uint4 v = make_uint4(__float_as_uint(__uint_as_float(o[4 * e]) * w), __float_as_uint(__uint_as_float(o[4 * e + 1]) * w),
                                            __float_as_uint(__uint_as_float(o[4 * e + 2]) * w), __float_as_uint(__uint_as_float(o[4 * e + 3]) * w));
-                sts128(base + st_id * 128 + ((e ^ (st_id & 7)) << 4), full ? v : make_uint4(0u, 0u, 0u, 0u));
+                sts128(base + st_id * 128 + ((e ^ (st_id & 7)) << 4), full ? v : make_uint4(empty, empty, empty, empty));
             }
             meet();
 #pragma unroll
@@ -550,7 +552,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         const bool owner = st_id < F::ROWS && st_id < rows;         // of row r in the results
         if (!whole && owner)
-            reinterpret_cast<float2*>(part + (size_t)F::ROWS * HD)[st_id] = live && ok && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+            reinterpret_cast<float2*>(part + (size_t)F::ROWS * HD)[st_id] =
+                !live ? make_float2(-INFINITY, -1.f) : ok && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
         if ((blk.bad[0] | blk.bad[1] | blk.bad[2] | blk.bad[3]) != 0u) {         // rare: what is no finite number, for the rows that see it
             if (owner && live && ok)
                 for (int u = 0; u < n; ++u) {
@@ -592,6 +595,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_join_kernel(const __grid_
     const int rr = blockIdx.y * kJoinRows + warp;
     if (rr >= rows) return;
     float m = -INFINITY, l = 0.f, acc[V];
+    bool nobody = false;
 #pragma unroll
     for (int c = 0; c < V; ++c) acc[c] = 0.f;
     for (int i0 = 0; i0 < a.n_splits; i0 += 8) {
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_join_kernel(const __grid_
         float m_new = m;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (ml[j].y != 0.f) m_new = fmaxf(m_new, ml[j].x);
+            if (!(ml[j].y <= 0.f)) m_new = fmaxf(m_new, ml[j].x);
         const float f = m == -INFINITY ? 0.f : exp2f(m - m_new);
         l *= f;
 #pragma unroll
@@ -623,14 +627,15 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_join_kernel(const __grid_
         m = m_new;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (ml[j].y == 0.f) continue;       // a part that has seen nothing has no O
+            nobody |= ml[j].y < 0.f;
+            if (ml[j].y <= 0.f) continue;       // a part that has seen nothing has no O
             const float w = exp2f(ml[j].x - m);
             l = fmaf(w, ml[j].y, l);
 #pragma unroll
             for (int c = 0; c < V; ++c) acc[c] = fmaf(w, o[j][c], acc[c]);
         }
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const float inv = nobody ? 0.f : 1.f / l;
     const int r = r0 + rr, node = node_of(sh, r);
     __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (((size_t)b * a.T + node) * a.Hq + kvh * a.G + r - node * a.G) * HD;
     if constexpr (V == 4) {

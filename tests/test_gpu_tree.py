@@ -289,6 +289,66 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(T):
     dev.close()
 
 
+# T, group, cache and io type, splits: every form of the kernels, whole, joined in a cluster and joined behind
+FORMS = [(1, 4, "bf16", 1), (4, 4, "bf16", 3), (4, 4, "bf16", 17), (12, 4, "bf16", 1), (12, 4, "bf16", 4), (24, 4, "bf16", 1), (24, 4, "bf16", 5),
+         (40, 4, "bf16", 1), (40, 4, "bf16", 3), (100, 4, "bf16", 2), (6, 4, "f32", 1), (6, 4, "f32", 4)]
+
+
+@pytest.mark.parametrize("T,group,io,splits", FORMS)
+def test_what_is_no_number_comes_out_as_none(T, group, io, splits):
+    """A row whose scores hold a NaN is NaN, and so is one whose scores are all -inf, in every form; a single score of -inf has no weight; the other
+    rows are as without it."""
+    from grilly_next import cabi
+    dev = cabi.Device(0)
+    r = np.random.default_rng(21)
+    Hkv, D, lens = 2, 128, [700 + T, T, 130 + T]
+    counts = [T, T, T // 2]
+    cache = Cache(dev, lens[:2] + [130 + T // 2], Hkv, D, 64, io, seed=21)
+    parents = [draw_parents(r, T, "tree") for _ in lens]
+    q = round_bf16(r.standard_normal((3, T, Hkv * group, D)).astype(np.float32))
+    q[..., 0] = 1 + np.abs(q[..., 0])
+    q = round_bf16(q)
+    call = lambda x: attend(dev, cache, x, parents, counts, io=io, splits=splits)  # noqa: E731
+    clean = call(q)
+    check_attention(clean, cache, q, parents, counts, io, io == "f32")
+    # a query
+    bad = q.copy()
+    bad[0, T - 1, 1, 5] = bad[1, 0, group, 77] = bad[2, 0, 0, 0] = np.nan
+    bad[2, T // 2:] = np.nan                                     # rows of padding
+    got = call(bad)
+    hit = np.isnan(bad).any(-1)
+    hit[2, T // 2:] = False
+    assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
+    # a key among the cached tokens, of one head; a key of a node
+    for b, at, value in ((0, 3, np.nan), (0, 699, np.nan), (2, 129, np.nan), (1, T // 3, np.nan)):
+        keep = cache.pools[0].copy()
+        cache.pools[0][cache.table[b, at // 64], 1, at % 64, 9] = value
+        cache.put(0, b, at, cache.pools[0][cache.table[b, at // 64], :, at % 64].copy())
+        got = call(q)
+        hit = np.zeros(got.shape[:3], bool)
+        first = cache.lens[b] - counts[b]
+        sees = np.ones(counts[b], bool) if at < first else orc.ancestors(parents[b], counts[b])[:, at - first]
+        hit[b, :counts[b], group:] = sees[:, None]
+        assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
+        cache.pools[0] = keep
+    # every key of a head -inf, then all but one
+    keep = cache.pools[0].copy()
+    cache.pools[0][:, 1, :, 0] = -np.inf
+    cache.put(0, 0, 0, cache.pools[0][cache.table[0, 0], :, 0].copy())
+    got = call(q)
+    hit = np.zeros(got.shape[:3], bool)
+    for b in range(3):
+        hit[b, :counts[b], group:] = True
+    assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
+    cache.put(0, 0, 5, keep[cache.table[0, 0], :, 5])
+    got = call(q)
+    for h in range(group, 2 * group):
+        v = cache.rows[1][0][5, 1]
+        assert (np.abs(got[0, :, h] - v) <= 2.0 ** -7 * np.abs(v)).all()       # a weight of one, rounded twice at the most
+    cache.free()
+    dev.close()
+
+
 def single_stages_that_run_out(T, splits, B=24):
     """Shares of one stage: all copies are on their way before any wait begins, and whoever asked for them waits no more.  With waits of one cycle
     it is a reader that gives up, and the kernel may leave only when the copies have landed: the calls in between take the same shared memory,
