@@ -14,7 +14,8 @@
 // A CTA takes one split of the stages of one (sequence, kv head, group of rows); the rows of several splits meet in tree_join_kernel.
 // The predicate is applied to the last stages only, those with nodes in them: a row has one bit for each of 128 nodes.  There, rows
 // of V past the sequence's end, which may hold anything, are cleared in shared memory ahead of the product, and so are elements
-// that are no finite number; rows that see such an element get it added behind the epilogue, so that it reaches nobody else.
+// that are no finite number; rows that see such an element get it added behind the epilogue, so that it reaches nobody else.  Among the
+// cached tokens, which all rows see, infinities stay where they are; only FOLD, whose zeros in P meet them too, puts right what came out as NaN.
 //
 // Measured: 32 x 8 heads x 4096 tokens, 64 rows 106 us (5.2 TB/s; HBM, and the ends of CTAs that have an SM to themselves), 1 x 8 x 131072, 244 rows
 // 147 to 163 us (800 to 900 TFLOP/s; tensor pipe 48 % busy, exponentials 53 %, the chain between them), 1 x 8 x 1001, 20 rows 10.6 us (latency).
@@ -47,7 +48,7 @@ constexpr long long kDrainCycles = 200000000;       // 0.1 s: how long a CTA tha
 struct Block {
     uint64_t bars[32];
     uint32_t tmem;
-    int abort, bad_tree;
+    int abort, bad_tree, nan_out;           // nan_out: FOLD, a result that is, or may be, NaN
     uint32_t bad[4];                        // nodes with elements of V that are no finite number
     int8_t up[GRL_MAX_TREE];                // parents
 };
@@ -158,6 +159,25 @@ __device__ __forceinline__ void clean_values(uint32_t slab, int k0, int prefix, 
 }
 
 
+// Which of inf (1), -inf (2) and NaN (4) are among the cached values of tokens k0 .. k1 - 1, by column; the 256 softmax threads.
+template <int HD>
+__device__ __forceinline__ void find_infinities(const TreeArgs& a, int b, int kvh, int k0, int k1, uint32_t* columns, int st_id) {
+    constexpr int CH = HD / 8;
+#pragma unroll 1
+    for (int idx = st_id; idx < (k1 - k0) * CH; idx += 256) {
+        const int at = k0 + idx / CH, c = idx % CH, page = a.block_table[(size_t)b * a.max_pages + at / a.P];
+        if ((unsigned)page >= (unsigned)a.num_pages) continue;
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.v_pages) +
+                                                             (((size_t)page * a.Hkv + kvh) * a.P + at % a.P) * HD) + c);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t x = w[e >> 1] >> (e & 1) * 16 & 0xffffu;
+            if ((x & 0x7f80u) == 0x7f80u) atomicOr(columns + 8 * c + e, x & 0x7fu ? 4u : x >> 15 ? 2u : 1u);
+        }
+    }
+}
+
 __device__ __forceinline__ int node_of(const Groups& sh, int r) { return sh.per_group ? (int)__umulhi((uint32_t)r, sh.per_group) : r; }
 
 template <int HD, Mode MODE>
@@ -192,7 +212,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             mbar_init(bar(F::DRAIN + t), 1);
         }
         mbar_init(bar(F::Q_READY), 256);
-        blk.abort = blk.bad_tree = 0;
+        blk.abort = blk.bad_tree = blk.nan_out = 0;
         blk.bad[0] = blk.bad[1] = blk.bad[2] = blk.bad[3] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
@@ -540,6 +560,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         const uint4 u = lds128(base + (x * F::ROWS + rr0 + 32 * k) * 128 + ((c ^ (rr0 & 7)) << 4));
                         v.x += __uint_as_float(u.x); v.y += __uint_as_float(u.y); v.z += __uint_as_float(u.z); v.w += __uint_as_float(u.w);
                     }
+                    if (FOLD && isnan((v.x + v.y) + (v.z + v.w)))
+                        *reinterpret_cast<volatile int*>(&blk.nan_out) = 1;
                 }
                 if (whole) {
                     const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x, v.y), p1 = __floats2bfloat162_rn(v.z, v.w);
@@ -554,6 +576,23 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!whole && owner)
             reinterpret_cast<float2*>(part + (size_t)F::ROWS * HD)[st_id] =
                 !live ? make_float2(-INFINITY, -1.f) : ok && ns > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+        if (FOLD && *reinterpret_cast<volatile int*>(&blk.nan_out)) {
+            // rare: an infinity among the cached values times the zeros that a half's rows have for the other's keys.  A row that has a sum at all
+            // has a weight for every cached token, so that its result is that infinity, or NaN where both are in the column, or a NaN.
+            uint32_t* columns = reinterpret_cast<uint32_t*>(smem);
+            if (st_id < HD) columns[st_id] = 0u;
+            meet();
+            find_infinities<HD>(a, b, kvh, min(prefix, st0 * BN), min(prefix, (st0 + ns) * BN), columns, st_id);
+            meet();
+            if (owner && live && ok && sum > 0.f)
+#pragma unroll 1
+                for (int d = 0; d < HD; ++d) {
+                    if (columns[d] != 1u && columns[d] != 2u) continue;
+                    const float x = columns[d] == 1u ? INFINITY : -INFINITY;
+                    if (whole) reinterpret_cast<__nv_bfloat16*>(a.out)[(((size_t)b * a.T + node) * a.Hq + kvh * a.G + r - node * a.G) * HD + d] = __float2bfloat16_rn(x);
+                    else part[(size_t)st_id * HD + d] = x;
+                }
+        }
         if ((blk.bad[0] | blk.bad[1] | blk.bad[2] | blk.bad[3]) != 0u) {         // rare: what is no finite number, for the rows that see it
             if (owner && live && ok)
                 for (int u = 0; u < n; ++u) {

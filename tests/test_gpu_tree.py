@@ -349,6 +349,38 @@ def test_what_is_no_number_comes_out_as_none(T, group, io, splits):
     dev.close()
 
 
+@pytest.mark.parametrize("T,group,io,splits", FORMS)
+def test_infinities_among_the_cached_values(dev, T, group, io, splits):
+    """Every node sees the cached tokens: an infinite value of one is the result of its column, both infinities are NaN, in every form; the other columns,
+    heads and sequences are as without them."""
+    r = np.random.default_rng(22)
+    Hkv, D, P = 2, 128, 64
+    counts = [T, T, max(T // 2, 1)]
+    first = [700, 0, 130]
+    cache = Cache(dev, [f + n for f, n in zip(first, counts)], Hkv, D, P, io, seed=22)
+    parents = [draw_parents(r, T, "tree") for _ in counts]
+    q = round_bf16(r.standard_normal((3, T, Hkv * group, D)).astype(np.float32))
+    call = lambda: attend(dev, cache, q, parents, counts, io=io, splits=splits)  # noqa: E731
+    clean = call()
+    want = clean.copy()
+    for b, at, column, value in ((0, 3, 9, np.inf), (0, 697, 10, -np.inf), (0, 300, 127, np.inf), (2, 129, 64, -np.inf), (2, 100, 65, np.inf)):
+        cache.pools[1][cache.table[b, at // P], 1, at % P, column] = value
+        want[b, :counts[b], group:, column] = value
+    for at, value in ((40, np.inf), (41, -np.inf), (500, np.inf)):
+        cache.pools[1][cache.table[0, at // P], 1, at % P, 77] = value
+    want[0, :, group:, 77] = np.nan
+    cache.pools[1][cache.table[0, 650 // P], 0, 650 % P, 0] = np.nan
+    want[0, :, :group, 0] = np.nan
+    # and a node's: added to an infinity of the other sign it is NaN, for the rows that see it
+    node = T // 2
+    sees = orc.ancestors(parents[0], T)[:, node]
+    cache.pools[1][cache.table[0, (700 + node) // P], 1, (700 + node) % P, 9] = -np.inf
+    want[0, sees, group:, 9] = np.nan
+    cache.put(1, 0, 0, cache.pools[1][cache.table[0, 0], :, 0].copy())
+    assert np.array_equal(call(), want, equal_nan=True)
+    cache.free()
+
+
 def single_stages_that_run_out(T, splits, B=24):
     """Shares of one stage: all copies are on their way before any wait begins, and whoever asked for them waits no more.  With waits of one cycle
     it is a reader that gives up, and the kernel may leave only when the copies have landed: the calls in between take the same shared memory,
