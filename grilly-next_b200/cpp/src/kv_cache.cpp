@@ -550,19 +550,19 @@ void checkDrafted(const char* op, const KVCache& kv, uint32_t n, uint32_t numQHe
     }
 }
 
-void launchTree(BufferPool& pool, const KVCache& kv, const void* q, void* out, int dtype, uint32_t n, uint32_t numQHeads, const int32_t* parents,
-                const int32_t* counts, float scale, std::vector<GrillyBuffer>& scratch) {
+// The parameters of a tree attention over sequences of at most `longest` tokens, looked over, and its workspace: all that can refuse it.
+grl_tree_params treeParams(BufferPool& pool, const KVCache& kv, const void* q, void* out, int dtype, uint32_t n, uint32_t numQHeads, int32_t longest,
+                           float scale, std::vector<GrillyBuffer>& scratch) {
     grl_tree_params p{};
     p.kv = kv.layout();
     p.q = q; p.out = out; p.io_dtype = dtype; p.num_q_heads = int(numQHeads); p.n_tree = int(n);
-    p.scale = scale; p.parents = parents; p.n_nodes = counts;
-    p.max_seq_len = *std::max_element(kv.hostSeqLens.begin(), kv.hostSeqLens.end());
+    p.scale = scale; p.max_seq_len = longest;
     check(grl_tree_workspace_bytes(pool.device().handle(), &p, &p.workspace_bytes), "treeAttention");
     if (p.workspace_bytes) {
         scratch.push_back(pool.acquire(p.workspace_bytes));
         p.workspace = scratch.back().dptr;
     }
-    check(grl_tree_attention(pool.device().handle(), &p), "treeAttention");
+    return p;
 }
 }  // namespace
 
@@ -575,26 +575,32 @@ void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kv, const 
     const size_t qBytes = size_t(c.batchSize) * n * numQHeads * c.headDim * elemSize(dtype), kBytes = qBytes / numQHeads * c.numHeads;
     if (q.size < qBytes || out.size < qBytes || kNew.size < kBytes || vNew.size < kBytes) throw std::runtime_error("draftStep: buffer too small");
     cache.getOrCreate("draft-step/" + std::to_string(c.headDim));
+    // what the attention refuses is refused before the append, which moves the lengths
+    const std::vector<int32_t> nodes = counts.empty() ? std::vector<int32_t>(c.batchSize, int32_t(n)) : counts;
+    int32_t longest = 0;
+    for (uint32_t b = 0; b < c.batchSize; ++b) longest = std::max(longest, kv.hostSeqLens[b] + nodes[b]);
+    scratch.push_back(pool.acquire(qBytes));
+    const GrillyBuffer rotated = scratch.back();
+    grl_tree_params t = treeParams(pool, kv, rotated.dptr, out.dptr, dtype, n, numQHeads, longest, scale, scratch);
     reservePages(pool, kv, n, counts);
     grl_append_norm_params a{};
     a.kv = kv.layout();
     a.parents = uploadInts(pool, parents, scratch);
     a.n_nodes = uploadInts(pool, counts, scratch);
-    scratch.push_back(pool.acquire(qBytes));
-    const GrillyBuffer rotated = scratch.back();
     a.k_new = kNew.dptr; a.v_new = vNew.dptr; a.q_in = q.dptr; a.q_out = rotated.dptr;
     a.q_weight = static_cast<const float*>(norm.qWeight.dptr); a.k_weight = static_cast<const float*>(norm.kWeight.dptr);
     a.eps = norm.eps; a.in_dtype = a.q_out_dtype = dtype;
     a.n_new = int(n); a.num_q_heads = int(numQHeads); a.rope = rope.spec(); a.update_lens = 1;
     a.pos_offsets = static_cast<const int32_t*>(kv.evicted.dptr);
     check(grl_kv_append_norm(pool.device().handle(), &a), "draftStep: append");
-    kv.draftNodes = counts.empty() ? std::vector<int32_t>(c.batchSize, int32_t(n)) : counts;
+    kv.draftNodes = nodes;
     for (uint32_t b = 0; b < c.batchSize; ++b) {
         kv.hostSeqLens[b] += kv.draftNodes[b];
         kv.totalAppended += uint64_t(kv.draftNodes[b]);
     }
     kv.currentLen = uint32_t(kv.hostSeqLens[0]);
-    launchTree(pool, kv, rotated.dptr, out.dptr, dtype, n, numQHeads, a.parents, a.n_nodes, scale, scratch);
+    t.parents = a.parents; t.n_nodes = a.n_nodes;
+    check(grl_tree_attention(pool.device().handle(), &t), "draftStep: attention");
 }
 
 void treeAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& kv, const GrillyBuffer& q, GrillyBuffer& out, int dtype,
@@ -606,8 +612,10 @@ void treeAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& 
     const size_t bytes = size_t(c.batchSize) * n * numQHeads * c.headDim * elemSize(dtype);
     if (q.size < bytes || out.size < bytes) throw std::runtime_error("treeAttention: buffer too small");
     cache.getOrCreate("tree-attention/" + std::to_string(c.headDim));
-    const int32_t* up = uploadInts(pool, parents, scratch);
-    launchTree(pool, kv, q.dptr, out.dptr, dtype, n, numQHeads, up, uploadInts(pool, kv.draftNodes, scratch), scale, scratch);
+    grl_tree_params t = treeParams(pool, kv, q.dptr, out.dptr, dtype, n, numQHeads, *std::max_element(kv.hostSeqLens.begin(), kv.hostSeqLens.end()), scale, scratch);
+    t.parents = uploadInts(pool, parents, scratch);
+    t.n_nodes = uploadInts(pool, kv.draftNodes, scratch);
+    check(grl_tree_attention(pool.device().handle(), &t), "treeAttention");
 }
 
 void kvCacheKeep(BufferPool& pool, PipelineCache& cache, KVCache& kv, const std::vector<std::vector<int32_t>>& paths) {

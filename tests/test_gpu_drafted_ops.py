@@ -247,3 +247,24 @@ def test_a_refused_step_gives_out_no_pages(gpu):
     for b in range(2):
         assert np.array_equal(gpu.kv_cache_decode(kv, b)["values"], np.array(rows[b]))
     gpu.destroy_kv_cache(kv)
+
+
+def test_a_step_that_the_attention_refuses_is_not_appended(gpu):
+    """What only the attention refuses comes before the append: the lengths stay, and the step that follows is that of a cache which saw no refusal."""
+    r = np.random.default_rng(12)
+    make = lambda: gpu.create_kv_cache(num_heads=2, head_dim=32, compression_ratio=1, max_cache_tokens=64, use_h2o=False, batch_size=2,  # noqa: E731
+                                       page_tokens=16, dtype="fp32")
+    q, k, v = draw(r, 2, 3, 4, 32), draw(r, 2, 3, 2, 32), draw(r, 2, 3, 2, 32)
+    kv, fresh = make(), make()
+    for cache in (kv, fresh):
+        gpu.draft_step(cache, q, k, v, None, [3, 2])
+    for bad in (dict(scale=-1.0), dict(scale=float("nan"))):
+        with pytest.raises(RuntimeError, match="scale"):
+            gpu.draft_step(kv, q, k, v, **bad)
+        assert kv.seq_lens == [3, 2]
+    gpu.kv_cache_keep(kv, [[0], [0, 1]])                         # the nodes are still those of the step before
+    gpu.kv_cache_keep(fresh, [[0], [0, 1]])
+    assert np.array_equal(gpu.draft_step(kv, q, k, v), gpu.draft_step(fresh, q, k, v))
+    assert kv.seq_lens == fresh.seq_lens == [4, 5]
+    for cache in (kv, fresh):
+        gpu.destroy_kv_cache(cache)
