@@ -3,6 +3,7 @@
 // shaders/rope.glsl:32-40 and shaders/attention-mask.glsl:18-24 (the reference ships the shaders
 // without a C++ dispatcher; these follow its op-layer conventions).
 #include <cstdint>
+#include <stdexcept>
 
 #include "grilly/buffer_pool.h"
 #include "grilly/command_batch.h"
@@ -18,21 +19,27 @@ void rope(CommandBatch& batch, BufferPool& pool, PipelineCache& cache, const flo
           RopeMode mode = RopeMode::Half, const float* cosTable = nullptr, const float* sinTable = nullptr);
 
 /// The rotation of normalised heads: the first rotaryDim elements (0: all), angles position * theta^(-2j/rotaryDim) / scaling, cosine
-/// and sine times gain.
+/// and sine times gain.  scaling and gain must be positive: the C structure reads 0 as 1.
 struct HeadRope {
     RopeMode mode = RopeMode::Interleaved;
     uint32_t rotaryDim = 0;
     float theta = 10000.0f, scaling = 1.0f, gain = 1.0f;
     grl_rope_spec spec() const {
+        if (!(scaling > 0.0f) || !(gain > 0.0f)) throw std::runtime_error("rope scaling and gain must be positive");
         grl_rope_spec s{};
         s.mode = int(mode); s.rotary_dim = int(rotaryDim); s.theta = theta; s.scaling = scaling; s.gain = gain;
         return s;
     }
 };
-/// The weights of normalised query and key heads: device float32 (headDim), or invalid buffers for ones.
+/// The weights of normalised query and key heads: device float32 (headDim), or invalid buffers for ones.  eps must be positive: the C structures
+/// read 0 as 1e-6.
 struct HeadNorm {
     GrillyBuffer qWeight, kWeight;
     float eps = 1e-6f;
+    float epsilon() const {
+        if (!(eps > 0.0f)) throw std::runtime_error("eps must be positive");
+        return eps;
+    }
 };
 
 /// Queries and keys of a layer normalised by head and rotated; q, qOut (B,S,Hq,D), k, kOut (B,S,Hkv,D) device buffers of `dtype`, k may be

@@ -394,7 +394,7 @@ static grl_qk_norm_params normParams(const GrillyBuffer& q, const GrillyBuffer& 
     p.q_weight = static_cast<const float*>(norm.qWeight.dptr); p.k_weight = static_cast<const float*>(norm.kWeight.dptr);
     p.in_dtype = p.out_dtype = dtype;
     p.batch = int(h.batch); p.seq_len = int(h.seqLen); p.num_q_heads = int(h.numQHeads); p.num_kv_heads = k.valid() ? int(h.numKvHeads) : 0;
-    p.head_dim = int(h.headDim); p.eps = norm.eps; p.rope = rope.spec();
+    p.head_dim = int(h.headDim); p.eps = norm.epsilon(); p.rope = rope.spec();
     p.positions = static_cast<const int32_t*>(positions.dptr); p.pos_base = posBase;
     return p;
 }

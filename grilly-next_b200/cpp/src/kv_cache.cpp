@@ -589,7 +589,7 @@ void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kv, const 
     a.n_nodes = uploadInts(pool, counts, scratch);
     a.k_new = kNew.dptr; a.v_new = vNew.dptr; a.q_in = q.dptr; a.q_out = rotated.dptr;
     a.q_weight = static_cast<const float*>(norm.qWeight.dptr); a.k_weight = static_cast<const float*>(norm.kWeight.dptr);
-    a.eps = norm.eps; a.in_dtype = a.q_out_dtype = dtype;
+    a.eps = norm.epsilon(); a.in_dtype = a.q_out_dtype = dtype;
     a.n_new = int(n); a.num_q_heads = int(numQHeads); a.rope = rope.spec(); a.update_lens = 1;
     a.pos_offsets = static_cast<const int32_t*>(kv.evicted.dptr);
     check(grl_kv_append_norm(pool.device().handle(), &a), "draftStep: append");

@@ -268,3 +268,14 @@ def test_a_step_that_the_attention_refuses_is_not_appended(gpu):
     assert kv.seq_lens == fresh.seq_lens == [4, 5]
     for cache in (kv, fresh):
         gpu.destroy_kv_cache(cache)
+
+
+@pytest.mark.parametrize("bad", [dict(eps=0.0), dict(eps=-1e-6), dict(rope_scaling=0.0), dict(rope_gain=0.0), dict(rope_gain=-1.0)], ids=str)
+def test_numbers_that_would_be_read_as_a_default_are_refused(gpu, bad):
+    x = np.ones((2, 3, 2, 32), np.float32)
+    kv = gpu.create_kv_cache(num_heads=2, head_dim=32, compression_ratio=1, max_cache_tokens=64, use_h2o=False, batch_size=2, page_tokens=16)
+    for call in (lambda: gpu.qk_norm_rope(x, x, **bad), lambda: gpu.qk_norm_rope_backward(x, x, x, x, **bad), lambda: gpu.draft_step(kv, x, x, x, **bad)):
+        with pytest.raises(RuntimeError, match="must be positive"):
+            call()
+    assert kv.seq_lens == [0, 0]
+    gpu.destroy_kv_cache(kv)

@@ -231,3 +231,30 @@ def test_python_operators_are_there():
     from grilly_next.backend import _bridge
     for n in ("qk_norm_rope", "qk_norm_rope_backward", "draft_step", "tree_attention", "kv_cache_keep"):
         assert hasattr(grilly_core, n) and hasattr(_bridge, n) and hasattr(grilly_next.Compute, n)
+
+
+def test_heads_refuse_what_the_c_structures_would_read_as_a_default(tmp_path):
+    """A caller of the operators who names 0 as eps, scaling or gain would get 1e-6 or 1 without a word."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "heads.cpp").write_text(r"""
+#include <cmath>
+#include <cstdio>
+#include "grilly/ops/rope.h"
+using namespace grilly::ops;
+template <typename F> static void say(F f) { try { f(); std::puts("ok"); } catch (const std::runtime_error& e) { std::puts(e.what()); } }
+int main() {
+    for (float v : {1e-30f, 1.0f, 0.0f, -1.0f, NAN}) {
+        say([&] { HeadNorm n; n.eps = v; n.epsilon(); });
+        say([&] { HeadRope r; r.scaling = v; r.spec(); });
+        say([&] { HeadRope r; r.gain = v; r.spec(); });
+    }
+}
+""")
+    cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
+    subprocess.check_call([cxx, "-std=c++17", "-I", os.path.join(root, "include"), "-I", os.path.join(root, "grilly-next_b200", "cpp", "include"),
+                           str(tmp_path / "heads.cpp"), "-o", str(tmp_path / "heads")])
+    said = subprocess.check_output([str(tmp_path / "heads")], text=True).split("\n")[:15]
+    assert said == ["ok"] * 6 + ["eps must be positive"] + ["rope scaling and gain must be positive"] * 2 + (
+        ["eps must be positive"] + ["rope scaling and gain must be positive"] * 2) * 2
