@@ -27,23 +27,26 @@ void reservePages(BufferPool& pool, KVCache& kv, uint32_t extra, const std::vect
     const auto pagesOf = [&](uint32_t b) {
         return (uint32_t(kv.hostSeqLens[b]) + (counts.empty() ? extra : uint32_t(counts[b])) + c.pageTokens - 1) / c.pageTokens;
     };
-    // looked over before any page is given out: a page given here and not uploaded would be taken for one that the device knows
+    // Looked over before any page is given out: a page given here and not uploaded would be taken for one that the device knows.  A sequence's pages
+    // are given in order, so its last entries tell, and a step that needs no page reads one a sequence.
+    const auto firstFresh = [&](uint32_t b, uint32_t need) {
+        const int32_t* row = kv.hostBlockTable.data() + size_t(b) * kv.maxPages;
+        while (need > 0 && row[need - 1] < 0) --need;
+        return need;
+    };
     uint32_t fresh = 0;
     for (uint32_t b = 0; b < c.batchSize; ++b) {
         const uint32_t need = pagesOf(b);
         if (need > kv.maxPages)
             throw std::runtime_error("kvCacheAppend: sequence would exceed max_cache_tokens (" +
                                      std::to_string(c.maxCacheTokens) + ")");
-        for (uint32_t i = 0; i < need; ++i) fresh += kv.hostBlockTable[size_t(b) * kv.maxPages + i] < 0;
+        fresh += need - firstFresh(b, need);
     }
     if (fresh > kv.numPages - kv.nextFreePage) throw std::runtime_error("kvCacheAppend: page pool exhausted");
     const bool changed = fresh > 0;
-    for (uint32_t b = 0; b < c.batchSize; ++b) {
+    for (uint32_t b = 0; b < c.batchSize && changed; ++b) {
         const uint32_t need = pagesOf(b);
-        for (uint32_t i = 0; i < need; ++i) {
-            int32_t& slot = kv.hostBlockTable[size_t(b) * kv.maxPages + i];
-            if (slot < 0) slot = int32_t(kv.nextFreePage++);
-        }
+        for (uint32_t i = firstFresh(b, need); i < need; ++i) kv.hostBlockTable[size_t(b) * kv.maxPages + i] = int32_t(kv.nextFreePage++);
     }
     if (changed) {
         // unassigned entries are uploaded as page 0; they are never read (beyond seq_lens)
