@@ -412,9 +412,10 @@ def single_stages_that_run_out(T, splits, B=24):
     dev.close()
 
 
-@pytest.mark.parametrize("T,splits", [(1, 9), (4, 6), (4, 20)])
-def test_a_reader_that_gives_up_leaves_no_copies_behind_few_rows(T, splits):
-    single_stages_that_run_out(T, splits)
+@pytest.mark.parametrize("T,splits,B", [(1, 9, 24), (4, 6, 24), (4, 20, 24), (4, 6, 2), (4, 12, 1)])
+def test_a_reader_that_gives_up_leaves_no_copies_behind_few_rows(T, splits, B):
+    """Joined behind, and in clusters where there are few sequences."""
+    single_stages_that_run_out(T, splits, B)
 
 
 @pytest.mark.parametrize("T,splits", [(8, 9), (16, 6), (20, 8), (61, 7)])
@@ -472,6 +473,62 @@ def test_page_outside_the_pool_raises_the_status_word(dev, io):
         with pytest.raises(cabi.GrlError) as e:
             attend(dev, cache, q, None, None, io=io)
         assert e.value.code == cabi.ERR_KERNEL and "page" in str(e.value)
+    cache.free()
+
+
+@pytest.mark.parametrize("fault", ["parent_forward", "parent_below", "count_high", "count_negative", "length", "length_long", "page_high", "page_negative"])
+@pytest.mark.parametrize("T,splits", [(4, 1), (4, 4), (4, 17), (8, 1), (24, 3), (40, 1), (100, 2)])
+def test_bad_numbers_in_every_tensor_core_form(dev, T, splits, fault):
+    """Few rows, the folded and the split tile, two tiles; whole, in a cluster and joined.  The kernels check every number before they use it; the rows of
+    a sequence whose numbers do not fit are 0 (with a page outside the pool they mean nothing), those of the other sequence are right."""
+    from grilly_next import cabi
+    lens = [T + 200, T + 130]
+    cache = Cache(dev, lens, 2, 128, 64, "bf16", seed=1)
+    r = np.random.default_rng(0)
+    parents, counts = [draw_parents(r, T, "tree") for _ in range(2)], [T, T]
+    q = round_bf16(r.standard_normal((2, T, 8, 128)).astype(np.float32))
+    given, table = [list(x) for x in parents], cache.table.copy()
+    if fault == "parent_forward": given[1][2] = 3
+    if fault == "parent_below": given[1][2] = -2
+    if fault == "count_high": counts[1] = T + 1
+    if fault == "count_negative": counts[1] = -1
+    if fault == "length": cache.set_lens([lens[0], T - 1])
+    if fault == "length_long": cache.set_lens([lens[0], cache.max_pages * 64 + 1])
+    if fault == "page_high": table[1, 1] = cache.num_pages
+    if fault == "page_negative": table[1, 0] = -1
+    cabi.check(dev.L.grl_memcpy_h2d(dev.h, cache.table_ptr, table.ctypes.data_as(C.c_void_p), table.nbytes))
+    p = cabi.TreeParams()
+    p.kv = cache.layout()
+    p.io_dtype, p.num_q_heads, p.n_tree, p.n_splits, p.max_seq_len = cabi.BF16, 8, T, splits, max(lens)
+    need = C.c_size_t()
+    keep = [dev.upload(to_bf16_bits(q.reshape(-1))), dev.upload(np.full(q.size, 0x5555, np.uint16)), dev.upload(np.array(given, np.int32)),
+            dev.upload(np.array(counts, np.int32))]
+    p.q, p.out, p.parents, p.n_nodes = keep
+    cabi.check(dev.L.grl_tree_workspace_bytes(dev.h, C.byref(p), C.byref(need)))
+    if need.value:
+        keep.append(dev.upload(np.full(need.value, 0xFF, np.uint8)))
+        p.workspace, p.workspace_bytes = keep[-1], need.value
+    cabi.check(dev.L.grl_tree_attention(dev.h, C.byref(p)))
+    with pytest.raises(cabi.GrlError) as e:
+        dev.sync()
+    assert e.value.code == cabi.ERR_KERNEL and "sequence 1" in str(e.value)
+    got = from_bf16_bits(dev.download(keep[1], q.shape, np.uint16))
+    if "page" not in fault:
+        assert np.all(got[1] == 0)
+    cache.rows = [x[:1] for x in cache.rows]
+    check_attention(got[:1], cache, q[:1], parents[:1], None, "bf16", False)
+    for k in keep:
+        dev.free(k)
+    cache.free()
+
+
+@pytest.mark.parametrize("T,splits,lens,counts", [(4, 5, [1500, 65, 4], [4, 2, 0]), (4, 16, [4000, 65, 4], [4, 1, 0]), (1, 8, [1030, 1, 0], [1, 1, 0]),
+                                                  (3, 3, [300, 3, 200], [3, 3, 2])])
+def test_few_rows_joined_in_a_cluster(dev, T, splits, lens, counts):
+    """Sequences without nodes, and shorter than their splits, among them."""
+    c = tree_case(T, 8, 2, 128, 32, lens, counts, kw_splits=splits)
+    got, cache, q, parents = run_tree(dev, c)
+    check_attention(got, cache, q, parents, counts, "bf16", False)
     cache.free()
 
 
