@@ -139,7 +139,8 @@ void decodeStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, 
 /// parents: empty for chains, else (B, n), a node's parent among the nodes before it or -1; counts: nodes of each sequence, empty for n each.
 /// q, out (B,n,Hq,D), kNew, vNew (B,n,Hkv,D): device buffers of `dtype`.  Keys and queries are normalised and rotated at cached tokens + depth,
 /// keys and values appended, and every node attends to the cached tokens, its ancestors and itself.  Rows of padding are written as 0.
-/// Asynchronous but for the upload of parents and counts; the buffers in `scratch` are the caller's to release behind the launch.
+/// Asynchronous, but the upload of parents and counts, where given, waits for the stream; the buffers in `scratch` are the caller's to release
+/// behind the launch.  A step that is refused leaves the lengths as they are.
 void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, const GrillyBuffer& q, const GrillyBuffer& kNew,
                      const GrillyBuffer& vNew, GrillyBuffer& out, int dtype, uint32_t n, uint32_t numQHeads,
                      const std::vector<int32_t>& parents, const std::vector<int32_t>& counts, const HeadNorm& norm, const HeadRope& rope,
@@ -147,7 +148,9 @@ void draftStepDevice(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, c
 /// The attention of the last draftStep's nodes over the cache for queries that are rotated already (another head count, another scale).
 void treeAttentionDevice(BufferPool& pool, PipelineCache& cache, const KVCache& kvCache, const GrillyBuffer& q, GrillyBuffer& out, int dtype,
                          uint32_t n, uint32_t numQHeads, const std::vector<int32_t>& parents, float scale, std::vector<GrillyBuffer>& scratch);
-/// Keeps the accepted path of the last draftStep, ascending node numbers of each sequence, and drops its other nodes.
+/// Keeps the accepted path of the last draftStep, ascending node numbers of each sequence, and drops its other nodes.  The tree is not known here
+/// any more: any ascending choice is kept as given, and its keys stay rotated to cached tokens + depth, so that only a path from the cached
+/// tokens leaves keys at consecutive positions.
 void kvCacheKeep(BufferPool& pool, PipelineCache& cache, KVCache& kvCache, const std::vector<std::vector<int32_t>>& paths);
 
 // Eviction family of the reference (kv_cache.h:186-229) on the paged cache.

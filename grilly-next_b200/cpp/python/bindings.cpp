@@ -812,7 +812,8 @@ PYBIND11_MODULE(grilly_core, m) {
         "RoPE(q,k) at the current position, append k/v, attend over the cache");
 
     // ---- normalised heads and steps of several drafted tokens.  Host arrays are uploaded (rounded to bf16 where dtype is "bf16") and come
-    // back as float32; DeviceTensors of one dtype stay on the device and nothing is waited for.
+    // back as float32; DeviceTensors of one dtype stay on the device, and their calls wait for the stream only where they bring a host
+    // array (positions, parents, n_nodes, paths).
     struct Operand {
         TensorPtr t;
         bool host = false;
@@ -1016,7 +1017,8 @@ PYBIND11_MODULE(grilly_core, m) {
         "kv_cache_keep",
         [](ContextPtr ctx, ops::KVCache& kv, const std::vector<std::vector<int32_t>>& paths) { ops::kvCacheKeep(ctx->pool, ctx->cache, kv, paths); },
         py::arg("device"), py::arg("kv_cache"), py::arg("paths"),
-        "Keep the accepted nodes of the last draft_step (ascending node numbers of each sequence) and drop the others");
+        "Keep the accepted nodes of the last draft_step (ascending node numbers of each sequence, taken as given: keys keep the positions that "
+        "their depths gave them) and drop the others");
 
     // ---- KV-sharded decode across processes (one per GPU): NCCL behind the C ABI
     struct PyShardGroup {

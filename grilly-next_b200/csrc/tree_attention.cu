@@ -22,7 +22,7 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
 // grid (splits, Hkv x chunks of rows, B), the fours of rows shared out evenly.  A tile of 32 keys lies in shared memory as float32; a
 // lane forms the scores of one key with the four rows of its warp, then the warp's lanes share out the columns of the output: a key, or a value,
 // that has been read from shared memory meets four rows.  The next tile is on its way to registers meanwhile.
-// Bound by shared-memory reads where there are many rows (8 x 8 heads x 4000 tokens, 64 rows of 128: 468 us, 18 TFLOP/s), by the chain of length, page
+// Bound by shared-memory reads where there are many rows (8 x 8 heads x 4000 tokens, 64 rows of 128: 468 us, 18 TFLOP/s, 553 over a bf16 cache), by the chain of length, page
 // and tile where there are few.  us, a row a warp / four: 5 x 2 heads x 777 tokens, 33 rows of 64 24.0 / 18.5; one row, 1 x 8 x 4000, 108 with a warp's
 // loads to a CTA, 26 with eight.
 template <typename TIO, typename TC, int D>

@@ -6,7 +6,9 @@
 // by TMA (boxes of 64 columns, 128-byte swizzle) into a ring; four compute warps take 16 tokens of each stage, with the rows as
 // an operand of mma.sync m16n8k16, and a running maximum and sum of their own for every row.  Two CTAs an SM.  The warps' sums meet in
 // shared memory, those of splits in the shared memory of a cluster where the splits of a head are one, else in tree_join_kernel.
-// Measured, 16 rows: 32 x 8 heads x 4096 tokens 82 us (6.5 TB/s), 4 x 8 x 4096 18.5, 1 x 8 x 1001 9.8, 1 x 8 x 300 8.8.
+// Measured, 16 rows: 32 x 8 heads x 4096 tokens 80 to 82 us (6.6 TB/s), 1 x 8 x 131072 86 (6.2 TB/s); 4 x 8 x 4096 18.5, 1 x 8 x 1001 9.8, 1 x 8 x 300 8.8,
+// and 14.9, 8.6, 7.7 where call follows call and the rows are in L2.
+// P is rounded to bf16 for its product with V, half a step of each probability; maxima, sums and O are float32.
 // The predicate, and the cleaning of what lies past a sequence's end, concern the last stages only, as in tree_sm100.cu.
 #include <cuda.h>
 

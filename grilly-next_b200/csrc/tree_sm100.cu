@@ -6,6 +6,8 @@
 //   warps 0, 2   one elected lane each issues tcgen05.mma:  S = Q K^T (64 keys) into TMEM,  O += P V  with P from TMEM
 //   warps 4-7 / 8-11   softmax: a thread a row; S from TMEM, running maximum and sum in the exp2 domain, P back as bf16; the accumulator is
 //                scaled only where a maximum grew by more than 2^8
+// P is rounded to bf16, the type of V, since a product has operands of one type; each probability is off by half a step at most, 2^-8 of it, and an
+// output by that of sum p |v|.  Scores, maxima, the sum (of the unrounded exponentials) and O are float32.
 // The two chains of products and softmax (t = 0, 1) are
 //   PAIR    two row tiles over the same stages, where there are more than 128 rows: a stage crosses shared memory once for 256 rows
 //   SPLIT   the even and the odd stages of one row tile, joined in the epilogue
@@ -17,10 +19,12 @@
 // that are no finite number; rows that see such an element get it added behind the epilogue, so that it reaches nobody else.  Among the
 // cached tokens, which all rows see, infinities stay where they are; only FOLD, whose zeros in P meet them too, puts right what came out as NaN.
 //
-// Measured: 32 x 8 heads x 4096 tokens, 64 rows 106 us (5.2 TB/s; HBM, and the ends of CTAs that have an SM to themselves), 1 x 8 x 131072, 244 rows
-// 147 to 163 us (800 to 900 TFLOP/s; tensor pipe 48 % busy, exponentials 53 %, the chain between them), 1 x 8 x 1001, 20 rows 10.6 us (latency).
+// Measured, from GPU to GPU: 32 x 8 heads x 4096 tokens, 64 rows 103 to 120 us (5.2 to 4.5 TB/s; HBM, and the ends of CTAs that have an SM to
+// themselves), 1 x 8 x 131072, 244 rows 144 to 175 us (910 to 750 TFLOP/s; tensor pipe 48 % busy, exponentials 53 %, the chain between them),
+// 1 x 8 x 1001, 20 rows 10.7 us (latency).
 //
-// Every mbarrier wait is bounded; on expiry the CTA records an error, drains its copies and returns.
+// Every mbarrier wait is bounded; on expiry the CTA records an error, and leaves when its copies and products in flight have ended, whichever
+// warp's wait it was.
 #include <cuda.h>
 
 #include "sm100_ptx.cuh"
@@ -726,7 +730,7 @@ int tree_join_launch(grl_device* dev, const TreeArgs& a, int rows) { return tree
 // The fewest stages of a split.  us, split into 1 / 2 / 3 / 4: 4 x 8 heads x 700 tokens, 124 rows 15.2 / 15.9 / 15.2 / 15.0, 64 rows 14.2 / 15.7 /
 // 13.3 / 13.5; 1500 tokens, 64 rows 21.4 / 18.1 / - / 17.7.  More heads than SMs are not split: 20 x 8 x 4096, 124 rows 98.7 / 106 / 110, 64 rows
 // 106 / 102 / 105, 20 x 8 x 1024 40.4 / 49.3 / 57.2, 24 x 8 x 4096 101 / 121.  Equal shares of all stages for every CTA, heads cut where they fall, are no
-// faster anywhere: 32 x 8 x 4096, 64 rows 118 for 106, 4 x 8 x 1500 27.1 for 17.7, 1 x 8 x 131072 of 244 rows 172 for 163.
+// faster anywhere: 4 x 8 x 1500 27.1 for 17.7, and in turn on one GPU 32 x 8 x 4096, 64 rows 130 for 120, 1 x 8 x 131072 of 244 rows 190 for 174.
 constexpr int kSplitStages = 4;
 // asked: the caller's number of splits, or 0.
 TreeTensorPlan tree_sm100_plan(const grl_device* dev, int B, int Hkv, int R, int D, int longest, int asked) {

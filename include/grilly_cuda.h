@@ -366,7 +366,8 @@ int grl_kv_append_norm(grl_device* dev, const grl_append_norm_params* p);
  * are its last n_nodes[b] rows.  Rows of out past a sequence's nodes are written as 0.  head_dim 32, 64, 128 or 256.  bf16 queries over a bf16
  * cache (head_dim 64 or 128, pages of 64, 32 or 16 tokens) run on the tensor cores, where probabilities are rounded to bf16;
  * everything else is computed in float32.
- * What a row must not see does not touch its result: rows past a sequence's end and nodes of other branches may hold anything. */
+ * What a row must not see does not touch its result: rows past a sequence's end and nodes of other branches may hold anything.  A row whose scores
+ * hold a NaN, or are -inf throughout, is NaN. */
 typedef struct {
     grl_kv_layout kv;
     const void* q;
@@ -386,7 +387,8 @@ typedef struct {
 int grl_tree_workspace_bytes(grl_device* dev, const grl_tree_params* p, size_t* bytes);
 int grl_tree_attention(grl_device* dev, const grl_tree_params* p);
 
-/* path (B,max_path): the accepted nodes of every sequence, ascending, the first n_path[b] entries (at most n_nodes[b], 0 keeps none).  Row
+/* path (B,max_path): the accepted nodes of every sequence, ascending, the first n_path[b] entries (at most n_nodes[b], 0 keeps none).  That they are
+ * a path of the tree is the caller's to see to: keys are moved as they are, rotated to the positions that their depths gave them.  Row
  * seq_lens[b] - n_nodes[b] + path[b][i] moves to seq_lens[b] - n_nodes[b] + i, keys and values, and the length becomes
  * seq_lens[b] - n_nodes[b] + n_path[b].  It is written to lens_out, or to kv.seq_lens where that is NULL.  meta: optional, the
  * eviction metadata of the cache: the entries of the accepted nodes move with them, those of the dropped ones are cleared. */
